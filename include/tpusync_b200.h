@@ -649,6 +649,108 @@ TS_API int ts_kv_relayout(int device, const uint64_t* d_src_bases,
                    int64_t dst_pages, int* d_err, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Paged KV cache operators: the write that fills a layer's pages and the    */
+/* attention that reads them (no reference counterpart: the reference moves  */
+/* the pages that its engines' kernels write and read).                      */
+/* ------------------------------------------------------------------------ */
+
+/* One layer's K and V storages of pages of `block_tokens` tokens x `heads`
+ * heads x `head_dim` elements.  Element e of head h of token t of page p lies
+ * at k_ptr + (p*k_page_stride + t*k_token_stride + h*k_head_stride + e)
+ * elements (same for V): token-major pages, head-major pages and views of a
+ * joint [pages, 2, ...] cache are all strides.  Strides count elements. */
+typedef struct ts_paged_kv {
+  uint64_t k_ptr;
+  uint64_t v_ptr;
+  int64_t pages;
+  int64_t block_tokens;
+  int64_t heads;
+  int64_t head_dim;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  int32_t dtype; /* TS_DTYPE_BF16 or TS_DTYPE_F16 */
+  int32_t pad_;
+} ts_paged_kv;
+
+/* New tokens of ts_kv_append.  All pointers are device addresses; strides
+ * count elements, the last dimension is contiguous. */
+typedef struct ts_kv_append_args {
+  uint64_t k, v;       /* [tokens, heads, head_dim], the storages' dtype */
+  uint64_t q;          /* [tokens, q_heads, head_dim], or 0: no queries */
+  uint64_t q_out;      /* [tokens, q_heads, head_dim]; may be q itself */
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t q_token_stride, q_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride;
+  int64_t tokens, q_heads;
+  uint64_t slots;      /* int64 [tokens]: page * block_tokens + offset, < 0: padding */
+  uint64_t positions;  /* int64 [tokens]; read only when cos_sin is given */
+  uint64_t cos_sin;    /* float [max_position, rotary]: cosines, then sines; 0: no rotation */
+  int64_t max_position, cos_sin_stride;
+  int64_t rotary;      /* rotated elements of a head (even, <= head_dim) */
+  uint64_t q_weight, k_weight; /* [head_dim] norm weights, or 0: no norm */
+  int32_t weight_dtype;        /* the storages' dtype or TS_DTYPE_F32 */
+  float eps;
+  int32_t interleaved; /* pairs (2i, 2i+1) instead of (i, i + rotary/2) */
+  int32_t zero_padding; /* q_out rows of padding tokens: 1 = zeros, 0 = left as they were */
+} ts_kv_append_args;
+
+/* For every token t with a slot >= 0, with x -> rot(norm(x)) the optional
+ * head norm w * x / sqrt(mean(x^2) + eps) and the optional rotation of pairs
+ * (a, b) -> (a c - b s, b c + a s) by row positions[t] of cos_sin:
+ *   K[slots[t]] = rot(norm_k(k[t])), V[slots[t]] = v[t],
+ *   q_out[t] = rot(norm_q(q[t])).
+ * 32-bit arithmetic, one rounding at the end.  The slots of one call are
+ * distinct; of tokens that name the same slot, the pieces of any may stay.
+ * A slot past the storage or a position outside the table writes nothing for
+ * that token (its q_out row counts as padding) and sets *err_flag (device or
+ * host-mapped int, may be NULL) to 1.  New tokens must not overlap the pages. */
+TS_API int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_append_args* args,
+                        int* err_flag, void* stream);
+
+/* Queries of ts_paged_attention (device addresses, strides in elements). */
+typedef struct ts_attention_args {
+  uint64_t q;           /* [batch, new_tokens, q_heads, head_dim], the storages' dtype */
+  uint64_t out;         /* the same shape, contiguous */
+  uint64_t lse;         /* float [batch, new_tokens, q_heads], or 0 */
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  int64_t batch, new_tokens, q_heads;
+  uint64_t block_table; /* int32 [batch, max_blocks] */
+  int64_t block_table_stride, max_blocks;
+  uint64_t seq_lens;    /* int32 [batch] */
+  uint64_t prefix_table; /* int32 [prefix_blocks]: pages every sequence sees first */
+  int64_t prefix_blocks;
+  int64_t prefix_len;
+  uint64_t prefix_len_dev; /* int32, or 0; the shared tokens are the smaller of both */
+  float scale;          /* scores are scale * q.k; finite and > 0 */
+  int32_t pad_;
+} ts_attention_args;
+
+/* Bytes of device workspace ts_paged_attention needs for these shapes (the
+ * pointers of `args` are not read).  A workspace belongs to one call at a
+ * time; nothing in it outlives the call. */
+TS_API int ts_paged_attention_workspace(int device, const ts_paged_kv* kv,
+                                        const ts_attention_args* args, uint64_t* bytes);
+
+/* Attention of each sequence's last `new_tokens` tokens over its pages:
+ * sequence b holds seq_lens[b] tokens in the pages block_table[b]; query j
+ * sees the first seq_lens[b] - new_tokens + 1 + j of them (causal), after the
+ * first prefix_len tokens of the pages prefix_table, which all sequences
+ * share (prefix_blocks = 0: none).  Query head h reads KV head
+ * h / (q_heads / heads).
+ *   out = sum_i exp(x_i) v_i / sum_i exp(x_i), x_i = scale * q . k_i,
+ *   lse = log sum_i exp(x_i);
+ * a query that sees nothing gets zeros and -inf.  Softmax statistics and
+ * values are held in 32 bits, probabilities rounded to the storages' dtype for
+ * the matrix products.  Tokens of a table entry outside [0, pages) are left
+ * out, lengths are cut to what their table holds, and either sets *err_flag
+ * (device or host-mapped int, may be NULL) to 1.  What lies in pages past a
+ * length is never used (it may be NaN).  head_dim is 64 or 128. */
+TS_API int ts_paged_attention(int device, const ts_paged_kv* kv, const ts_attention_args* args,
+                              void* workspace, uint64_t workspace_bytes, int* err_flag,
+                              void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Pinned host tier.                                                         */
 /* ------------------------------------------------------------------------ */
 

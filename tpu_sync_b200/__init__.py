@@ -3,8 +3,10 @@
 KV block extract/insert between paged HBM storages and a block-major
 staging layout, the pinned host tier offload/reload built on it (with the
 tier-2 prefix cache and its crash-persistent metadata), the prefill -> decode
-KV hand-offs (relayout, pool reshard plans, the managers' pull protocol), and
-the weight-sync reshard executor.  Compute runs in hand-written sm_100a
+KV hand-offs (relayout, pool reshard plans, the managers' pull protocol), the
+paged cache operators an engine runs between them (append with head norms and
+rotation, attention over pages and shared prefixes), and the weight-sync
+reshard executor.  Compute runs in hand-written sm_100a
 kernels behind the C ABI of ``include/tpusync_b200.h``; this package is the
 Python surface over it, with the reference's class names.
 """

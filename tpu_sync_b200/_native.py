@@ -96,6 +96,44 @@ class PageGeometry(ctypes.Structure):
               ("pad_", ctypes.c_int32)]
 
 
+class PagedKvC(ctypes.Structure):
+  _fields_ = [("k_ptr", ctypes.c_uint64), ("v_ptr", ctypes.c_uint64),
+              ("pages", ctypes.c_int64), ("block_tokens", ctypes.c_int64),
+              ("heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+              ("k_page_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64),
+              ("k_head_stride", ctypes.c_int64), ("v_page_stride", ctypes.c_int64),
+              ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+              ("dtype", ctypes.c_int32), ("pad_", ctypes.c_int32)]
+
+
+class KvAppendArgs(ctypes.Structure):
+  _fields_ = [("k", ctypes.c_uint64), ("v", ctypes.c_uint64), ("q", ctypes.c_uint64),
+              ("q_out", ctypes.c_uint64), ("k_token_stride", ctypes.c_int64),
+              ("k_head_stride", ctypes.c_int64), ("v_token_stride", ctypes.c_int64),
+              ("v_head_stride", ctypes.c_int64), ("q_token_stride", ctypes.c_int64),
+              ("q_head_stride", ctypes.c_int64), ("q_out_token_stride", ctypes.c_int64),
+              ("q_out_head_stride", ctypes.c_int64), ("tokens", ctypes.c_int64),
+              ("q_heads", ctypes.c_int64), ("slots", ctypes.c_uint64),
+              ("positions", ctypes.c_uint64), ("cos_sin", ctypes.c_uint64),
+              ("max_position", ctypes.c_int64), ("cos_sin_stride", ctypes.c_int64),
+              ("rotary", ctypes.c_int64), ("q_weight", ctypes.c_uint64),
+              ("k_weight", ctypes.c_uint64), ("weight_dtype", ctypes.c_int32),
+              ("eps", ctypes.c_float), ("interleaved", ctypes.c_int32),
+              ("zero_padding", ctypes.c_int32)]
+
+
+class AttentionArgs(ctypes.Structure):
+  _fields_ = [("q", ctypes.c_uint64), ("out", ctypes.c_uint64), ("lse", ctypes.c_uint64),
+              ("q_batch_stride", ctypes.c_int64), ("q_token_stride", ctypes.c_int64),
+              ("q_head_stride", ctypes.c_int64), ("batch", ctypes.c_int64),
+              ("new_tokens", ctypes.c_int64), ("q_heads", ctypes.c_int64),
+              ("block_table", ctypes.c_uint64), ("block_table_stride", ctypes.c_int64),
+              ("max_blocks", ctypes.c_int64), ("seq_lens", ctypes.c_uint64),
+              ("prefix_table", ctypes.c_uint64), ("prefix_blocks", ctypes.c_int64),
+              ("prefix_len", ctypes.c_int64), ("prefix_len_dev", ctypes.c_uint64),
+              ("scale", ctypes.c_float), ("pad_", ctypes.c_int32)]
+
+
 class StorageDesc(ctypes.Structure):
   _fields_ = [("dev_ptr", ctypes.c_uint64), ("nbytes", ctypes.c_uint64),
               ("dim0", ctypes.c_int64), ("device", ctypes.c_int32),
@@ -292,6 +330,13 @@ _SIGS = {
     "ts_ipc_open": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.POINTER(_V)]),
     "ts_ipc_close": (ctypes.c_int, [ctypes.c_int, _V]),
     "ts_ipc_export": (ctypes.c_int, [_V, ctypes.c_char_p, c_u64_p]),
+    "ts_kv_append": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(PagedKvC),
+                                    ctypes.POINTER(KvAppendArgs), _V, _V]),
+    "ts_paged_attention_workspace": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(PagedKvC),
+                                                    ctypes.POINTER(AttentionArgs), c_u64_p]),
+    "ts_paged_attention": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(PagedKvC),
+                                          ctypes.POINTER(AttentionArgs), _V, ctypes.c_uint64,
+                                          _V, _V]),
     "ts_kv_relayout": (ctypes.c_int, [ctypes.c_int, _V, _V, ctypes.c_int,
                                       PageGeometry, PageGeometry, _V, ctypes.c_int64,
                                       _V, ctypes.c_int64, ctypes.c_int64,

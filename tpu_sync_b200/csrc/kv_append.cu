@@ -1,0 +1,249 @@
+// Append of new tokens to a paged KV cache: head norms of queries and keys,
+// the position rotation and the scatter of keys and values into their pages,
+// in one pass over the projections' output.
+//
+// Per token t (slot, position from device arrays) and head vector x:
+//   x' = w * x / sqrt(mean(x^2) + eps)            (queries and keys, optional)
+//   (a, b) -> (a c - b s, b c + a s)              (pairs of the first `rotary`
+//                                                  elements, optional)
+// and the result goes to q_out, or to page slot / block_tokens at offset
+// slot % block_tokens.  Everything is read once and written once with a
+// handful of operations per element: bound by HBM for prompts, by one chain of
+// dependent loads (position -> table row) for decode steps.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <utility>
+
+#include "paged_kv.h"
+#include "ts_internal.h"
+
+namespace tsb {
+namespace {
+
+struct AppendParams {
+  ts_paged_kv kv;
+  ts_kv_append_args a;
+  int* err;
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+
+// Token t's slot and position; false (and the flag set for a bad one) when
+// nothing of the token is to be written.
+__device__ __forceinline__ bool token_place(const AppendParams& p, int64_t t, bool rot,
+                                            int64_t* page, int64_t* off, int64_t* pos) {
+  const int64_t slot = reinterpret_cast<const int64_t*>(p.a.slots)[t];
+  *pos = rot ? reinterpret_cast<const int64_t*>(p.a.positions)[t] : 0;
+  if (slot < 0) return false;
+  const int64_t pg = slot / p.kv.block_tokens;
+  if (pg >= p.kv.pages || (rot && (*pos < 0 || *pos >= p.a.max_position))) {
+    if (p.err != nullptr) *reinterpret_cast<volatile int*>(p.err) = 1;
+    return false;
+  }
+  *page = pg;
+  *off = slot - pg * p.kv.block_tokens;
+  return true;
+}
+
+template <typename T>
+__device__ __forceinline__ float weight_at(uint64_t w, int f32, int e) {
+  return f32 ? reinterpret_cast<const float*>(w)[e] : to_f32<T>(reinterpret_cast<const T*>(w)[e]);
+}
+
+// Any head size, alignment and stride: a warp per (token, head), a lane per
+// pair.  Serves what the vector kernel's rule leaves out.
+template <typename T>
+__global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__ AppendParams p) {
+  const int lane = threadIdx.x & 31;
+  const int hq = p.a.q != 0 ? int(p.a.q_heads) : 0;
+  const int hk = int(p.kv.heads);
+  const int d = int(p.kv.head_dim);
+  const bool rot = p.a.cos_sin != 0;
+  const int64_t units = p.a.tokens * (hq + 2 * hk);
+  for (int64_t u = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); u < units;
+       u += int64_t(gridDim.x) * 8) {
+    const int64_t t = u / (hq + 2 * hk);
+    const int h = int(u - t * (hq + 2 * hk));
+    int64_t page = 0, off = 0, pos = 0;
+    const bool live = token_place(p, t, rot, &page, &off, &pos);
+    const T* src;
+    T* dst;
+    uint64_t w = 0;
+    int half = rot ? int(p.a.rotary) / 2 : 0;
+    if (h < hq) {
+      src = reinterpret_cast<const T*>(p.a.q) + t * p.a.q_token_stride + h * p.a.q_head_stride;
+      dst = reinterpret_cast<T*>(p.a.q_out) + t * p.a.q_out_token_stride +
+            h * p.a.q_out_head_stride;
+      w = p.a.q_weight;
+      if (!live) {
+        if (p.a.zero_padding)
+          for (int e = lane; e < d; e += 32) dst[e] = from_f32<T>(0.f);
+        continue;
+      }
+    } else if (!live) {
+      continue;
+    } else if (h < hq + hk) {
+      const int kh = h - hq;
+      src = reinterpret_cast<const T*>(p.a.k) + t * p.a.k_token_stride + kh * p.a.k_head_stride;
+      dst = reinterpret_cast<T*>(p.kv.k_ptr) + page * p.kv.k_page_stride +
+            off * p.kv.k_token_stride + kh * p.kv.k_head_stride;
+      w = p.a.k_weight;
+    } else {
+      const int vh = h - hq - hk;
+      src = reinterpret_cast<const T*>(p.a.v) + t * p.a.v_token_stride + vh * p.a.v_head_stride;
+      dst = reinterpret_cast<T*>(p.kv.v_ptr) + page * p.kv.v_page_stride +
+            off * p.kv.v_token_stride + vh * p.kv.v_head_stride;
+      for (int e = lane; e < d; e += 32) dst[e] = src[e];
+      continue;
+    }
+    float inv = 1.f;
+    if (w != 0) {
+      float ss = 0.f;
+      for (int e = lane; e < d; e += 32) {
+        const float x = to_f32<T>(src[e]);
+        ss += x * x;
+      }
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) ss += __shfl_xor_sync(~0u, ss, m);
+      inv = rsqrtf(ss / float(d) + p.a.eps);
+    }
+    __syncwarp();  // q_out may be q: every lane has read the head before any writes it
+    const float* cs = reinterpret_cast<const float*>(p.a.cos_sin) + pos * p.a.cos_sin_stride;
+    for (int i = lane; i < half; i += 32) {
+      const int ia = p.a.interleaved ? 2 * i : i, ib = p.a.interleaved ? 2 * i + 1 : i + half;
+      float a = to_f32<T>(src[ia]) * inv, b = to_f32<T>(src[ib]) * inv;
+      if (w != 0) {
+        a *= weight_at<T>(w, p.a.weight_dtype == TS_DTYPE_F32, ia);
+        b *= weight_at<T>(w, p.a.weight_dtype == TS_DTYPE_F32, ib);
+      }
+      const float c = cs[i], s = cs[i + half];
+      dst[ia] = from_f32<T>(a * c - b * s);
+      dst[ib] = from_f32<T>(b * c + a * s);
+    }
+    for (int e = 2 * half + lane; e < d; e += 32) {
+      float x = to_f32<T>(src[e]) * inv;
+      if (w != 0) x *= weight_at<T>(w, p.a.weight_dtype == TS_DTYPE_F32, e);
+      dst[e] = from_f32<T>(x);
+    }
+  }
+}
+
+template <typename T>
+int launch_append(const AppendParams& p, int device, cudaStream_t s) {
+  const int64_t heads = (p.a.q != 0 ? p.a.q_heads : 0) + 2 * p.kv.heads;
+  const int64_t ctas = (p.a.tokens * heads + 7) / 8;
+  const int64_t cap = int64_t(sm_count(device)) * 64;
+  append_any_kernel<T><<<int(std::min(ctas, cap)), 256, 0, s>>>(p);
+  TS_CUDA_RET(cudaGetLastError(), "kv append launch");
+  return TS_OK;
+}
+
+}  // namespace
+
+int check_paged_kv(const ts_paged_kv* kv) {
+  if (!kv) return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  if (kv->dtype != TS_DTYPE_BF16 && kv->dtype != TS_DTYPE_F16)
+    return set_error(TS_UNIMPLEMENTED, "pages must be bf16 or fp16");
+  if (kv->pages < 0 || kv->block_tokens <= 0 || kv->heads <= 0 || kv->head_dim <= 0)
+    return set_error(TS_INVALID_ARGUMENT, "page geometry needs positive sizes");
+  if (kv->pages > INT32_MAX || kv->block_tokens > INT32_MAX || kv->heads > 65535 ||
+      kv->head_dim > 65535)
+    return set_error(TS_INVALID_ARGUMENT, "page geometry too large");
+  if (kv->pages > 0 && (!kv->k_ptr || !kv->v_ptr))
+    return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  // no element of the pages at two indexes
+  for (int i = 0; i < 2; ++i) {
+    std::pair<int64_t, int64_t> dim[3] = {
+        {i ? kv->v_page_stride : kv->k_page_stride, kv->pages},
+        {i ? kv->v_token_stride : kv->k_token_stride, kv->block_tokens},
+        {i ? kv->v_head_stride : kv->k_head_stride, kv->heads}};
+    std::sort(dim, dim + 3);
+    int64_t span = kv->head_dim;
+    for (const auto& x : dim) {
+      if (x.second <= 1) continue;
+      if (x.first < span) return set_error(TS_INVALID_ARGUMENT, "page strides overlap");
+      span += (x.second - 1) * x.first;
+    }
+  }
+  return TS_OK;
+}
+
+}  // namespace tsb
+
+using tsb::set_error;
+
+extern "C" int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_append_args* args,
+                            int* err_flag, void* stream) {
+  tsb::clear_error();
+  if (int rc = tsb::check_paged_kv(kv)) return rc;
+  if (!args) return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  const ts_kv_append_args& a = *args;
+  if (a.tokens < 0 || a.tokens > INT32_MAX || a.q_heads < 0 || a.q_heads > 65535)
+    return set_error(TS_INVALID_ARGUMENT, "token or head count out of range");
+  if (a.tokens == 0) return TS_OK;
+  if (!a.k || !a.v || !a.slots || (a.q && (!a.q_out || a.q_heads == 0)) ||
+      (a.cos_sin && !a.positions))
+    return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  if (a.cos_sin && (a.rotary <= 0 || a.rotary % 2 != 0 || a.rotary > kv->head_dim))
+    return set_error(TS_INVALID_ARGUMENT, "rotary must be even and at most head_dim");
+  if (a.cos_sin && (a.max_position < 0 || a.cos_sin_stride < a.rotary))
+    return set_error(TS_INVALID_ARGUMENT, "rotation table rows overlap");
+  if ((a.q_weight || a.k_weight) && a.weight_dtype != kv->dtype &&
+      a.weight_dtype != TS_DTYPE_F32)
+    return set_error(TS_INVALID_ARGUMENT, "norm weights must be float32 or the pages' dtype");
+  if ((a.q_weight || a.k_weight) && !(a.eps >= 0.f))
+    return set_error(TS_INVALID_ARGUMENT, "eps must be >= 0");
+  if (a.k_token_stride < 0 || a.k_head_stride < 0 || a.v_token_stride < 0 ||
+      a.v_head_stride < 0 || (a.q && (a.q_token_stride < 0 || a.q_head_stride < 0)))
+    return set_error(TS_INVALID_ARGUMENT, "strides must be non-negative");
+  const int64_t d = kv->head_dim;
+  const tsb::Extent ek = tsb::extent(a.k, a.tokens, a.k_token_stride, kv->heads,
+                                     a.k_head_stride, 1, 0, d);
+  const tsb::Extent ev = tsb::extent(a.v, a.tokens, a.v_token_stride, kv->heads,
+                                     a.v_head_stride, 1, 0, d);
+  tsb::Extent eq{0, 0}, eo{0, 0};
+  if (a.q) {
+    eq = tsb::extent(a.q, a.tokens, a.q_token_stride, a.q_heads, a.q_head_stride, 1, 0, d);
+    eo = tsb::extent(a.q_out, a.tokens, a.q_out_token_stride, a.q_heads, a.q_out_head_stride, 1,
+                     0, d);
+    const bool rows = a.q_out_token_stride >= (a.q_heads - 1) * a.q_out_head_stride + d &&
+                      a.q_out_head_stride >= d;
+    const bool cols = a.q_out_head_stride >= (a.tokens - 1) * a.q_out_token_stride + d &&
+                      a.q_out_token_stride >= d;
+    if (!(rows || cols || (a.tokens == 1 && a.q_out_head_stride >= d) ||
+          (a.q_heads == 1 && a.q_out_token_stride >= d) || (a.tokens == 1 && a.q_heads == 1)))
+      return set_error(TS_INVALID_ARGUMENT, "q_out strides overlap");
+    const bool in_place = a.q == a.q_out && a.q_token_stride == a.q_out_token_stride &&
+                          a.q_head_stride == a.q_out_head_stride;
+    // Projections in one buffer interleave rows: q_out inside that buffer is
+    // told from an overlap only when it is q itself.
+    if (!in_place && (eo.meets(eq) || eo.meets(ek) || eo.meets(ev)))
+      return set_error(TS_INVALID_ARGUMENT, "q_out must be q itself or apart from the new tokens");
+  }
+  for (int i = 0; i < 2; ++i) {
+    const tsb::Extent e = tsb::pages_extent(*kv, i == 1);
+    if (e.meets(ek) || e.meets(ev) || e.meets(eq) || e.meets(eo))
+      return set_error(TS_INVALID_ARGUMENT, "new tokens overlap the pages");
+  }
+  tsb::DeviceGuard g(device);
+  tsb::AppendParams p{*kv, a, err_flag};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return kv->dtype == TS_DTYPE_BF16 ? tsb::launch_append<__nv_bfloat16>(p, device, s)
+                                    : tsb::launch_append<__half>(p, device, s);
+}

@@ -1,0 +1,835 @@
+// Attention over a paged KV cache: each sequence's last tokens against its own
+// pages, and, for a batch that continues one cached prefix, against the shared
+// pages, which are read once for all sequences.
+//
+// For a query row q and the keys it sees, x_i = scale * q . k_i,
+//   m = max x_i, l = sum exp(x_i - m), acc = sum exp(x_i - m) v_i, out = acc / l.
+// Disjoint key ranges join exactly: with M = max(m1, m2),
+//   l = l1 exp(m1 - M) + l2 exp(m2 - M), the same for acc.
+// So a key range can be cut anywhere, and the cuts are chosen for balance:
+//
+//   walk_kernel   every CTA takes an equal, contiguous share of all 64-token
+//                 tiles of the batch (ordered by sequence, row tile, KV head),
+//                 computed on the device from the lengths: no host copy of the
+//                 lengths, no empty CTAs for short sequences, the same code
+//                 for one long sequence and for many short ones.  A share that
+//                 cuts an item in two leaves a partial (m, l, acc).
+//   join_kernel   joins partials per query row, in a fixed order.
+//
+// A warp owns 16 tokens of each tile (its own cp.async ring, its own softmax
+// statistics and accumulator), so the loop over keys has no CTA barrier; the
+// four warps are joined once per item.  All query heads of a KV head, and all
+// new tokens, are rows of one mma tile: K and V are read once per KV head.
+// Decode is bound by reading K and V from HBM.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "paged_kv.h"
+#include "ts_internal.h"
+
+namespace tsb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kWarpTokens = 16;
+constexpr int kTile = kWarps * kWarpTokens;  // tokens of a tile
+constexpr int kStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct WalkParams {
+  ts_paged_kv kv;
+  ts_attention_args a;
+  float scale_log2;   // scale * log2(e): softmax in powers of two
+  int group;          // query heads per KV head
+  int rows_own;       // rows of a sequence and KV head: new_tokens * group
+  int row_tiles_own;  // tiles of 16 * MT rows of them
+  int rows_pre;       // rows of the shared prefix and a KV head: all sequences'
+  int row_tiles_pre;  // 0: no prefix in this kernel
+  float* slots_acc;   // [ctas][2][16 * MT][D]: partials of items cut between CTAs
+  float* slots_ml;    // [ctas][2][16 * MT][2]
+  float* own_acc;     // [rows][D]: own parts of a batch that has a prefix
+  float* own_ml;      // [rows][2]
+  float* pre_acc;     // [rows][D]: whole prefix parts
+  float* pre_ml;
+  int* err;
+  int ctas;
+};
+
+__device__ __forceinline__ void raise(int* err) {
+  if (err != nullptr) *reinterpret_cast<volatile int*>(err) = 1;
+}
+
+// Tokens a sequence (b < batch) or the prefix (b == batch) holds, cut to what
+// its table holds.
+__device__ __forceinline__ int tokens_of(const WalkParams& p, int64_t b, bool* bad) {
+  int64_t n, cap;
+  if (b < p.a.batch) {
+    n = reinterpret_cast<const int32_t*>(p.a.seq_lens)[b];
+    cap = p.a.max_blocks * p.kv.block_tokens;
+  } else {
+    n = p.a.prefix_len;
+    if (p.a.prefix_len_dev) {
+      const int64_t dev = *reinterpret_cast<const int32_t*>(p.a.prefix_len_dev);
+      n = dev < n ? dev : n;
+    }
+    cap = p.a.prefix_blocks * p.kv.block_tokens;
+  }
+  *bad = n < 0 || n > cap;
+  return int(n < 0 ? 0 : (n > cap ? cap : n));
+}
+
+__device__ __forceinline__ int64_t tiles_of(const WalkParams& p, int64_t b, bool* bad) {
+  const int64_t per = b < p.a.batch ? int64_t(p.row_tiles_own) * p.kv.heads
+                                    : int64_t(p.row_tiles_pre) * p.kv.heads;
+  return int64_t((tokens_of(p, b, bad) + kTile - 1) / kTile) * per;
+}
+
+// Sum over sequences [0, end) of their tiles; every lane of the warp gets it.
+__device__ __forceinline__ int64_t tiles_before(const WalkParams& p, int64_t end) {
+  int64_t sum = 0;
+  bool bad, any = false;
+  for (int64_t b = threadIdx.x & 31; b < end; b += 32) {
+    sum += tiles_of(p, b, &bad);
+    any = any || bad;
+  }
+  if (any) raise(p.err);
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(~0u, sum, m);
+  return sum;
+}
+
+// CTA w of n takes tiles [total * w / n, total * (w + 1) / n), and n is cut to
+// the tiles there are, so that no CTA of them is without a tile.
+__device__ __forceinline__ int64_t sharers(const WalkParams& p, int64_t total) {
+  return total < p.ctas ? total : p.ctas;
+}
+
+// Position in the CTA's share: the item (sequence, row tile, KV head) and the
+// tiles [tile, end) of it that are this CTA's.
+struct Cursor {
+  int64_t left;    // tiles of the share from `tile` on
+  int64_t b;
+  int sub;         // row tile * heads + head
+  int tile, end;
+  int len;         // tokens of the sequence
+  int nt;          // tiles of the item
+
+  __device__ __forceinline__ void open(const WalkParams& p) {
+    // enter sequence b (skipping empty ones); sub and tile are set
+    bool bad;
+    for (; b < p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0); ++b) {
+      len = tokens_of(p, b, &bad);
+      nt = (len + kTile - 1) / kTile;
+      if (nt > 0) return clip();
+    }
+    left = 0;
+  }
+  __device__ __forceinline__ void clip() {
+    const int64_t rest = nt - tile;
+    end = tile + int(rest < left ? rest : left);
+  }
+  // the first share tile: global tile index lo
+  __device__ __forceinline__ void start(const WalkParams& p, int64_t lo, int64_t count) {
+    left = count;
+    b = 0;
+    sub = tile = end = len = nt = 0;
+    if (count <= 0) return;
+    const int lane = threadIdx.x & 31;
+    int64_t base = 0;
+    const int64_t seqs = p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0);
+    for (int64_t b0 = 0; b0 < seqs; b0 += 32) {
+      bool bad;
+      const int64_t mine = b0 + lane < seqs ? tiles_of(p, b0 + lane, &bad) : 0;
+      int64_t run = mine;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int64_t up = __shfl_up_sync(~0u, run, m);
+        if (lane >= m) run += up;
+      }
+      const unsigned past = __ballot_sync(~0u, base + run > lo);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        b = b0 + at;
+        const int64_t in_seq = lo - base - __shfl_sync(~0u, run - mine, at);
+        bool ignore;
+        len = tokens_of(p, b, &ignore);
+        nt = (len + kTile - 1) / kTile;
+        sub = int(in_seq / nt);
+        tile = int(in_seq - int64_t(sub) * nt);
+        clip();
+        return;
+      }
+      base += __shfl_sync(~0u, run, 31);
+    }
+    left = 0;
+  }
+  __device__ __forceinline__ bool done() const { return left <= 0; }
+  __device__ __forceinline__ int subs(const WalkParams& p) const {
+    return (b < p.a.batch ? p.row_tiles_own : p.row_tiles_pre) * int(p.kv.heads);
+  }
+  // past this item's tiles of the share
+  __device__ __forceinline__ void next_item(const WalkParams& p) {
+    left -= end - tile;
+    if (left <= 0) return;
+    tile = 0;
+    if (++sub == subs(p)) {
+      sub = 0;
+      ++b;
+      open(p);
+    } else {
+      clip();
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return uint32_t(__cvta_generic_to_shared(p));
+}
+// 16 bytes global -> shared; zeros when !ok
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <typename T>
+struct Ops;
+template <>
+struct Ops<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Ops<__half> {
+  static __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int D>
+__host__ __device__ constexpr int stage_bytes() { return 2 * kWarpTokens * D * 2; }  // K and V of a warp's tokens
+template <int D>
+__host__ __device__ constexpr int join_floats() { return 2 * 16 * (D + 4); }
+template <int D>
+__host__ __device__ constexpr int walk_smem() {
+  return kWarps * kStages * stage_bytes<D>() + join_floats<D>() * 4 + kWarps * kStages * 4;
+}
+
+// Row r of an item: which query (token index over the batch, head).
+__device__ __forceinline__ int64_t row_token(const WalkParams& p, const Cursor& c, int row) {
+  const int64_t base = c.b < p.a.batch ? c.b * p.a.new_tokens : 0;
+  return base + row / p.group;
+}
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_constant__ WalkParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, tg = lane & 3;
+  constexpr int kChunks = D / 8;          // 16-byte pieces of a head vector
+  constexpr int kRowBytes = D * 2;
+  constexpr int kRows = 16 * MT;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
+  float* join = reinterpret_cast<float*>(smem + kWarps * kStages * stage_bytes<D>());
+  uint32_t* masks = reinterpret_cast<uint32_t*>(join + join_floats<D>()) + warp * kStages;
+
+  const int64_t seqs = p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0);
+  const int64_t total = tiles_before(p, seqs);
+  const int64_t ctas = sharers(p, total);
+  if (blockIdx.x >= ctas) return;
+  const int64_t lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
+  Cursor ld, cu;
+  cu.start(p, lo, hi - lo);
+  ld = cu;
+  int ld_tile = ld.tile;
+
+  // Queues the warp's 16 tokens of tile ld_tile into ring stage `st`.
+  auto load = [&](int st) {
+    if (ld.done()) {
+      cp_commit();
+      return;
+    }
+    const int head = ld.sub % int(p.kv.heads);
+    const int t0 = ld_tile * kTile + warp * kWarpTokens;
+    // lanes 0..15 place one token each
+    const int t = t0 + (lane & 15);
+    const int blk = t / int(p.kv.block_tokens);
+    const int off = t - blk * int(p.kv.block_tokens);
+    bool ok = t < ld.len;
+    int page = 0;
+    if (ok) {
+      const int32_t* table = ld.b < p.a.batch
+          ? reinterpret_cast<const int32_t*>(p.a.block_table) + ld.b * p.a.block_table_stride
+          : reinterpret_cast<const int32_t*>(p.a.prefix_table);
+      page = table[blk];
+      if (page < 0 || page >= p.kv.pages) {
+        raise(p.err);
+        ok = false;
+        page = 0;
+      }
+    }
+    const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
+    if (lane == 0) masks[st] = mask;
+    const uint64_t ka = p.kv.k_ptr + uint64_t(page * p.kv.k_page_stride +
+                                              off * p.kv.k_token_stride +
+                                              head * p.kv.k_head_stride) * 2;
+    const uint64_t va = p.kv.v_ptr + uint64_t(page * p.kv.v_page_stride +
+                                              off * p.kv.v_token_stride +
+                                              head * p.kv.v_head_stride) * 2;
+    const uint32_t kdst = ring + st * stage_bytes<D>();
+    const uint32_t vdst = kdst + kWarpTokens * kRowBytes;
+    const int c = lane % kChunks;
+    constexpr int kPer = 32 / kChunks;  // tokens a warp's 32 lanes copy at once
+#pragma unroll
+    for (int i = 0; i < kWarpTokens / kPer; ++i) {
+      const int r = i * kPer + lane / kChunks;
+      const uint64_t kr = __shfl_sync(~0u, ka, r), vr = __shfl_sync(~0u, va, r);
+      const bool in = (mask >> r) & 1;
+      const uint32_t at = r * kRowBytes + ((c ^ (r & 7)) << 4);
+      cp_async16(kdst + at, reinterpret_cast<const void*>((in ? kr : p.kv.k_ptr) + c * 16), in);
+      cp_async16(vdst + at, reinterpret_cast<const void*>((in ? vr : p.kv.v_ptr) + c * 16), in);
+    }
+    cp_commit();
+    if (++ld_tile == ld.end) {
+      ld.next_item(p);
+      ld_tile = ld.tile;
+    }
+  };
+
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load(s);
+  int st = 0;
+
+  while (!cu.done()) {
+    const int head = cu.sub % int(p.kv.heads);
+    const int row0 = (cu.sub / int(p.kv.heads)) * kRows;
+    const bool own = cu.b < p.a.batch;
+    const int n_rows = own ? p.rows_own : p.rows_pre;
+    // the query rows as mma A fragments, and what each of this thread's rows sees
+    uint32_t qf[MT][D / 16][4];
+    int vis[MT][2];
+    int vis_min = INT32_MAX;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int row = row0 + mt * 16 + hf * 8 + g;
+        const bool in = row < n_rows;
+        const T* src = nullptr;
+        vis[mt][hf] = cu.len;
+        if (in) {
+          const int64_t tok = row_token(p, cu, row);
+          const int64_t b = tok / p.a.new_tokens, j = tok - b * p.a.new_tokens;
+          const int hq = head * p.group + row % p.group;
+          src = reinterpret_cast<const T*>(p.a.q) + b * p.a.q_batch_stride +
+                j * p.a.q_token_stride + hq * p.a.q_head_stride;
+          if (own) vis[mt][hf] = cu.len - int(p.a.new_tokens) + 1 + int(j);
+        }
+        vis_min = min(vis_min, vis[mt][hf]);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t x = 0, y = 0;
+          if (in) {
+            x = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg);
+            y = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg + 8);
+          }
+          qf[mt][ks][hf] = x;
+          qf[mt][ks][hf + 2] = y;
+        }
+      }
+    }
+    vis_min = __reduce_min_sync(~0u, vis_min);
+
+    float acc[MT][D / 8][4];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        acc[mt][i][0] = acc[mt][i][1] = acc[mt][i][2] = acc[mt][i][3] = 0.f;
+    }
+
+    for (int tile = cu.tile; tile < cu.end; ++tile) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      const uint32_t kb = ring + st * stage_bytes<D>();
+      const uint32_t vb = kb + kWarpTokens * kRowBytes;
+      const uint32_t mask = masks[st];
+      const int t0 = tile * kTile + warp * kWarpTokens;
+      float s[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[mt][i][0] = s[mt][i][1] = s[mt][i][2] = s[mt][i][3] = 0.f;
+      // S = Q K^T: lane addresses rows (tokens) 0-7 / 8-15 and the two halves of 16 elements
+      {
+        const int r = (lane & 7) + ((lane >> 4) << 3);
+        const int hb = (lane >> 3) & 1;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t b[4];
+          ldsm4(b, kb + r * kRowBytes + (((2 * ks + hb) ^ (r & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            Ops<T>::mma(s[mt][0], qf[mt][ks], b[0], b[1]);
+            Ops<T>::mma(s[mt][1], qf[mt][ks], b[2], b[3]);
+          }
+        }
+      }
+      const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
+      uint32_t pf[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float x[4] = {s[mt][0][2 * hf], s[mt][0][2 * hf + 1], s[mt][1][2 * hf],
+                        s[mt][1][2 * hf + 1]};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] *= p.scale_log2;
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int tok = (i >> 1) * 8 + 2 * tg + (i & 1);
+              if (!((mask >> tok) & 1) || t0 + tok >= vis[mt][hf]) x[i] = -INFINITY;
+            }
+          }
+          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+          const float mn = fmaxf(m[mt][hf], mx);
+          const float base = mn == -INFINITY ? 0.f : mn;
+          const float corr = ex2(m[mt][hf] - base);
+          m[mt][hf] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = ex2(x[i] - base);
+            sum += x[i];
+          }
+          l[mt][hf] = l[mt][hf] * corr + sum;
+          pf[mt][hf] = Ops<T>::pack(x[0], x[1]);
+          pf[mt][hf + 2] = Ops<T>::pack(x[2], x[3]);
+          if (__any_sync(~0u, corr != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+              acc[mt][i][2 * hf] *= corr;
+              acc[mt][i][2 * hf + 1] *= corr;
+            }
+          }
+        }
+      }
+      // acc += P V
+      {
+        const int r = lane & 15, hb = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t b[4];
+          ldsm4_t(b, vb + r * kRowBytes + (((2 * i + hb) ^ (r & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            Ops<T>::mma(acc[mt][2 * i], pf[mt], b[0], b[1]);
+            Ops<T>::mma(acc[mt][2 * i + 1], pf[mt], b[2], b[3]);
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the stage before it is filled again
+      int fill = st + kStages - 1;
+      load(fill >= kStages ? fill - kStages : fill);
+      if (++st == kStages) st = 0;
+    }
+
+    // Join the four warps (2 and 3 into 0 and 1, then 1 into 0), one 16-row
+    // tile at a time through a buffer of two.
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        l[mt][hf] += __shfl_xor_sync(~0u, l[mt][hf], 1);
+        l[mt][hf] += __shfl_xor_sync(~0u, l[mt][hf], 2);
+      }
+#pragma unroll
+      for (int step = 2; step >= 1; step >>= 1) {
+        __syncthreads();
+        float* buf = join + (warp & 1 & (step - 1)) * 16 * (D + 4);
+        if (warp >= step && warp < 2 * step) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            float* row = buf + (hf * 8 + g) * (D + 4);
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+              *reinterpret_cast<float2*>(row + i * 8 + 2 * tg) =
+                  make_float2(acc[mt][i][2 * hf], acc[mt][i][2 * hf + 1]);
+            if (tg == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[mt][hf], l[mt][hf]);
+          }
+        }
+        __syncthreads();
+        if (warp < step) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float* row = buf + (hf * 8 + g) * (D + 4);
+            const float2 ml = *reinterpret_cast<const float2*>(row + D);
+            const float mn = fmaxf(m[mt][hf], ml.x);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float w0 = ex2(m[mt][hf] - base), w1 = ex2(ml.x - base);
+            m[mt][hf] = mn;
+            l[mt][hf] = l[mt][hf] * w0 + ml.y * w1;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+              const float2 o = *reinterpret_cast<const float2*>(row + i * 8 + 2 * tg);
+              acc[mt][i][2 * hf] = acc[mt][i][2 * hf] * w0 + o.x * w1;
+              acc[mt][i][2 * hf + 1] = acc[mt][i][2 * hf + 1] * w0 + o.y * w1;
+            }
+          }
+        }
+      }
+    }
+
+    if (warp == 0) {
+      const bool complete = cu.tile == 0 && cu.end == cu.nt;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int rl = mt * 16 + hf * 8 + g;
+          const int row = row0 + rl;
+          if (row >= n_rows) continue;
+          float *da, *dm;
+          if (!complete) {
+            const int64_t slot = int64_t(blockIdx.x) * 2 + (cu.tile == 0 ? 1 : 0);
+            da = p.slots_acc + (slot * kRows + rl) * D;
+            dm = p.slots_ml + (slot * kRows + rl) * 2;
+          } else {
+            const int64_t out_row = row_token(p, cu, row) * p.a.q_heads +
+                                    head * p.group + row % p.group;
+            if (own && p.a.prefix_blocks == 0) {
+              // the whole row: the result itself
+              const float li = l[mt][hf];
+              const float inv = li > 0.f ? 1.f / li : (li == 0.f ? 0.f : li);
+              T* o = reinterpret_cast<T*>(p.a.out) + out_row * D;
+#pragma unroll
+              for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<uint32_t*>(o + i * 8 + 2 * tg) =
+                    Ops<T>::pack(acc[mt][i][2 * hf] * inv, acc[mt][i][2 * hf + 1] * inv);
+              if (p.a.lse && tg == 0)
+                reinterpret_cast<float*>(p.a.lse)[out_row] =
+                    li == 0.f ? -INFINITY : (m[mt][hf] + log2f(li)) * kLn2;
+              continue;
+            }
+            da = (own ? p.own_acc : p.pre_acc) + out_row * D;
+            dm = (own ? p.own_ml : p.pre_ml) + out_row * 2;
+          }
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+            *reinterpret_cast<float2*>(da + i * 8 + 2 * tg) =
+                make_float2(acc[mt][i][2 * hf], acc[mt][i][2 * hf + 1]);
+          if (tg == 0) *reinterpret_cast<float2*>(dm) = make_float2(m[mt][hf], l[mt][hf]);
+        }
+    }
+    cu.next_item(p);
+  }
+  cp_wait<0>();
+}
+
+// Where one part (own or prefix) of a query row lies: `count` partials, the
+// i-th at acc + i * stride rows (slots of consecutive CTAs), except that the
+// first may sit in a CTA's second slot.
+struct Part {
+  const float* acc0;
+  const float* ml0;
+  const float* acc1;  // the second and later ones, one CTA (two slots) apart
+  const float* ml1;
+  int count;
+};
+
+template <int D>
+__device__ __forceinline__ Part part_of(const WalkParams& p, int64_t total, int64_t start, int nt,
+                                        int rows, int rl, const float* whole_acc,
+                                        const float* whole_ml, int64_t out_row) {
+  Part r{};
+  if (nt == 0) return r;
+  // owner of global tile t: the CTA whose range holds it
+  const int64_t ctas = sharers(p, total);
+  const int64_t w0 = ((start + 1) * ctas - 1) / total;
+  const int64_t w1 = ((start + nt) * ctas - 1) / total;
+  if (w0 == w1) {
+    r.count = 1;
+    r.acc0 = whole_acc + out_row * D;
+    r.ml0 = whole_ml + out_row * 2;
+    return r;
+  }
+  r.count = int(w1 - w0) + 1;
+  // the first CTA begins the item (its second slot); the others go on with it
+  const int64_t s0 = (w0 * 2 + 1) * rows + rl, s1 = (w0 + 1) * 2 * rows + rl;
+  r.acc0 = p.slots_acc + s0 * D;
+  r.ml0 = p.slots_ml + s0 * 2;
+  r.acc1 = p.slots_acc + s1 * D;
+  r.ml1 = p.slots_ml + s1 * 2;
+  return r;
+}
+
+// One warp per query row: joins the partials of its own part and of its
+// prefix part.  Rows that walk_kernel finished itself are left alone; rows
+// whose sequence is empty are written here.
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkParams p) {
+  constexpr int kRows = 16 * MT, kPer = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t out_row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (out_row >= p.a.batch * p.a.new_tokens * p.a.q_heads) return;
+  const int64_t tok = out_row / p.a.q_heads;
+  const int hq = int(out_row - tok * p.a.q_heads);
+  const int64_t b = tok / p.a.new_tokens;
+  const int head = hq / p.group;
+  const int64_t heads = p.kv.heads;
+  const int64_t own_total = tiles_before(p, p.a.batch);
+  bool bad;
+  const int64_t total = own_total + (p.row_tiles_pre > 0 ? tiles_of(p, p.a.batch, &bad) : 0);
+
+  Part parts[2] = {};
+  {
+    const int nt = (tokens_of(p, b, &bad) + kTile - 1) / kTile;
+    const int row = int(tok - b * p.a.new_tokens) * p.group + hq % p.group;
+    const int64_t start = tiles_before(p, b) + (int64_t(row / kRows) * heads + head) * nt;
+    parts[0] = part_of<D>(p, total, start, nt, kRows, row % kRows, p.own_acc, p.own_ml, out_row);
+    if (p.a.prefix_blocks == 0 && parts[0].count == 1) return;  // written by walk_kernel
+  }
+  if (p.row_tiles_pre > 0) {
+    const int nt = (tokens_of(p, p.a.batch, &bad) + kTile - 1) / kTile;
+    const int64_t row = tok * p.group + hq % p.group;
+    const int64_t start = own_total + (row / kRows * heads + head) * nt;
+    parts[1] = part_of<D>(p, total, start, nt, kRows, int(row % kRows), p.pre_acc, p.pre_ml,
+                          out_row);
+  }
+  const int n0 = parts[0].count, n = n0 + parts[1].count;
+  auto at = [&](int i, const float** acc, const float** ml) {
+    const Part& q = parts[i < n0 ? 0 : 1];
+    const int k = i < n0 ? i : i - n0;
+    *acc = k == 0 ? q.acc0 : q.acc1 + int64_t(k - 1) * 2 * kRows * D;
+    *ml = k == 0 ? q.ml0 : q.ml1 + int64_t(k - 1) * 2 * kRows * 2;
+  };
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 32) {
+    const float *acc, *ml;
+    at(i, &acc, &ml);
+    m = fmaxf(m, ml[0]);
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, k));
+  const float base = m == -INFINITY ? 0.f : m;
+  float o[kPer] = {};
+  float l = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float *acc, *ml;
+    at(i, &acc, &ml);
+    const float w = ex2(ml[0] - base);
+    l += ml[1] * w;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] += acc[lane * kPer + e] * w;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* out = reinterpret_cast<T*>(p.a.out) + out_row * D + lane * kPer;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2)
+    *reinterpret_cast<uint32_t*>(out + e) = Ops<T>::pack(o[e] * inv, o[e + 1] * inv);
+  if (p.a.lse && lane == 0)
+    reinterpret_cast<float*>(p.a.lse)[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+int check_attention(const ts_paged_kv* kv, const ts_attention_args* args) {
+  if (int rc = check_paged_kv(kv)) return rc;
+  if (!args) return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  const ts_attention_args& a = *args;
+  if (kv->head_dim != 64 && kv->head_dim != 128)
+    return set_error(TS_UNIMPLEMENTED, "attention needs a head_dim of 64 or 128");
+  if (a.batch < 0 || a.new_tokens < 0 || a.q_heads <= 0 || a.max_blocks < 0 ||
+      a.prefix_blocks < 0 || a.prefix_len < 0 || a.block_table_stride < 0)
+    return set_error(TS_INVALID_ARGUMENT, "counts must be non-negative");
+  if (a.q_heads % kv->heads != 0)
+    return set_error(TS_INVALID_ARGUMENT, "query heads must be a multiple of the KV heads");
+  // rows and token positions are 32-bit in the kernels
+  if (a.batch > (1 << 24) || a.new_tokens > (1 << 20) || a.q_heads > 65535 ||
+      a.batch * a.new_tokens * a.q_heads > INT32_MAX / 2)
+    return set_error(TS_INVALID_ARGUMENT, "too many query rows");
+  if (a.max_blocks > INT32_MAX / 2 / kv->block_tokens ||
+      a.prefix_blocks > INT32_MAX / 2 / kv->block_tokens)
+    return set_error(TS_INVALID_ARGUMENT, "block tables hold too many tokens");
+  if (!(a.scale > 0.f) || !std::isfinite(a.scale))
+    return set_error(TS_INVALID_ARGUMENT, "scale must be finite and positive");
+  return TS_OK;
+}
+
+struct Layout {
+  int mt, ctas;
+  uint64_t slots_acc, slots_ml, own_acc, own_ml, pre_acc, pre_ml, bytes;
+};
+
+Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) {
+  Layout w{};
+  const int64_t group = a.q_heads / kv.heads;
+  const int64_t rows = a.batch * a.new_tokens * a.q_heads;
+  // 32-row tiles read K and V half as often once the rows pass one 16-row
+  // tile; below that they only waste registers and matrix work.
+  const bool pre = a.prefix_blocks > 0;
+  w.mt = a.new_tokens * group > 16 || (pre && a.batch * a.new_tokens * group > 16) ? 2 : 1;
+  w.ctas = 2 * sm_count(device);
+  uint64_t at = 0;
+  auto take = [&](uint64_t n) {
+    const uint64_t o = at;
+    at += (n * 4 + 255) / 256 * 256;
+    return o;
+  };
+  const uint64_t slot_rows = uint64_t(w.ctas) * 2 * 16 * w.mt;
+  w.slots_acc = take(slot_rows * kv.head_dim);
+  w.slots_ml = take(slot_rows * 2);
+  w.own_acc = take(pre ? rows * kv.head_dim : 0);
+  w.own_ml = take(pre ? rows * 2 : 0);
+  w.pre_acc = take(pre ? rows * kv.head_dim : 0);
+  w.pre_ml = take(pre ? rows * 2 : 0);
+  w.bytes = at;
+  return w;
+}
+
+template <typename T, int D, int MT>
+int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
+  static bool ready[64] = {};
+  if (device < 0 || device >= 64 || !ready[device]) {
+    TS_CUDA_RET(cudaFuncSetAttribute(walk_kernel<T, D, MT>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, walk_smem<D>()),
+                "attention shared memory");
+    if (device >= 0 && device < 64) ready[device] = true;
+  }
+  walk_kernel<T, D, MT><<<p.ctas, kWarps * 32, walk_smem<D>(), s>>>(p);
+  TS_CUDA_RET(cudaGetLastError(), "attention launch");
+  const int64_t rows = p.a.batch * p.a.new_tokens * p.a.q_heads;
+  join_kernel<T, D, MT><<<unsigned((rows + 3) / 4), 128, 0, s>>>(p);
+  TS_CUDA_RET(cudaGetLastError(), "attention join launch");
+  return TS_OK;
+}
+
+template <typename T>
+int launch_attention(const WalkParams& p, int mt, int device, cudaStream_t s) {
+  if (p.kv.head_dim == 64)
+    return mt == 1 ? launch_attention<T, 64, 1>(p, device, s)
+                   : launch_attention<T, 64, 2>(p, device, s);
+  return mt == 1 ? launch_attention<T, 128, 1>(p, device, s)
+                 : launch_attention<T, 128, 2>(p, device, s);
+}
+
+}  // namespace
+}  // namespace tsb
+
+using tsb::set_error;
+
+extern "C" int ts_paged_attention_workspace(int device, const ts_paged_kv* kv,
+                                            const ts_attention_args* args, uint64_t* bytes) {
+  tsb::clear_error();
+  if (int rc = tsb::check_attention(kv, args)) return rc;
+  if (!bytes) return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  *bytes = tsb::layout_of(*kv, *args, device).bytes;
+  return TS_OK;
+}
+
+extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
+                                  const ts_attention_args* args, void* workspace,
+                                  uint64_t workspace_bytes, int* err_flag, void* stream) {
+  tsb::clear_error();
+  if (int rc = tsb::check_attention(kv, args)) return rc;
+  const ts_attention_args& a = *args;
+  if (a.batch == 0 || a.new_tokens == 0) return TS_OK;
+  if (!a.q || !a.out || !a.seq_lens || (a.max_blocks > 0 && !a.block_table) ||
+      (a.prefix_blocks > 0 && !a.prefix_table))
+    return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  // 16-byte loads of queries, keys and values
+  const int64_t strides[] = {kv->k_page_stride, kv->k_token_stride, kv->k_head_stride,
+                             kv->v_page_stride, kv->v_token_stride, kv->v_head_stride,
+                             a.q_batch_stride,  a.q_token_stride,  a.q_head_stride};
+  for (int64_t x : strides)
+    if (x < 0 || x % 8 != 0)
+      return set_error(TS_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
+  if (kv->k_ptr % 16 || kv->v_ptr % 16 || a.q % 16 || a.out % 16)
+    return set_error(TS_INVALID_ARGUMENT, "pages, queries and output must be 16-byte aligned");
+  const tsb::Extent eq = tsb::extent(a.q, a.batch, a.q_batch_stride, a.new_tokens,
+                                     a.q_token_stride, a.q_heads, a.q_head_stride, kv->head_dim);
+  const tsb::Extent eo{a.out, a.out + uint64_t(a.batch * a.new_tokens * a.q_heads *
+                                               kv->head_dim) * 2};
+  if (eo.meets(eq) || eo.meets(tsb::pages_extent(*kv, false)) ||
+      eo.meets(tsb::pages_extent(*kv, true)))
+    return set_error(TS_INVALID_ARGUMENT, "output overlaps the queries or the pages");
+  const tsb::Layout w = tsb::layout_of(*kv, a, device);
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < w.bytes)
+    return set_error(TS_INVALID_ARGUMENT, "workspace too small or unaligned");
+  tsb::DeviceGuard g(device);
+  tsb::WalkParams p{};
+  p.kv = *kv;
+  p.a = a;
+  p.scale_log2 = a.scale * tsb::kLog2e;
+  p.group = int(a.q_heads / kv->heads);
+  p.rows_own = int(a.new_tokens) * p.group;
+  p.row_tiles_own = (p.rows_own + 16 * w.mt - 1) / (16 * w.mt);
+  p.rows_pre = int(a.batch) * p.rows_own;
+  p.row_tiles_pre = a.prefix_blocks > 0 ? (p.rows_pre + 16 * w.mt - 1) / (16 * w.mt) : 0;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  p.slots_acc = reinterpret_cast<float*>(base + w.slots_acc);
+  p.slots_ml = reinterpret_cast<float*>(base + w.slots_ml);
+  p.own_acc = reinterpret_cast<float*>(base + w.own_acc);
+  p.own_ml = reinterpret_cast<float*>(base + w.own_ml);
+  p.pre_acc = reinterpret_cast<float*>(base + w.pre_acc);
+  p.pre_ml = reinterpret_cast<float*>(base + w.pre_ml);
+  p.err = err_flag;
+  p.ctas = w.ctas;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return kv->dtype == TS_DTYPE_BF16
+             ? tsb::launch_attention<__nv_bfloat16>(p, w.mt, device, s)
+             : tsb::launch_attention<__half>(p, w.mt, device, s);
+}

@@ -1,0 +1,32 @@
+// What the paged KV cache operators share.
+#pragma once
+
+#include <cstdint>
+
+#include "tpusync_b200.h"
+
+namespace tsb {
+
+// Checks of a layer's page description (kv_append.cu).
+int check_paged_kv(const ts_paged_kv* kv);
+
+// Address range [lo, hi) of a strided tensor of 2-byte elements, for the
+// overlap checks; empty for a tensor without elements.
+struct Extent {
+  uint64_t lo, hi;
+  bool meets(const Extent& o) const { return lo < o.hi && o.lo < hi; }
+};
+inline Extent extent(uint64_t base, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2,
+                     int64_t s2, int64_t d) {
+  if (n0 <= 0 || n1 <= 0 || n2 <= 0) return {0, 0};
+  const int64_t last = (n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + d;
+  return {base, base + uint64_t(last) * 2};
+}
+inline Extent pages_extent(const ts_paged_kv& kv, bool v) {
+  return v ? extent(kv.v_ptr, kv.pages, kv.v_page_stride, kv.block_tokens, kv.v_token_stride,
+                    kv.heads, kv.v_head_stride, kv.head_dim)
+           : extent(kv.k_ptr, kv.pages, kv.k_page_stride, kv.block_tokens, kv.k_token_stride,
+                    kv.heads, kv.k_head_stride, kv.head_dim);
+}
+
+}  // namespace tsb

@@ -4,12 +4,18 @@ These take torch CUDA tensors, build the small device-side descriptor tables
 the kernels read, and launch on the current stream.  They are what the
 manager, the weight synchronizer and the hand-off executor are made of, and
 what the parity tests and the benchmark call directly.
+
+The paged cache operators at the end (`PagedKV`, `kv_append`,
+`paged_attention`, `shared_prefix_attention`) are what an engine runs between
+those transfers, on the same storages: the write of new tokens into their
+pages and the attention that reads the pages.
 """
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -396,3 +402,278 @@ def kv_relayout(src_storages: Sequence, dst_storages: Sequence, src_geom: dict,
       ctypes.c_void_p(err.data_ptr()), _stream(stream, device)), "kv_relayout: ")
   _keep([d_src, d_dst, st, dt, err], stream)
   return err
+
+
+def _on(stream: Optional[torch.cuda.Stream]):
+  """What a call allocates or converts belongs to the stream it runs on."""
+  return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+_PAGE_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
+
+
+class PagedKV:
+  """One layer's K and V storages as the paged cache operators address them.
+
+  k_pages / v_pages: bf16 or fp16 CUDA tensors [pages, block_tokens, heads,
+  head_dim], or with `head_major` [pages, heads, block_tokens, head_dim] (the
+  page orders of kv_relayout): the storages given to the manager, or strided
+  views of a joint cache such as kv[:, 0] and kv[:, 1] of [pages, 2, ...].
+  The last dimension is contiguous.  Like StorageTable it is built once and
+  describes the memory; it keeps the tensors alive.
+  """
+
+  def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, head_major: bool = False):
+    for t in (k_pages, v_pages):
+      if not t.is_cuda or t.dim() != 4:
+        raise ValueError("pages must be 4-dimensional CUDA tensors")
+      if t.dtype not in _PAGE_DTYPES:
+        raise ValueError(f"pages must be bfloat16 or float16, not {t.dtype}")
+      if t.shape[3] > 1 and t.stride(3) != 1:
+        raise ValueError("the last dimension of the pages must be contiguous")
+    if (k_pages.shape, k_pages.dtype, k_pages.device) != (v_pages.shape, v_pages.dtype,
+                                                          v_pages.device):
+      raise ValueError("K and V pages must have one shape, dtype and device")
+    if min(k_pages.shape[1:]) < 1:
+      raise ValueError("pages need at least one token, head and element")
+    self.k_pages, self.v_pages, self.head_major = k_pages, v_pages, bool(head_major)
+    self.device, self.dtype = k_pages.device, k_pages.dtype
+    tok, head = (2, 1) if head_major else (1, 2)
+    self.pages, self.block_tokens = k_pages.shape[0], k_pages.shape[tok]
+    self.heads, self.head_dim = k_pages.shape[head], k_pages.shape[3]
+    self._c = _native.PagedKvC(
+        k_pages.data_ptr(), v_pages.data_ptr(), self.pages, self.block_tokens, self.heads,
+        self.head_dim, k_pages.stride(0), k_pages.stride(tok), k_pages.stride(head),
+        v_pages.stride(0), v_pages.stride(tok), v_pages.stride(head),
+        _PAGE_DTYPES[self.dtype], 0)
+    self._ref = ctypes.byref(self._c)
+    self._index = self.device.index
+
+
+def _check_heads(kv: PagedKV, name: str, t: torch.Tensor, tokens: int, heads: Optional[int]):
+  if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != kv.head_dim or (
+      heads is not None and t.shape[1] != heads):
+    raise ValueError(f"{name} must be [{tokens}, {heads or 'heads'}, {kv.head_dim}], got "
+                     f"{list(t.shape)}")
+  _check_like(kv, name, t)
+
+
+def _check_like(kv: PagedKV, name: str, t: torch.Tensor):
+  if t.dtype != kv.dtype or t.device != kv.device:
+    raise ValueError(f"{name} must have the pages' dtype and device")
+  if t.stride(-1) != 1 and t.shape[-1] > 1:
+    raise ValueError(f"the last dimension of {name} must be contiguous")
+  if t.requires_grad and torch.is_grad_enabled():
+    raise ValueError(f"{name} requires grad: the paged cache operators have no backward pass")
+
+
+def _check_index(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int, device):
+  if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != dims or t.device != device:
+    raise ValueError(f"{name} must be a {dims}-dimensional {dtype} tensor on {device}")
+  if t.stride(-1) != 1 and t.shape[-1] > 1:
+    raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+def _check_flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
+  if err_flag is None:
+    return 0
+  if err_flag.dtype != torch.int32 or err_flag.device != kv.device or err_flag.numel() < 1:
+    raise ValueError("err_flag must be an int32 tensor on the pages' device")
+  return err_flag.data_ptr()
+
+
+def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
+              q: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+              cos_sin: Optional[torch.Tensor] = None, interleaved: bool = False,
+              q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+              eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+              err_flag: Optional[torch.Tensor] = None,
+              stream: Optional[torch.cuda.Stream] = None) -> Optional[torch.Tensor]:
+  """Writes new tokens' keys and values into their pages; norms and rotates
+  queries and keys on the way.  Returns the queries (None without `q`).
+
+  k, v [tokens, heads, head_dim] and q [tokens, q_heads, head_dim] may be
+  strided views of one projection's output.  slots: int64 [tokens], page *
+  block_tokens + offset; negative for a padding token, which writes nothing.
+  cos_sin: float32 [max_position, rotary], row p = the cosines, then the sines,
+  of position p's rotary / 2 angles; rotates the first `rotary` elements of a
+  head by row positions[t] (int64), pairs (i, i + rotary/2), or (2i, 2i+1) if
+  `interleaved`.  q_weight / k_weight [head_dim] (the pages' dtype or float32)
+  apply x * weight / sqrt(mean(x^2) + eps) to every query / key head before the
+  rotation.  q_out may be q itself; its padding rows stay as they were (a new
+  one has zeros there).
+
+  The slots of one call are distinct: where two tokens name one slot, it is not
+  defined which of them stays.  A slot past the pages or a position past
+  cos_sin writes nothing for its token and sets err_flag (int32, on the device)
+  to 1.
+  """
+  tokens = k.shape[0] if k.dim() else 0
+  _check_heads(kv, "k", k, tokens, kv.heads)
+  _check_heads(kv, "v", v, tokens, kv.heads)
+  _check_index("slots", slots, torch.int64, 1, kv.device)
+  if slots.shape[0] != tokens:
+    raise ValueError(f"slots must hold {tokens} entries")
+  flag = _check_flag(kv, err_flag)
+  a = _native.KvAppendArgs()
+  a.k, a.v, a.slots, a.tokens = k.data_ptr(), v.data_ptr(), slots.data_ptr(), tokens
+  a.k_token_stride, a.k_head_stride, _ = k.stride()
+  a.v_token_stride, a.v_head_stride, _ = v.stride()
+  if cos_sin is not None:
+    _check_index("positions", positions, torch.int64, 1, kv.device)
+    _check_index("cos_sin", cos_sin, torch.float32, 2, kv.device)
+    if positions.shape[0] != tokens:
+      raise ValueError(f"positions must hold {tokens} entries")
+    a.positions, a.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
+    a.max_position, a.rotary = cos_sin.shape
+    a.cos_sin_stride = cos_sin.stride(0) if a.max_position > 1 else a.rotary
+    a.interleaved = bool(interleaved)
+    if a.max_position == 0:
+      raise ValueError("cos_sin has no rows")
+  elif interleaved or positions is not None:
+    raise ValueError("positions and interleaved need cos_sin")
+  if q_weight is not None or k_weight is not None:
+    w = q_weight if q_weight is not None else k_weight
+    if w.dtype not in (kv.dtype, torch.float32):
+      raise ValueError("norm weights must be float32 or of the pages' dtype")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+      if t is None:
+        continue
+      _check_index(name, t, w.dtype, 1, kv.device)
+      if t.shape[0] != kv.head_dim:
+        raise ValueError(f"{name} must hold {kv.head_dim} entries")
+      if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad: the paged cache operators have no backward pass")
+    a.q_weight = q_weight.data_ptr() if q_weight is not None else 0
+    a.k_weight = k_weight.data_ptr() if k_weight is not None else 0
+    a.weight_dtype = _TORCH_TO_TS[w.dtype]
+    a.eps = eps
+    if q_weight is not None and q is None:
+      raise ValueError("q_weight needs q")
+  if q is not None:
+    _check_heads(kv, "q", q, tokens, None)
+    if q_out is None:
+      with _on(stream):
+        q_out = torch.empty(q.shape, dtype=kv.dtype, device=kv.device)
+      a.zero_padding = 1
+    else:
+      _check_heads(kv, "q_out", q_out, tokens, q.shape[1])
+    a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+    a.q_token_stride, a.q_head_stride, _ = q.stride()
+    a.q_out_token_stride, a.q_out_head_stride, _ = q_out.stride()
+    if a.q_heads == 0:
+      raise ValueError("q needs at least one head")
+  elif q_out is not None:
+    raise ValueError("q_out needs q")
+  _native.check(_native.lib().ts_kv_append(kv._index, kv._ref, ctypes.byref(a), flag,
+                                           _stream(stream, kv.device)), "kv_append: ")
+  return q_out
+
+
+def _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, out, return_lse,
+               err_flag, stream):
+  if q.dim() == 3:
+    batch, q_heads, dim = q.shape
+    new = 1
+  elif q.dim() == 4:
+    batch, new, q_heads, dim = q.shape
+  else:
+    raise ValueError("q must be [batch, q_heads, head_dim] or [batch, new_tokens, q_heads, "
+                     "head_dim]")
+  if dim != kv.head_dim or q_heads == 0:
+    raise ValueError(f"q heads must have {kv.head_dim} elements")
+  _check_like(kv, "q", q)
+  _check_index("block_table", block_table, torch.int32, 2, kv.device)
+  _check_index("seq_lens", seq_lens, torch.int32, 1, kv.device)
+  if block_table.shape[0] != batch or seq_lens.shape[0] != batch:
+    raise ValueError(f"block_table and seq_lens must hold {batch} sequences")
+  flag = _check_flag(kv, err_flag)
+  a = _native.AttentionArgs()
+  a.q, a.batch, a.new_tokens, a.q_heads = q.data_ptr(), batch, new, q_heads
+  strides = q.stride()
+  # a dimension of one element is never stepped over: its stride says nothing
+  a.q_batch_stride = strides[0] if batch > 1 else 0
+  a.q_token_stride = strides[1] if new > 1 else 0
+  a.q_head_stride = strides[-2] if q_heads > 1 else 0
+  a.block_table, a.max_blocks = block_table.data_ptr(), block_table.shape[1]
+  a.block_table_stride = block_table.stride(0) if batch > 1 else 0
+  a.seq_lens = seq_lens.data_ptr()
+  a.scale = dim ** -0.5 if scale is None else scale
+  if prefix_table is not None:
+    _check_index("prefix_table", prefix_table, torch.int32, 1, kv.device)
+    a.prefix_table, a.prefix_blocks = prefix_table.data_ptr(), prefix_table.shape[0]
+    if isinstance(prefix_len, torch.Tensor):
+      if prefix_len.dtype != torch.int32 or prefix_len.device != kv.device or (
+          prefix_len.numel() != 1):
+        raise ValueError("prefix_len must be an int or one int32 on the pages' device")
+      a.prefix_len_dev, a.prefix_len = prefix_len.data_ptr(), 2**31 - 1
+    else:
+      if not 0 <= prefix_len <= a.prefix_blocks * kv.block_tokens:
+        raise ValueError(f"prefix_table does not hold {prefix_len} tokens")
+      a.prefix_len = prefix_len
+  if out is not None:
+    _check_like(kv, "out", out)
+    if out.shape != q.shape or not out.is_contiguous():
+      raise ValueError("out must be contiguous and of q's shape")
+  lib = _native.lib()
+  nbytes = ctypes.c_uint64()
+  _native.check(lib.ts_paged_attention_workspace(kv._index, kv._ref, ctypes.byref(a),
+                                                 ctypes.byref(nbytes)), "attention: ")
+  with _on(stream):
+    if out is None:
+      out = torch.empty(q.shape, dtype=kv.dtype, device=kv.device)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=kv.device) if return_lse else None
+    work = torch.empty(nbytes.value, dtype=torch.uint8, device=kv.device)
+  a.out = out.data_ptr()
+  if return_lse:
+    a.lse = lse.data_ptr()
+  _native.check(lib.ts_paged_attention(kv._index, kv._ref, ctypes.byref(a), work.data_ptr(),
+                                       nbytes.value, flag, _stream(stream, kv.device)),
+                "attention: ")
+  return (out, lse) if return_lse else out
+
+
+def paged_attention(kv: PagedKV, q: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                    err_flag: Optional[torch.Tensor] = None,
+                    stream: Optional[torch.cuda.Stream] = None
+                    ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+  """Attention of each sequence's last tokens over its pages.
+
+  q: [batch, q_heads, head_dim], or [batch, n, q_heads, head_dim] for the last
+  n tokens of each sequence (drafted tokens); query head h reads KV head
+  h / (q_heads / heads).  block_table: int32 [batch, max_blocks], the pages of
+  a sequence in order; seq_lens: int32 [batch], its tokens in the cache, the
+  new ones included.  Query j sees the first seq_len - n + 1 + j tokens; one
+  that sees none gets zeros.  scale: default head_dim ** -0.5.  With
+  return_lse also returns float32 log(sum(exp(scores))) per query head (-inf
+  for a query that sees nothing).  head_dim is 64 or 128.
+
+  Tokens of a table entry outside the pages are left out, a length is cut to
+  what its table row holds, and either sets err_flag (int32, on the device) to
+  1.  Nothing is read back: lengths and tables may change between replays of a
+  captured call.
+  """
+  return _attention(kv, q, block_table, seq_lens, None, 0, scale, out, return_lse, err_flag,
+                    stream)
+
+
+def shared_prefix_attention(kv: PagedKV, q: torch.Tensor, prefix_table: torch.Tensor,
+                            prefix_len: Union[int, torch.Tensor], block_table: torch.Tensor,
+                            seq_lens: torch.Tensor, scale: Optional[float] = None,
+                            out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                            err_flag: Optional[torch.Tensor] = None,
+                            stream: Optional[torch.cuda.Stream] = None
+                            ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+  """paged_attention of a batch whose sequences continue one cached prefix.
+
+  Every query sees the first prefix_len tokens of the pages prefix_table
+  (int32 [blocks]), which are read once for the whole batch, and then its
+  sequence's own tokens as in paged_attention: block_table and seq_lens count
+  the tokens after the prefix (a sequence with none sees the prefix alone).
+  prefix_len: an int, or one int32 on the device (cut to what the table holds,
+  with err_flag set).
+  """
+  return _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, out,
+                    return_lse, err_flag, stream)
