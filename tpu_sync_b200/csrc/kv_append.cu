@@ -144,8 +144,232 @@ __global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__
   }
 }
 
+// Eight elements of a head vector, as loaded and in 32 bits.
+__device__ __forceinline__ void unpack8(const int4& v, float* f, __nv_bfloat16) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = __bfloat1622float2(h[i]);
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
+  }
+}
+__device__ __forceinline__ void unpack8(const int4& v, float* f, __half) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = __half22float2(h[i]);
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
+  }
+}
+__device__ __forceinline__ int4 pack8(const float* f, __nv_bfloat16) {
+  int4 v;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+__device__ __forceinline__ int4 pack8(const float* f, __half) {
+  int4 v;
+  __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void weights8(uint64_t w, int f32, int e, float* f) {
+  if (f32) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<float4*>(f + 4 * i) = reinterpret_cast<const float4*>(w)[e / 4 + i];
+  } else {
+    unpack8(*reinterpret_cast<const int4*>(reinterpret_cast<const T*>(w) + e), f, T{});
+  }
+}
+
+enum Rotation { kNone = 0, kHalves = 1, kPairs = 2 };
+constexpr int kHeadsAhead = 3;  // head vectors a lane holds before it works on the first
+
+// A CTA per token; kLanes = head_dim / 8 lanes hold a head, 16 bytes each, so
+// a warp takes 32 / kLanes heads at a time and a lane meets the same elements
+// of every head: its cosines and sines are loaded once per token.  Rotated
+// halves are 8-element pieces of another lane of the same head (one shuffle
+// per element); interleaved pairs lie within a lane.  All of a lane's head
+// vectors are loaded before the first is used, and before the slot and
+// position they depend on are known.
+template <typename T, int kLanes, int kRot, bool kNorm>
+__global__ void __launch_bounds__(256) append_vec_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kHeads = 32 / kLanes;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int j = lane % kLanes;
+  const int64_t t = blockIdx.x;
+  const int hq = p.a.q != 0 ? int(p.a.q_heads) : 0;
+  const int hk = int(p.kv.heads);
+  const int heads = hq + 2 * hk;
+  const T* q = reinterpret_cast<const T*>(p.a.q) + t * p.a.q_token_stride + j * 8;
+  const T* k = reinterpret_cast<const T*>(p.a.k) + t * p.a.k_token_stride + j * 8;
+  const T* v = reinterpret_cast<const T*>(p.a.v) + t * p.a.v_token_stride + j * 8;
+  T* qo = reinterpret_cast<T*>(p.a.q_out) + t * p.a.q_out_token_stride + j * 8;
+  const int step = warps * kHeads;
+
+  int4 x[kHeadsAhead];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < kHeadsAhead; ++i) {
+      const int h = h0 + i * step;
+      if (h < heads) {
+        const T* src = h < hq ? q + h * p.a.q_head_stride
+                              : (h < hq + hk ? k + (h - hq) * p.a.k_head_stride
+                                             : v + (h - hq - hk) * p.a.v_head_stride);
+        x[i] = __ldcs(reinterpret_cast<const int4*>(src));
+      }
+    }
+  };
+  int h0 = warp * kHeads + lane / kLanes;
+  load(h0);
+  int64_t page = 0, off = 0, pos = 0;
+  const bool live = token_place(p, t, kRot != kNone, &page, &off, &pos);
+  if (!live) {
+    if (p.a.zero_padding)
+      for (int h = h0; h < hq; h += step)
+        *reinterpret_cast<int4*>(qo + h * p.a.q_out_head_stride) = make_int4(0, 0, 0, 0);
+    return;
+  }
+  T* kd = reinterpret_cast<T*>(p.kv.k_ptr) + page * p.kv.k_page_stride + off * p.kv.k_token_stride +
+          j * 8;
+  T* vd = reinterpret_cast<T*>(p.kv.v_ptr) + page * p.kv.v_page_stride + off * p.kv.v_token_stride +
+          j * 8;
+  // this lane's cosines and sines, and the lane of its pairs' other halves
+  constexpr int kAngles = kRot == kPairs ? 4 : 8;
+  float c[kAngles], s[kAngles];
+  int mate = lane;
+  bool turns = false, second = false;
+  if (kRot != kNone) {
+    const int half = int(p.a.rotary) / 2;
+    const float* row = reinterpret_cast<const float*>(p.a.cos_sin) + pos * p.a.cos_sin_stride;
+    int at;
+    if (kRot == kPairs) {
+      turns = j * 8 < int(p.a.rotary);
+      at = j * 4;
+    } else {
+      const int half_lanes = half / 8;
+      turns = j < 2 * half_lanes;
+      second = j >= half_lanes;
+      at = (second ? j - half_lanes : j) * 8;
+      if (turns) mate = second ? lane - half_lanes : lane + half_lanes;
+    }
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < kAngles / 4; ++i) {
+        *reinterpret_cast<float4*>(c + 4 * i) =
+            __ldg(reinterpret_cast<const float4*>(row + at) + i);
+        *reinterpret_cast<float4*>(s + 4 * i) =
+            __ldg(reinterpret_cast<const float4*>(row + half + at) + i);
+      }
+    }
+  }
+  // every lane of a warp makes the same rounds: the shuffles need them all
+  for (int base = warp * kHeads; base < heads; base += kHeadsAhead * step, h0 += kHeadsAhead * step) {
+    if (base != warp * kHeads) load(h0);
+#pragma unroll
+    for (int i = 0; i < kHeadsAhead; ++i) {
+      if (base + i * step >= heads) break;
+      const int h = h0 + i * step;
+      const bool is_q = h < hq, is_k = !is_q && h < hq + hk;
+      if ((kNorm || kRot != kNone) && base + i * step < hq + hk) {
+        float f[8];
+        unpack8(x[i], f, T{});
+        if (kNorm) {
+          const uint64_t w = is_q ? p.a.q_weight : p.a.k_weight;
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+#pragma unroll
+          for (int m = kLanes / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(~0u, ss, m);
+          if (w != 0 && (is_q || is_k)) {
+            const float inv = rsqrtf(ss * (1.f / (8 * kLanes)) + p.a.eps);
+            float g[8];
+            weights8<T>(w, p.a.weight_dtype == TS_DTYPE_F32, j * 8, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = f[e] * inv * g[e];
+          }
+        }
+        if (kRot == kHalves) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float o = __shfl_sync(~0u, f[e], mate);
+            if (turns) f[e] = second ? f[e] * c[e] + o * s[e] : f[e] * c[e] - o * s[e];
+          }
+        } else if (kRot == kPairs) {
+          if (turns) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float a = f[2 * e], b = f[2 * e + 1];
+              f[2 * e] = a * c[e % kAngles] - b * s[e % kAngles];
+              f[2 * e + 1] = b * c[e % kAngles] + a * s[e % kAngles];
+            }
+          }
+        }
+        if (is_q || is_k) x[i] = pack8(f, T{});
+      }
+      if (h < heads) {
+        T* dst = is_q ? qo + h * p.a.q_out_head_stride
+                      : (is_k ? kd + (h - hq) * p.kv.k_head_stride
+                              : vd + (h - hq - hk) * p.kv.v_head_stride);
+        *reinterpret_cast<int4*>(dst) = x[i];
+      }
+    }
+  }
+}
+
+// The vector kernel's rule: heads of 64, 128 or 256 elements, every address and
+// stride a multiple of 16 bytes, rotated halves (pairs) made of whole 8-element
+// pieces.
+bool vector_ok(const AppendParams& p) {
+  const ts_paged_kv& kv = p.kv;
+  const ts_kv_append_args& a = p.a;
+  if (kv.head_dim != 64 && kv.head_dim != 128 && kv.head_dim != 256) return false;
+  uint64_t ptrs = kv.k_ptr | kv.v_ptr | a.k | a.v | a.q | a.q_out | a.cos_sin | a.q_weight |
+                  a.k_weight;
+  int64_t strides = kv.k_page_stride | kv.k_token_stride | kv.k_head_stride | kv.v_page_stride |
+                    kv.v_token_stride | kv.v_head_stride | a.k_token_stride | a.k_head_stride |
+                    a.v_token_stride | a.v_head_stride;
+  if (a.q)
+    strides |= a.q_token_stride | a.q_head_stride | a.q_out_token_stride | a.q_out_head_stride;
+  if (ptrs % 16 != 0 || strides % 8 != 0) return false;
+  if (!a.cos_sin) return true;
+  return a.cos_sin_stride % 4 == 0 && a.rotary % (a.interleaved ? 8 : 16) == 0;
+}
+
+template <typename T, int kLanes>
+void launch_vec(const AppendParams& p, cudaStream_t s) {
+  constexpr int kHeads = 32 / kLanes;
+  const int heads = int(p.a.q != 0 ? p.a.q_heads : 0) + 2 * int(p.kv.heads);
+  const int warps = std::min(8, (heads + kHeads - 1) / kHeads);
+  const bool norm = p.a.q_weight || p.a.k_weight;
+  const dim3 grid(static_cast<unsigned>(p.a.tokens)), block(warps * 32);
+  if (!p.a.cos_sin)
+    norm ? append_vec_kernel<T, kLanes, kNone, true><<<grid, block, 0, s>>>(p)
+         : append_vec_kernel<T, kLanes, kNone, false><<<grid, block, 0, s>>>(p);
+  else if (p.a.interleaved)
+    norm ? append_vec_kernel<T, kLanes, kPairs, true><<<grid, block, 0, s>>>(p)
+         : append_vec_kernel<T, kLanes, kPairs, false><<<grid, block, 0, s>>>(p);
+  else
+    norm ? append_vec_kernel<T, kLanes, kHalves, true><<<grid, block, 0, s>>>(p)
+         : append_vec_kernel<T, kLanes, kHalves, false><<<grid, block, 0, s>>>(p);
+}
+
 template <typename T>
 int launch_append(const AppendParams& p, int device, cudaStream_t s) {
+  if (vector_ok(p)) {
+    p.kv.head_dim == 64    ? launch_vec<T, 8>(p, s)
+    : p.kv.head_dim == 128 ? launch_vec<T, 16>(p, s)
+                           : launch_vec<T, 32>(p, s);
+    TS_CUDA_RET(cudaGetLastError(), "kv append launch");
+    return TS_OK;
+  }
   const int64_t heads = (p.a.q != 0 ? p.a.q_heads : 0) + 2 * p.kv.heads;
   const int64_t ctas = (p.a.tokens * heads + 7) / 8;
   const int64_t cap = int64_t(sm_count(device)) * 64;
