@@ -339,17 +339,17 @@ def test_shared_prefix_attention(cuda, case, dt):
   assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("lens", [[700, 64], [3] * 40], ids=["few", "many"])
 @pytest.mark.parametrize("std", [0.0, 30.0])
-def test_flat_and_sharp_scores(cuda, std):
+def test_flat_and_sharp_scores(cuda, std, lens):
   """All scores equal, and scores of a few hundred (one key takes nearly all the weight)."""
-  lens = [700, 64]
   pools, table, lens_t, ptable, q, own, shared = build(7, BF, 8, 2, 128, 16, False, 1, lens, 300,
                                                        std=std)
   kv = ops.PagedKV(*pools)
   out, lse = ops.shared_prefix_attention(kv, q, ptable, 300, table, lens_t, return_lse=True,
                                          scale=0.05)
   x = 30 * 0.05 * math.sqrt(128) * 5  # largest score: its 32-bit roundings bound the weights
-  for i in range(2):
+  for i in range(len(lens)):
     k = torch.cat([shared[0], own[i][0]])
     v = torch.cat([shared[1], own[i][1]])
     s = torch.einsum("hgd,thd->hgt", q[i, 0].double().view(2, 4, 128), k) * 0.05
@@ -404,6 +404,51 @@ def test_bad_pages_and_lengths(cuda):
   check(out, lse, q, own, shared, lens, 2, BF)
 
 
+@pytest.mark.parametrize("d,bt,dt", [(128, 16, BF), (64, 64, FP)])
+def test_bad_pages_of_a_prefix_with_many_rows(cuda, d, bt, dt):
+  """The same for the tensor-core form (many query rows): holes in any tile, the first one
+  among them, a whole tile of holes, and a length past the table."""
+  lens = [(5 * i) % 23 for i in range(80)]
+  n = 1000
+  pools, table, lens_t, ptable, q, own, shared = build(15, dt, 8, 2, d, bt, False, 1, lens, n)
+  kv = ops.PagedKV(*pools)
+  err = torch.zeros(1, dtype=torch.int32, device="cuda")
+  holes = [0, 3] + list(range(128 // bt, 256 // bt)) + [ptable.shape[0] - 1]
+  pbad = ptable.clone()
+  pbad[torch.tensor(holes)] = torch.tensor([-1, 2 ** 31 - 1, -2 ** 31, pools[0].shape[0]] * 9,
+                                           dtype=torch.int32)[:len(holes)].cuda()
+  out, lse = ops.shared_prefix_attention(kv, q, pbad, n, table, lens_t, return_lse=True,
+                                         err_flag=err)
+  assert int(err) == 1
+  keep = torch.tensor([i for i in range(n) if i // bt not in holes])
+  check(out, lse, q, own, [x[keep.cuda()] for x in shared], lens, 2, dt)
+  err.zero_()
+  all_bad = torch.full_like(ptable, -1)
+  out, lse = ops.shared_prefix_attention(kv, q, all_bad, n, table, lens_t, return_lse=True,
+                                         err_flag=err)
+  assert int(err) == 1
+  check(out, lse, q, own, None, lens, 2, dt)
+  err.zero_()
+  long = torch.tensor([ptable.shape[0] * bt + 1], dtype=torch.int32, device="cuda")
+  whole = ptable[:n // bt]
+  out, lse = ops.shared_prefix_attention(kv, q, whole, long, table, lens_t, return_lse=True,
+                                         err_flag=err)
+  assert int(err) == 1
+  check(out, lse, q, own, [x[:n // bt * bt] for x in shared], lens, 2, dt)
+
+
+@pytest.mark.parametrize("prefix", [1, 127, 128, 129, 255, 1023, 20000])
+def test_prefix_lengths_with_many_rows(cuda, prefix):
+  """Tile ends, one key, and more tiles than CTAs; 130 rows and 1040 rows per KV head."""
+  for hq, hk, count in ((13, 1, 10), (26, 1, 40)):
+    lens = [(3 * i) % 7 for i in range(count)]
+    pools, table, lens_t, ptable, q, own, shared = build(prefix, BF, hq, hk, 128, 16, True, 1,
+                                                         lens, prefix)
+    out, lse = ops.shared_prefix_attention(ops.PagedKV(*pools, head_major=True), q, ptable, prefix,
+                                           table, lens_t, return_lse=True)
+    check(out, lse, q, own, shared, lens, hk, BF)
+
+
 def test_no_sequences_and_no_blocks(cuda):
   pools, table, lens_t, ptable, q, own, shared = build(9, FP, 8, 2, 64, 16, False, 1, [20, 3], 40)
   kv = ops.PagedKV(*pools)
@@ -455,6 +500,11 @@ def test_far_pages(cuda):
   check(out, lse, q, [[k.double(), v.double()]], None, [40], 8, BF)
   out, lse = ops.shared_prefix_attention(kv, q, table[0], 40, table, lens * 0, return_lse=True)
   check(out, lse, q, [[k[:0].double(), v[:0].double()]], [k.double(), v.double()], [0], 8, BF)
+  many = rand(g, 9, 1, 32, 128, dtype=BF)
+  out, lse = ops.shared_prefix_attention(kv, many, table[0], 40, table.repeat(9, 1),
+                                         lens.repeat(9) * 0, return_lse=True)
+  check(out, lse, many, [[k[:0].double(), v[:0].double()]] * 9, [k.double(), v.double()], [0] * 9,
+        8, BF)
 
 
 def test_other_stream_and_repeatable(cuda):

@@ -28,8 +28,10 @@
 
 #include <cmath>
 #include <cstdint>
+#include <numeric>
 
 #include "paged_kv.h"
+#include "prefix_attention.h"
 #include "ts_internal.h"
 
 namespace tsb {
@@ -59,6 +61,11 @@ struct WalkParams {
   float* pre_ml;
   int* err;
   int ctas;
+  // the prefix part when prefix_attention.cu does it: its partition and partials
+  int tensor_ctas;    // 0: it does not
+  int tensor_row_tiles;
+  float* tensor_acc;
+  float* tensor_ml;
 };
 
 __device__ __forceinline__ void raise(int* err) {
@@ -68,18 +75,9 @@ __device__ __forceinline__ void raise(int* err) {
 // Tokens a sequence (b < batch) or the prefix (b == batch) holds, cut to what
 // its table holds.
 __device__ __forceinline__ int tokens_of(const WalkParams& p, int64_t b, bool* bad) {
-  int64_t n, cap;
-  if (b < p.a.batch) {
-    n = reinterpret_cast<const int32_t*>(p.a.seq_lens)[b];
-    cap = p.a.max_blocks * p.kv.block_tokens;
-  } else {
-    n = p.a.prefix_len;
-    if (p.a.prefix_len_dev) {
-      const int64_t dev = *reinterpret_cast<const int32_t*>(p.a.prefix_len_dev);
-      n = dev < n ? dev : n;
-    }
-    cap = p.a.prefix_blocks * p.kv.block_tokens;
-  }
+  if (b >= p.a.batch) return prefix_tokens(p.kv, p.a, bad);
+  const int64_t n = reinterpret_cast<const int32_t*>(p.a.seq_lens)[b];
+  const int64_t cap = p.a.max_blocks * p.kv.block_tokens;
   *bad = n < 0 || n > cap;
   return int(n < 0 ? 0 : (n > cap ? cap : n));
 }
@@ -106,8 +104,8 @@ __device__ __forceinline__ int64_t tiles_before(const WalkParams& p, int64_t end
 
 // CTA w of n takes tiles [total * w / n, total * (w + 1) / n), and n is cut to
 // the tiles there are, so that no CTA of them is without a tile.
-__device__ __forceinline__ int64_t sharers(const WalkParams& p, int64_t total) {
-  return total < p.ctas ? total : p.ctas;
+__device__ __forceinline__ int64_t sharers(int64_t total, int ctas) {
+  return total < ctas ? total : ctas;
 }
 
 // Position in the CTA's share: the item (sequence, row tile, KV head) and the
@@ -283,7 +281,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
 
   const int64_t seqs = p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0);
   const int64_t total = tiles_before(p, seqs);
-  const int64_t ctas = sharers(p, total);
+  const int64_t ctas = sharers(total, p.ctas);
   if (blockIdx.x >= ctas) return;
   const int64_t lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
   Cursor ld, cu;
@@ -588,17 +586,20 @@ struct Part {
   const float* ml0;
   const float* acc1;  // the second and later ones, one CTA (two slots) apart
   const float* ml1;
+  int step;           // rows between them
   int count;
 };
 
+// The part of a row (row rl of an item's `rows`) whose item holds the tiles
+// [start, start + nt) of `total`, shared by `ctas` CTAs.
 template <int D>
-__device__ __forceinline__ Part part_of(const WalkParams& p, int64_t total, int64_t start, int nt,
-                                        int rows, int rl, const float* whole_acc,
+__device__ __forceinline__ Part part_of(int64_t total, int64_t ctas, int64_t start, int nt,
+                                        int rows, int rl, const float* slots_acc,
+                                        const float* slots_ml, const float* whole_acc,
                                         const float* whole_ml, int64_t out_row) {
   Part r{};
   if (nt == 0) return r;
-  // owner of global tile t: the CTA whose range holds it
-  const int64_t ctas = sharers(p, total);
+  // owner of tile t: the CTA whose share holds it
   const int64_t w0 = ((start + 1) * ctas - 1) / total;
   const int64_t w1 = ((start + nt) * ctas - 1) / total;
   if (w0 == w1) {
@@ -610,10 +611,11 @@ __device__ __forceinline__ Part part_of(const WalkParams& p, int64_t total, int6
   r.count = int(w1 - w0) + 1;
   // the first CTA begins the item (its second slot); the others go on with it
   const int64_t s0 = (w0 * 2 + 1) * rows + rl, s1 = (w0 + 1) * 2 * rows + rl;
-  r.acc0 = p.slots_acc + s0 * D;
-  r.ml0 = p.slots_ml + s0 * 2;
-  r.acc1 = p.slots_acc + s1 * D;
-  r.ml1 = p.slots_ml + s1 * 2;
+  r.acc0 = slots_acc + s0 * D;
+  r.ml0 = slots_ml + s0 * 2;
+  r.step = 2 * rows;
+  r.acc1 = slots_acc + s1 * D;
+  r.ml1 = slots_ml + s1 * 2;
   return r;
 }
 
@@ -636,26 +638,34 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkP
   const int64_t total = own_total + (p.row_tiles_pre > 0 ? tiles_of(p, p.a.batch, &bad) : 0);
 
   Part parts[2] = {};
+  const int64_t ctas = sharers(total, p.ctas);
   {
     const int nt = (tokens_of(p, b, &bad) + kTile - 1) / kTile;
     const int row = int(tok - b * p.a.new_tokens) * p.group + hq % p.group;
     const int64_t start = tiles_before(p, b) + (int64_t(row / kRows) * heads + head) * nt;
-    parts[0] = part_of<D>(p, total, start, nt, kRows, row % kRows, p.own_acc, p.own_ml, out_row);
+    parts[0] = part_of<D>(total, ctas, start, nt, kRows, row % kRows, p.slots_acc, p.slots_ml,
+                          p.own_acc, p.own_ml, out_row);
     if (p.a.prefix_blocks == 0 && parts[0].count == 1) return;  // written by walk_kernel
   }
+  const int64_t row = tok * p.group + hq % p.group;
   if (p.row_tiles_pre > 0) {
     const int nt = (tokens_of(p, p.a.batch, &bad) + kTile - 1) / kTile;
-    const int64_t row = tok * p.group + hq % p.group;
     const int64_t start = own_total + (row / kRows * heads + head) * nt;
-    parts[1] = part_of<D>(p, total, start, nt, kRows, int(row % kRows), p.pre_acc, p.pre_ml,
-                          out_row);
+    parts[1] = part_of<D>(total, ctas, start, nt, kRows, int(row % kRows), p.slots_acc,
+                          p.slots_ml, p.pre_acc, p.pre_ml, out_row);
+  } else if (p.tensor_ctas > 0) {
+    const int nt = (tokens_of(p, p.a.batch, &bad) + kPrefixTile - 1) / kPrefixTile;
+    const int64_t all = int64_t(nt) * p.tensor_row_tiles * heads;
+    parts[1] = part_of<D>(all, sharers(all, p.tensor_ctas), (row / kPrefixRows * heads + head) * nt,
+                          nt, kPrefixRows, int(row % kPrefixRows), p.tensor_acc, p.tensor_ml,
+                          p.pre_acc, p.pre_ml, out_row);
   }
   const int n0 = parts[0].count, n = n0 + parts[1].count;
   auto at = [&](int i, const float** acc, const float** ml) {
     const Part& q = parts[i < n0 ? 0 : 1];
     const int k = i < n0 ? i : i - n0;
-    *acc = k == 0 ? q.acc0 : q.acc1 + int64_t(k - 1) * 2 * kRows * D;
-    *ml = k == 0 ? q.ml0 : q.ml1 + int64_t(k - 1) * 2 * kRows * 2;
+    *acc = k == 0 ? q.acc0 : q.acc1 + int64_t(k - 1) * q.step * D;
+    *ml = k == 0 ? q.ml0 : q.ml1 + int64_t(k - 1) * q.step * 2;
   };
   float m = -INFINITY;
   for (int i = lane; i < n; i += 32) {
@@ -711,7 +721,8 @@ int check_attention(const ts_paged_kv* kv, const ts_attention_args* args) {
 
 struct Layout {
   int mt, ctas;
-  uint64_t slots_acc, slots_ml, own_acc, own_ml, pre_acc, pre_ml, bytes;
+  bool tensor;  // the prefix part goes to the tensor-core kernel
+  uint64_t slots_acc, slots_ml, own_acc, own_ml, pre_acc, pre_ml, tensor_acc, tensor_ml, bytes;
 };
 
 Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) {
@@ -721,7 +732,11 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   // 32-row tiles read K and V half as often once the rows pass one 16-row
   // tile; below that they only waste registers and matrix work.
   const bool pre = a.prefix_blocks > 0;
-  w.mt = a.new_tokens * group > 16 || (pre && a.batch * a.new_tokens * group > 16) ? 2 : 1;
+  w.tensor = pre && a.batch * a.new_tokens * group > 32 && prefix_geometry_ok(kv);
+  w.mt = a.new_tokens * group > 16 ||
+                 (pre && !w.tensor && a.batch * a.new_tokens * group > 16)
+             ? 2
+             : 1;
   w.ctas = 2 * sm_count(device);
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
@@ -736,6 +751,9 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   w.own_ml = take(pre ? rows * 2 : 0);
   w.pre_acc = take(pre ? rows * kv.head_dim : 0);
   w.pre_ml = take(pre ? rows * 2 : 0);
+  const uint64_t tensor_rows = w.tensor ? uint64_t(sm_count(device)) * 2 * kPrefixRows : 0;
+  w.tensor_acc = take(tensor_rows * kv.head_dim);
+  w.tensor_ml = take(tensor_rows * 2);
   w.bytes = at;
   return w;
 }
@@ -818,7 +836,8 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
   p.rows_own = int(a.new_tokens) * p.group;
   p.row_tiles_own = (p.rows_own + 16 * w.mt - 1) / (16 * w.mt);
   p.rows_pre = int(a.batch) * p.rows_own;
-  p.row_tiles_pre = a.prefix_blocks > 0 ? (p.rows_pre + 16 * w.mt - 1) / (16 * w.mt) : 0;
+  p.row_tiles_pre = a.prefix_blocks > 0 && !w.tensor ? (p.rows_pre + 16 * w.mt - 1) / (16 * w.mt)
+                                                     : 0;
   uint8_t* base = static_cast<uint8_t*>(workspace);
   p.slots_acc = reinterpret_cast<float*>(base + w.slots_acc);
   p.slots_ml = reinterpret_cast<float*>(base + w.slots_ml);
@@ -829,6 +848,27 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
   p.err = err_flag;
   p.ctas = w.ctas;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (w.tensor) {
+    tsb::PrefixParams t{};
+    t.kv = *kv;
+    t.a = a;
+    t.scale_log2 = p.scale_log2;
+    t.group = p.group;
+    t.rows = p.rows_pre;
+    t.row_tiles = (p.rows_pre + tsb::kPrefixRows - 1) / tsb::kPrefixRows;
+    t.piece = int(std::gcd(kv->block_tokens, int64_t(tsb::kPrefixTile)));
+    t.ctas = tsb::sm_count(device);
+    t.slots_acc = reinterpret_cast<float*>(base + w.tensor_acc);
+    t.slots_ml = reinterpret_cast<float*>(base + w.tensor_ml);
+    t.whole_acc = p.pre_acc;
+    t.whole_ml = p.pre_ml;
+    t.err = err_flag;
+    p.tensor_ctas = t.ctas;
+    p.tensor_row_tiles = t.row_tiles;
+    p.tensor_acc = t.slots_acc;
+    p.tensor_ml = t.slots_ml;
+    if (int rc = tsb::launch_prefix(t, device, s)) return rc;
+  }
   return kv->dtype == TS_DTYPE_BF16
              ? tsb::launch_attention<__nv_bfloat16>(p, w.mt, device, s)
              : tsb::launch_attention<__half>(p, w.mt, device, s);

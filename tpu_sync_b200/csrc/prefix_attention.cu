@@ -1,0 +1,643 @@
+// Attention of all query rows of a batch over the pages they share, on the
+// tensor cores of sm_100a.
+//
+// With B sequences, n new tokens and G query heads per KV head, one KV head has
+// B n G query rows against the same keys: S = Q K^T and O = P V are true matrix
+// products, 4 D operations per row and key, against 4 D bytes per key.  Past
+// about 250 rows the tensor cores bound it, and next to them the exponentials
+// (16 per cycle and SM, one per row and key).
+//
+// A unit is (256 query rows, KV head).  A CTA takes an equal, contiguous share
+// of all 128-key tiles of all units (shares are cut on the device, from the
+// prefix length there); a share that cuts a unit leaves partials (m, l, acc),
+// joined per row by join_kernel.  Roles of the ten warps:
+//
+//   warps 0-3, 4-7  one query row per thread, 128 rows each (halves A and B):
+//                   S from TMEM, running maximum and sum, P = 2^(S - m) back to
+//                   TMEM over S as the A operand of the second product.  The
+//                   accumulator is rescaled only when a maximum grew by more
+//                   than 2^8: m is any common reference, so the result is the
+//                   same, and P stays below 2^8.
+//   warp 8          page lookups and TMA loads of K and V tiles into a ring.
+//   warp 9          all tcgen05.mma: while one half's softmax runs, the other
+//                   half's products do.
+//
+// TMEM (512 columns at D = 128): S/P of A and B (128 each), O of A and B (D
+// each).  Shared memory: both halves' queries, and a ring of 128-key tiles of K
+// and V, all in the 128-byte swizzle TMA writes and tcgen05 reads.
+// Keys past the length are masked and their V rows zeroed (a page may hold
+// anything there); table entries outside the pages load as zeros through TMA's
+// bounds and are masked.
+//
+// Every wait is bounded: on running out it raises the flag (value 2), and all
+// roles leave.
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+#include <numeric>
+#include <type_traits>
+
+#include "prefix_attention.h"
+#include "ts_internal.h"
+
+namespace tsb {
+namespace {
+
+constexpr int kThreads = 320;
+constexpr uint32_t kWaitRounds = 1u << 24;  // try_waits (each suspends for a while): seconds
+
+template <int D>
+struct Shape {
+  static constexpr int kTileBytes = kPrefixTile * D * 2;  // a K or V tile
+  static constexpr int kStages = D == 128 ? 5 : 9;
+  static constexpr int kQBytes = kPrefixRows * D * 2;
+  static constexpr int kBars = 2 * kStages + 8;
+  static constexpr int kSmem = kQBytes + kStages * kTileBytes + kBars * 8 + 16 + 1024;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return uint32_t(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// A whole warp's wait; false (for all its lanes) when it ran out here or in
+// another role.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
+  bool ok = bar_try(bar, parity);
+  for (uint32_t i = 0; !ok && i < kWaitRounds && !*gone; ++i) ok = bar_try(bar, parity);
+  if (!ok) *gone = 1;
+  return __all_sync(~0u, ok);
+}
+
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                       int token, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(token), "r"(head), "r"(page)
+      : "memory");
+}
+
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+// D[tmem] (+)= A B, both operands in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+
+#define TS_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), \
+                    "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define TS_W8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), \
+                    "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+// 32 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : TS_R8(r, 0), TS_R8(r, 8), TS_R8(r, 16), TS_R8(r, 24)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      TS_W8(r, 0), TS_W8(r, 8), TS_W8(r, 16), TS_W8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      TS_W8(r, 0), TS_W8(r, 8)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory operand descriptor in the 128-byte swizzle: rows of 128 bytes,
+// groups of eight rows 1024 bytes apart; `lead` is the distance between
+// 64-element blocks of an operand whose rows run along N (V).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  return uint64_t((addr >> 4) & 0x3fff) | uint64_t((lead >> 4) & 0x3fff) << 16 |
+         uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+
+// Instruction descriptor: 32-bit accumulator, operands of T (fp16 0, bf16 1),
+// M = 128, N = kN; B's rows along N when kAlongN.
+template <typename T, int kN, bool kAlongN>
+struct InstrDesc {
+  static constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  static constexpr uint32_t value = 1u << 4 | kType << 7 | kType << 10 |
+                                    (kAlongN ? 1u << 16 : 0u) | uint32_t(kN >> 3) << 17 |
+                                    uint32_t(128 >> 4) << 24;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A CTA's share of one unit.
+struct Segment {
+  int unit, tile, count;
+};
+struct Shares {
+  int64_t lo, hi;
+  int nt;
+  __device__ __forceinline__ bool next(Segment* s) {
+    if (lo >= hi) return false;
+    s->unit = int(lo / nt);
+    s->tile = int(lo - int64_t(s->unit) * nt);
+    const int64_t left = hi - lo;
+    s->count = int(left < nt - s->tile ? left : nt - s->tile);
+    lo += s->count;
+    return true;
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap) {
+  using S = Shape<D>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t q_smem = smem_u32(smem);
+  const uint32_t ring = q_smem + S::kQBytes;
+  uint8_t* ctl = smem + S::kQBytes + S::kStages * S::kTileBytes;
+  const uint32_t bars = smem_u32(ctl);
+  const uint32_t full = bars, empty = bars + 8 * S::kStages, q_full = bars + 16 * S::kStages,
+                 s_full = q_full + 16, p_ready = q_full + 32, o_full = q_full + 48;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 8 * S::kBars);
+  volatile int* gone = reinterpret_cast<volatile int*>(ctl + 8 * S::kBars + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  bool bad;
+  const int len = prefix_tokens(p.kv, p.a, &bad);
+  const int heads = int(p.kv.heads);
+  Shares shares{};
+  shares.nt = (len + kPrefixTile - 1) / kPrefixTile;
+  const int64_t total = int64_t(shares.nt) * p.row_tiles * heads;
+  if (bad && blockIdx.x == 0 && threadIdx.x == 0 && p.err)
+    *reinterpret_cast<volatile int*>(p.err) = 1;
+  const int64_t ctas = total < p.ctas ? total : p.ctas;
+  if (blockIdx.x >= ctas) return;
+  shares.lo = total * blockIdx.x / ctas;
+  shares.hi = total * (blockIdx.x + 1) / ctas;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      bar_init(full + 8 * i, 1);
+      bar_init(empty + 8 * i, 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      bar_init(q_full + 8 * x, 128);
+      bar_init(s_full + 8 * x, 1);
+      bar_init(p_ready + 8 * x, 128);
+      bar_init(o_full + 8 * x, 1);
+    }
+    *gone = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(tmem_slot))
+                 : "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem_s = tmem, tmem_o = tmem + 256;  // + 128 x and + D x for half x
+  const int32_t* table = reinterpret_cast<const int32_t*>(p.a.prefix_table);
+  const int bt = int(p.kv.block_tokens);
+  Segment seg;
+
+  if (warp == 8) {
+    // -- loads ----------------------------------------------------------------
+    const int pieces = kPrefixTile / p.piece;
+    uint32_t n = 0;  // tiles loaded, K and V counted apart
+    bool ok = true;
+    while (ok && shares.next(&seg)) {
+      const int head = seg.unit % heads;
+      for (int j = 0; ok && j < seg.count; ++j) {
+        // lane i < pieces places piece i; the page past the last one loads zeros
+        int page = int(p.kv.pages), off = 0;
+        const int t = (seg.tile + j) * kPrefixTile + lane * p.piece;
+        if (lane < pieces && t < len) {
+          const int blk = t / bt;
+          off = t - blk * bt;
+          const int id = table[blk];
+          if (id >= 0 && id < p.kv.pages) {
+            page = id;
+          } else if (p.err) {
+            *reinterpret_cast<volatile int*>(p.err) = 1;
+          }
+        }
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t st = n % S::kStages, round = n / S::kStages;
+          ok = bar_wait(empty + 8 * st, (round & 1) ^ 1, gone);
+          if (!ok) break;
+          if (lane == 0) bar_expect(full + 8 * st, S::kTileBytes);
+          __syncwarp();
+          if (lane < pieces) {
+            const uint32_t dst = ring + st * S::kTileBytes + lane * p.piece * 128;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              tma_4d(dst + h * kPrefixTile * 128, kv ? &vmap : &kmap, full + 8 * st, h * 64, off,
+                     head, page);
+          }
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // -- matrix products --------------------------------------------------------
+    constexpr uint32_t kIdescS = InstrDesc<T, kPrefixTile, false>::value;
+    constexpr uint32_t kIdescO = InstrDesc<T, D, true>::value;
+    uint32_t n = 0;              // ring position (as the loads')
+    uint32_t q_n[2] = {0, 0}, p_n[2] = {0, 0};
+    bool ok = true;
+    auto scores = [&](int x, uint32_t st) {
+      if (lane == 0) {
+        const uint32_t a = q_smem + x * 128 * 128, b = ring + st * S::kTileBytes;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          // 64 elements (four steps) per 128-byte block
+          const uint64_t ad = smem_desc(a + (k / 4) * kPrefixRows * 128 + (k % 4) * 32, 16);
+          const uint64_t bd = smem_desc(b + (k / 4) * kPrefixTile * 128 + (k % 4) * 32, 16);
+          mma_ss(tmem_s + 128 * x, ad, bd, kIdescS, k > 0);
+        }
+        commit(s_full + 8 * x);
+      }
+      __syncwarp();
+    };
+    while (ok && shares.next(&seg)) {
+      const int rt = seg.unit / heads;
+      const int halves = p.rows - rt * kPrefixRows > 128 ? 2 : 1;
+      ok = bar_wait(full + 8 * (n % S::kStages), (n / S::kStages) & 1, gone);
+      for (int x = 0; ok && x < halves; ++x) {
+        ok = bar_wait(q_full + 8 * x, q_n[x] & 1, gone);
+        ++q_n[x];
+        fence_after();
+        if (ok) scores(x, n % S::kStages);
+      }
+      if (lane == 0) commit(empty + 8 * (n % S::kStages));
+      ++n;
+      for (int j = 0; ok && j < seg.count; ++j) {
+        const uint32_t vst = n % S::kStages;
+        ok = bar_wait(full + 8 * vst, (n / S::kStages) & 1, gone);
+        const int past = len - (seg.tile + j) * kPrefixTile;  // keys of this tile that count
+        if (ok && past < kPrefixTile) {
+          // V rows past the length: whatever the page holds must not meet a weight of 0
+          for (int i = lane; i < (kPrefixTile - past) * (D / 64) * 8; i += 32) {
+            const int r = past + i / (D / 64 * 8), c = i % (D / 64 * 8);
+            const uint32_t at = ring + vst * S::kTileBytes + (c / 8) * kPrefixTile * 128 +
+                                r * 128 + (c % 8) * 16;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        const bool more = j + 1 < seg.count;
+        for (int x = 0; ok && x < halves; ++x) {
+          ok = bar_wait(p_ready + 8 * x, p_n[x] & 1, gone);
+          ++p_n[x];
+          fence_after();
+          if (!ok) break;
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < kPrefixTile / 16; ++k)
+              mma_ts(tmem_o + D * x, tmem_s + 128 * x + 8 * k,
+                     smem_desc(ring + vst * S::kTileBytes + k * 16 * 128, kPrefixTile * 128),
+                     kIdescO, j > 0 || k > 0);
+            if (!more) commit(o_full + 8 * x);
+          }
+          __syncwarp();
+          if (more) {
+            if (x == 0)
+              ok = bar_wait(full + 8 * ((n + 1) % S::kStages), ((n + 1) / S::kStages) & 1, gone);
+            if (ok) scores(x, (n + 1) % S::kStages);
+          }
+        }
+        if (lane == 0) {
+          commit(empty + 8 * vst);
+          if (more) commit(empty + 8 * ((n + 1) % S::kStages));
+        }
+        n += more ? 2 : 1;
+      }
+    }
+  } else {
+    // -- softmax ----------------------------------------------------------------
+    const int x = warp >> 2;               // half
+    const int r = threadIdx.x & 127;       // row of the half
+    const uint32_t lanes = uint32_t(warp & 3) << 21;  // this warp's TMEM lanes
+    const uint32_t ts = tmem_s + 128 * x + lanes, to = tmem_o + D * x + lanes;
+    uint32_t s_n = 0, o_n = 0;
+    bool ok = true;
+    while (ok && shares.next(&seg)) {
+      const int head = seg.unit % heads, rt = seg.unit / heads;
+      const int row0 = rt * kPrefixRows + x * 128;
+      if (x == 1 && row0 >= p.rows) continue;
+      // this half's queries into shared memory: 16 bytes a thread, rows swizzled
+      {
+        constexpr int kC = D / 8;
+        const int c = r % kC;
+#pragma unroll 8
+        for (int i = 0; i < kC; ++i) {
+          const int rr = i * (128 / kC) + r / kC;
+          const int row = row0 + rr;
+          int4 v = make_int4(0, 0, 0, 0);
+          if (row < p.rows) {
+            const int64_t tok = row / p.group;
+            const int64_t b = tok / p.a.new_tokens, jj = tok - b * p.a.new_tokens;
+            v = *reinterpret_cast<const int4*>(
+                reinterpret_cast<const T*>(p.a.q) + b * p.a.q_batch_stride +
+                jj * p.a.q_token_stride +
+                (head * p.group + row - tok * p.group) * p.a.q_head_stride + c * 8);
+          }
+          const uint32_t at = q_smem + (c / 8) * kPrefixRows * 128 + (x * 128 + rr) * 128 +
+                              (((c % 8) ^ (rr & 7)) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y),
+                       "r"(v.z), "r"(v.w)
+                       : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        bar_arrive(q_full + 8 * x);
+      }
+      // whether any page of the segment is bad: then every tile is looked at
+      bool hole = false;
+      {
+        const int first = seg.tile * kPrefixTile / bt;
+        const int last = min(len, (seg.tile + seg.count) * kPrefixTile);
+        for (int b = first + lane; b * int64_t(bt) < last; b += 32) {
+          const int id = table[b];
+          hole = hole || id < 0 || id >= p.kv.pages;
+        }
+        hole = __any_sync(~0u, hole);
+      }
+
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < seg.count; ++j) {
+        ok = bar_wait(s_full + 8 * x, s_n & 1, gone);
+        ++s_n;
+        if (!ok) break;
+        fence_after();
+        float s[kPrefixTile];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_ld32(reinterpret_cast<uint32_t*>(s) + 32 * c, ts + 32 * c);
+        tmem_wait_ld();
+        const int t0 = (seg.tile + j) * kPrefixTile;
+        if (hole || t0 + kPrefixTile > len) {
+          for (int c = 0; c < 4; ++c) {
+            const int t = t0 + 32 * c + lane;
+            bool in = t < len;
+            if (in && hole) {
+              const int id = table[t / bt];
+              in = id >= 0 && id < p.kv.pages;
+            }
+            const uint32_t mask = __ballot_sync(~0u, in);
+#pragma unroll
+            for (int k = 0; k < kPrefixTile; ++k)
+              if (k / 32 == c && !((mask >> (k % 32)) & 1)) s[k] = -INFINITY;
+          }
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int k = 4; k < kPrefixTile; ++k) mx[k % 4] = fmaxf(mx[k % 4], s[k]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        const bool grew = top > m + 8.f;
+        if (__any_sync(~0u, grew)) {
+          const float f = grew ? ex2(m - top) : 1.f;
+          if (grew) m = top;
+          l *= f;
+          if (j > 0) {
+            // the products up to the last tile are done: s_full was committed after them
+            uint32_t o[32];
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              tmem_ld32(o, to + 32 * c);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st32(to + 32 * c, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float a = ex2(fmaf(s[32 * c + 2 * k], p.scale_log2, -base));
+            const float b = ex2(fmaf(s[32 * c + 2 * k + 1], p.scale_log2, -base));
+            sum[k % 2 * 2] += a;
+            sum[k % 2 * 2 + 1] += b;
+            pk[k] = pack2(a, b, T{});
+          }
+          tmem_st16(ts + 16 * c, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        fence_before();
+        bar_arrive(p_ready + 8 * x);
+      }
+      if (!ok) break;
+      ok = bar_wait(o_full + 8 * x, o_n & 1, gone);
+      ++o_n;
+      if (!ok) break;
+      fence_after();
+      // the row's partial
+      const int row = row0 + r;
+      float *da = nullptr, *dm = nullptr;
+      if (row < p.rows) {
+        if (seg.count == shares.nt) {
+          const int64_t tok = row / p.group;
+          const int64_t out_row = tok * p.a.q_heads + head * p.group + row - tok * p.group;
+          da = p.whole_acc + out_row * D;
+          dm = p.whole_ml + out_row * 2;
+        } else {
+          const int64_t slot = (int64_t(blockIdx.x) * 2 + (seg.tile == 0 ? 1 : 0)) * kPrefixRows +
+                               x * 128 + r;
+          da = p.slots_acc + slot * D;
+          dm = p.slots_ml + slot * 2;
+        }
+        *reinterpret_cast<float2*>(dm) = make_float2(m, l);
+      }
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o, to + 32 * c);
+        tmem_wait_ld();
+        if (da) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<uint4*>(da + 32 * c + 4 * k) =
+                make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      }
+      fence_before();
+    }
+  }
+
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (*gone) {
+    // a wait ran out: give copies and products in flight time to land before
+    // the shared memory and TMEM they target are given back
+    if (threadIdx.x == 0 && p.err) *reinterpret_cast<volatile int*>(p.err) = 2;
+    for (int i = 0; i < 100; ++i) __nanosleep(100000);
+    __syncthreads();
+  }
+  if (warp == 9)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) !=
+            cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// [pages][heads][tokens][D] with the storage's strides; boxes of 64 elements x
+// `piece` tokens.
+int make_map(CUtensorMap* map, const ts_paged_kv& kv, bool v, int piece) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return set_error(TS_INTERNAL, "cuTensorMapEncodeTiled is not available");
+  const int64_t st[3] = {v ? kv.v_token_stride : kv.k_token_stride,
+                         v ? kv.v_head_stride : kv.k_head_stride,
+                         v ? kv.v_page_stride : kv.k_page_stride};
+  const int64_t n[3] = {kv.block_tokens, kv.heads, kv.pages};
+  cuuint64_t dims[4] = {cuuint64_t(kv.head_dim), cuuint64_t(n[0]), cuuint64_t(n[1]),
+                        cuuint64_t(n[2])};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i)  // the stride of a dimension of one is never used
+    strides[i] = n[i] > 1 ? cuuint64_t(st[i]) * 2 : cuuint64_t(kv.head_dim) * 2;
+  const cuuint32_t box[4] = {64, cuuint32_t(piece), 1, 1};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult rc = fn(map,
+                         kv.dtype == TS_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         4, reinterpret_cast<void*>(v ? kv.v_ptr : kv.k_ptr), dims, strides, box,
+                         ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return set_errorf(TS_INTERNAL, "tensor map: CUDA driver error %d", int(rc));
+  return TS_OK;
+}
+
+template <typename T, int D>
+int launch(const PrefixParams& p, const CUtensorMap& k, const CUtensorMap& v, int device,
+           cudaStream_t s) {
+  static bool ready[64] = {};
+  if (device >= 64 || !ready[device]) {
+    TS_CUDA_RET(cudaFuncSetAttribute(prefix_kernel<T, D>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem),
+                "prefix attention shared memory");
+    if (device < 64) ready[device] = true;
+  }
+  prefix_kernel<T, D><<<p.ctas, kThreads, Shape<D>::kSmem, s>>>(p, k, v);
+  TS_CUDA_RET(cudaGetLastError(), "prefix attention launch");
+  return TS_OK;
+}
+
+}  // namespace
+
+bool prefix_geometry_ok(const ts_paged_kv& kv) {
+  // a box of whole swizzle groups (eight tokens); strides as tensor maps take them
+  if (kv.pages < 1 || std::gcd(kv.block_tokens, int64_t(kPrefixTile)) < 8) return false;
+  const int64_t limit = int64_t(1) << 39;  // elements: 2^40 bytes
+  for (int64_t x : {kv.k_page_stride, kv.k_token_stride, kv.k_head_stride, kv.v_page_stride,
+                    kv.v_token_stride, kv.v_head_stride})
+    if (x >= limit) return false;
+  return true;
+}
+
+int launch_prefix(const PrefixParams& p, int device, cudaStream_t s) {
+  CUtensorMap k, v;
+  if (int rc = make_map(&k, p.kv, false, p.piece)) return rc;
+  if (int rc = make_map(&v, p.kv, true, p.piece)) return rc;
+  if (p.kv.dtype == TS_DTYPE_BF16)
+    return p.kv.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, k, v, device, s)
+                               : launch<__nv_bfloat16, 128>(p, k, v, device, s);
+  return p.kv.head_dim == 64 ? launch<__half, 64>(p, k, v, device, s)
+                             : launch<__half, 128>(p, k, v, device, s);
+}
+
+}  // namespace tsb
