@@ -279,10 +279,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
   float* join = reinterpret_cast<float*>(smem + kWarps * kStages * stage_bytes<D>());
   uint32_t* masks = reinterpret_cast<uint32_t*>(join + join_floats<D>()) + warp * kStages;
 
+  // Lets join_kernel take SMs as they fall free.  With a prefix kernel before
+  // it, this one may itself run early: it reads nothing that kernel writes, and
+  // waits for it before it ends, so that join_kernel's wait covers both.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t seqs = p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0);
   const int64_t total = tiles_before(p, seqs);
   const int64_t ctas = sharers(total, p.ctas);
-  if (blockIdx.x >= ctas) return;
+  if (blockIdx.x >= ctas) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int64_t lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
   Cursor ld, cu;
   cu.start(p, lo, hi - lo);
@@ -576,23 +583,24 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
     cu.next_item(p);
   }
   cp_wait<0>();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Where one part (own or prefix) of a query row lies: `count` partials, the
-// i-th at acc + i * stride rows (slots of consecutive CTAs), except that the
-// first may sit in a CTA's second slot.
+// first at row `first`, the others from row `next` on, `step` rows apart (the
+// slots of consecutive CTAs).
 struct Part {
-  const float* acc0;
-  const float* ml0;
-  const float* acc1;  // the second and later ones, one CTA (two slots) apart
-  const float* ml1;
-  int step;           // rows between them
-  int count;
+  const float* acc;
+  const float* ml;
+  int64_t first, next;
+  int step, count;
+  __device__ __forceinline__ int64_t row(int i) const {
+    return i == 0 ? first : next + int64_t(i - 1) * step;
+  }
 };
 
 // The part of a row (row rl of an item's `rows`) whose item holds the tiles
 // [start, start + nt) of `total`, shared by `ctas` CTAs.
-template <int D>
 __device__ __forceinline__ Part part_of(int64_t total, int64_t ctas, int64_t start, int nt,
                                         int rows, int rl, const float* slots_acc,
                                         const float* slots_ml, const float* whole_acc,
@@ -602,90 +610,142 @@ __device__ __forceinline__ Part part_of(int64_t total, int64_t ctas, int64_t sta
   // owner of tile t: the CTA whose share holds it
   const int64_t w0 = ((start + 1) * ctas - 1) / total;
   const int64_t w1 = ((start + nt) * ctas - 1) / total;
-  if (w0 == w1) {
-    r.count = 1;
-    r.acc0 = whole_acc + out_row * D;
-    r.ml0 = whole_ml + out_row * 2;
+  r.count = int(w1 - w0) + 1;
+  if (r.count == 1) {
+    r.acc = whole_acc;
+    r.ml = whole_ml;
+    r.first = out_row;
     return r;
   }
-  r.count = int(w1 - w0) + 1;
   // the first CTA begins the item (its second slot); the others go on with it
-  const int64_t s0 = (w0 * 2 + 1) * rows + rl, s1 = (w0 + 1) * 2 * rows + rl;
-  r.acc0 = slots_acc + s0 * D;
-  r.ml0 = slots_ml + s0 * 2;
+  r.acc = slots_acc;
+  r.ml = slots_ml;
+  r.first = (w0 * 2 + 1) * rows + rl;
+  r.next = (w0 + 1) * 2 * rows + rl;
   r.step = 2 * rows;
-  r.acc1 = slots_acc + s1 * D;
-  r.ml1 = slots_ml + s1 * 2;
   return r;
 }
 
-// One warp per query row: joins the partials of its own part and of its
+// kSplit warps per query row join the partials of its own part and of its
 // prefix part.  Rows that walk_kernel finished itself are left alone; rows
-// whose sequence is empty are written here.
-template <typename T, int D, int MT>
+// whose sequence is empty are written here.  All that depends on the lengths
+// alone is done before waiting for the kernels that write the partials.
+template <typename T, int D, int MT, int kSplit>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkParams p) {
   constexpr int kRows = 16 * MT, kPer = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t out_row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (out_row >= p.a.batch * p.a.new_tokens * p.a.q_heads) return;
-  const int64_t tok = out_row / p.a.q_heads;
-  const int hq = int(out_row - tok * p.a.q_heads);
-  const int64_t b = tok / p.a.new_tokens;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n_rows = p.a.batch * p.a.new_tokens * p.a.q_heads;
+  const int64_t out_row = kSplit == 1 ? int64_t(blockIdx.x) * 4 + warp : int64_t(blockIdx.x);
+  if (out_row >= n_rows) return;
+  const int tok = int(out_row / p.a.q_heads);
+  const int hq = int(out_row) - tok * int(p.a.q_heads);
+  const int b = tok / int(p.a.new_tokens);
   const int head = hq / p.group;
   const int64_t heads = p.kv.heads;
-  const int64_t own_total = tiles_before(p, p.a.batch);
   bool bad;
-  const int64_t total = own_total + (p.row_tiles_pre > 0 ? tiles_of(p, p.a.batch, &bad) : 0);
+  // tiles of all sequences, and of those before b
+  int64_t total = 0, before = 0;
+  for (int i = lane; i < p.a.batch; i += 32) {
+    const int64_t t = tiles_of(p, i, &bad);
+    total += t;
+    before += i < b ? t : 0;
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) {
+    total += __shfl_xor_sync(~0u, total, k);
+    before += __shfl_xor_sync(~0u, before, k);
+  }
+  const int64_t own_total = total;
+  if (p.row_tiles_pre > 0) total += tiles_of(p, p.a.batch, &bad);
 
-  Part parts[2] = {};
   const int64_t ctas = sharers(total, p.ctas);
-  {
-    const int nt = (tokens_of(p, b, &bad) + kTile - 1) / kTile;
-    const int row = int(tok - b * p.a.new_tokens) * p.group + hq % p.group;
-    const int64_t start = tiles_before(p, b) + (int64_t(row / kRows) * heads + head) * nt;
-    parts[0] = part_of<D>(total, ctas, start, nt, kRows, row % kRows, p.slots_acc, p.slots_ml,
-                          p.own_acc, p.own_ml, out_row);
-    if (p.a.prefix_blocks == 0 && parts[0].count == 1) return;  // written by walk_kernel
-  }
-  const int64_t row = tok * p.group + hq % p.group;
+  const int nt = (tokens_of(p, b, &bad) + kTile - 1) / kTile;
+  const int own_row = (tok - b * int(p.a.new_tokens)) * p.group + hq % p.group;
+  const Part own = part_of(total, ctas, before + (own_row / kRows * heads + head) * nt, nt, kRows,
+                           own_row % kRows, p.slots_acc, p.slots_ml, p.own_acc, p.own_ml, out_row);
+  if (p.a.prefix_blocks == 0 && own.count == 1) return;  // written by walk_kernel
+  const int64_t row = int64_t(tok) * p.group + hq % p.group;
+  Part pre{};
   if (p.row_tiles_pre > 0) {
-    const int nt = (tokens_of(p, p.a.batch, &bad) + kTile - 1) / kTile;
-    const int64_t start = own_total + (row / kRows * heads + head) * nt;
-    parts[1] = part_of<D>(total, ctas, start, nt, kRows, int(row % kRows), p.slots_acc,
-                          p.slots_ml, p.pre_acc, p.pre_ml, out_row);
+    const int n = (tokens_of(p, p.a.batch, &bad) + kTile - 1) / kTile;
+    pre = part_of(total, ctas, own_total + (row / kRows * heads + head) * n, n, kRows,
+                  int(row % kRows), p.slots_acc, p.slots_ml, p.pre_acc, p.pre_ml, out_row);
   } else if (p.tensor_ctas > 0) {
-    const int nt = (tokens_of(p, p.a.batch, &bad) + kPrefixTile - 1) / kPrefixTile;
-    const int64_t all = int64_t(nt) * p.tensor_row_tiles * heads;
-    parts[1] = part_of<D>(all, sharers(all, p.tensor_ctas), (row / kPrefixRows * heads + head) * nt,
-                          nt, kPrefixRows, int(row % kPrefixRows), p.tensor_acc, p.tensor_ml,
-                          p.pre_acc, p.pre_ml, out_row);
+    const int n = (tokens_of(p, p.a.batch, &bad) + kPrefixTile - 1) / kPrefixTile;
+    const int64_t all = int64_t(n) * p.tensor_row_tiles * heads;
+    pre = part_of(all, sharers(all, p.tensor_ctas), (row / kPrefixRows * heads + head) * n, n,
+                  kPrefixRows, int(row % kPrefixRows), p.tensor_acc, p.tensor_ml, p.pre_acc,
+                  p.pre_ml, out_row);
   }
-  const int n0 = parts[0].count, n = n0 + parts[1].count;
-  auto at = [&](int i, const float** acc, const float** ml) {
-    const Part& q = parts[i < n0 ? 0 : 1];
-    const int k = i < n0 ? i : i - n0;
-    *acc = k == 0 ? q.acc0 : q.acc1 + int64_t(k - 1) * q.step * D;
-    *ml = k == 0 ? q.ml0 : q.ml1 + int64_t(k - 1) * q.step * 2;
-  };
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 32) {
-    const float *acc, *ml;
-    at(i, &acc, &ml);
-    m = fmaxf(m, ml[0]);
-  }
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, k));
-  const float base = m == -INFINITY ? 0.f : m;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // 32 partials at a time (this warp's of every kSplit): their weights, then
+  // their rows
+  float m = -INFINITY, l = 0.f;
   float o[kPer] = {};
-  float l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float *acc, *ml;
-    at(i, &acc, &ml);
-    const float w = ex2(ml[0] - base);
-    l += ml[1] * w;
+  const int n = own.count + pre.count;
+  const int mine = kSplit == 1 ? n : (n - warp + kSplit - 1) / kSplit;
+  for (int i0 = 0; i0 < mine; i0 += 32) {
+    const int i = kSplit == 1 ? i0 + lane : (i0 + lane) * kSplit + warp;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    const float* acc = nullptr;
+    if (i < n) {
+      const bool first = i < own.count;
+      const int64_t at = first ? own.row(i) : pre.row(i - own.count);
+      ml = *reinterpret_cast<const float2*>((first ? own.ml : pre.ml) + at * 2);
+      acc = (first ? own.acc : pre.acc) + at * D;
+    }
+    float top = ml.x;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] += acc[lane * kPer + e] * w;
+    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
+    const float mn = fmaxf(m, top);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float w = ex2(ml.x - base), corr = ex2(m - base);
+    float lw = ml.y * w;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) lw += __shfl_xor_sync(~0u, lw, k);
+    l = l * corr + lw;
+    m = mn;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] *= corr;
+    const int count = min(32, mine - i0);
+#pragma unroll 8
+    for (int k = 0; k < count; ++k) {
+      const float wk = __shfl_sync(~0u, w, k);
+      const float* src = reinterpret_cast<const float*>(
+          __shfl_sync(~0u, reinterpret_cast<uint64_t>(acc), k)) + lane * kPer;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + e);
+        o[e] += v.x * wk;
+        o[e + 1] += v.y * wk;
+      }
+    }
+  }
+  if constexpr (kSplit > 1) {
+    __shared__ float part[kSplit][D + 2];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) part[warp][lane * kPer + e] = o[e];
+    if (lane == 0) {
+      part[warp][D] = m;
+      part[warp][D + 1] = l;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kSplit; ++k) m = fmaxf(m, part[k][D]);
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSplit; ++k) {
+      const float w = ex2(part[k][D] - base);
+      l += part[k][D + 1] * w;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] += part[k][lane * kPer + e] * w;
+    }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   T* out = reinterpret_cast<T*>(p.a.out) + out_row * D + lane * kPer;
@@ -694,6 +754,24 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkP
     *reinterpret_cast<uint32_t*>(out + e) = Ops<T>::pack(o[e] * inv, o[e + 1] * inv);
   if (p.a.lse && lane == 0)
     reinterpret_cast<float*>(p.a.lse)[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Launches on `s`; `early`: may start while the kernel before it in the stream
+// still runs (it waits for that kernel's results itself).
+template <typename... Args>
+cudaError_t launch_on(void (*kernel)(Args...), unsigned grid, unsigned block, size_t smem,
+                      cudaStream_t s, bool early, Args... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(block);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &attr;
+  c.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
 int check_attention(const ts_paged_kv* kv, const ts_attention_args* args) {
@@ -767,11 +845,17 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
                 "attention shared memory");
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  walk_kernel<T, D, MT><<<p.ctas, kWarps * 32, walk_smem<D>(), s>>>(p);
-  TS_CUDA_RET(cudaGetLastError(), "attention launch");
+  TS_CUDA_RET(launch_on(walk_kernel<T, D, MT>, unsigned(p.ctas), kWarps * 32, walk_smem<D>(), s,
+                        p.tensor_ctas > 0, p),
+              "attention launch");
+  // Few items leave many partials to each row, which then takes four warps.
   const int64_t rows = p.a.batch * p.a.new_tokens * p.a.q_heads;
-  join_kernel<T, D, MT><<<unsigned((rows + 3) / 4), 128, 0, s>>>(p);
-  TS_CUDA_RET(cudaGetLastError(), "attention join launch");
+  const int64_t items = p.a.batch * p.row_tiles_own * p.kv.heads +
+                        int64_t(p.row_tiles_pre) * p.kv.heads;
+  const bool many = p.ctas >= 8 * items;
+  TS_CUDA_RET(launch_on(many ? join_kernel<T, D, MT, 4> : join_kernel<T, D, MT, 1>,
+                        unsigned(many ? rows : (rows + 3) / 4), 128, 0, s, true, p),
+              "attention join launch");
   return TS_OK;
 }
 

@@ -234,6 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 8 * S::kBars);
   volatile int* gone = reinterpret_cast<volatile int*>(ctl + 8 * S::kBars + 4);
 
+  // the walk over the sequences' own pages may take SMs as they fall free
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   bool bad;
   const int len = prefix_tokens(p.kv, p.a, &bad);

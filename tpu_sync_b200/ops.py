@@ -404,11 +404,6 @@ def kv_relayout(src_storages: Sequence, dst_storages: Sequence, src_geom: dict,
   return err
 
 
-def _on(stream: Optional[torch.cuda.Stream]):
-  """What a call allocates or converts belongs to the stream it runs on."""
-  return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
-
-
 _PAGE_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 
 
@@ -448,38 +443,49 @@ class PagedKV:
         _PAGE_DTYPES[self.dtype], 0)
     self._ref = ctypes.byref(self._c)
     self._index = self.device.index
+    self._workspace = {}  # bytes of attention workspace by shapes
 
 
-def _check_heads(kv: PagedKV, name: str, t: torch.Tensor, tokens: int, heads: Optional[int]):
-  if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != kv.head_dim or (
-      heads is not None and t.shape[1] != heads):
-    raise ValueError(f"{name} must be [{tokens}, {heads or 'heads'}, {kv.head_dim}], got "
-                     f"{list(t.shape)}")
-  _check_like(kv, name, t)
-
-
-def _check_like(kv: PagedKV, name: str, t: torch.Tensor):
+def _heads(kv: PagedKV, name: str, t: torch.Tensor, shape: Tuple[int, ...]) -> Tuple[int, ...]:
+  """Strides of a tensor of heads of this shape, checked."""
+  strides = t.stride()
+  if (t.shape == shape and t.dtype is kv.dtype and t.get_device() == kv._index and
+      (strides[-1] == 1 or shape[-1] <= 1) and not (t.requires_grad and torch.is_grad_enabled())):
+    return strides
+  if t.shape != shape:
+    raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
   if t.dtype != kv.dtype or t.device != kv.device:
     raise ValueError(f"{name} must have the pages' dtype and device")
-  if t.stride(-1) != 1 and t.shape[-1] > 1:
-    raise ValueError(f"the last dimension of {name} must be contiguous")
   if t.requires_grad and torch.is_grad_enabled():
     raise ValueError(f"{name} requires grad: the paged cache operators have no backward pass")
+  raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
-def _check_index(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int, device):
-  if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != dims or t.device != device:
-    raise ValueError(f"{name} must be a {dims}-dimensional {dtype} tensor on {device}")
-  if t.stride(-1) != 1 and t.shape[-1] > 1:
+def _index(kv: PagedKV, name: str, t: torch.Tensor, dtype: torch.dtype, dims: int,
+           length: Optional[int]) -> Tuple[int, ...]:
+  """Shape of an index tensor, a table or a weight, checked; `length`: of its first dimension."""
+  if not isinstance(t, torch.Tensor):
+    raise ValueError(f"{name} must be a tensor")
+  shape = t.shape
+  if t.dtype is not dtype or len(shape) != dims or t.get_device() != kv._index:
+    raise ValueError(f"{name} must be a {dims}-dimensional {dtype} tensor on {kv.device}")
+  if t.stride()[-1] != 1 and shape[-1] > 1:
     raise ValueError(f"the last dimension of {name} must be contiguous")
+  if length is not None and shape[0] != length:
+    raise ValueError(f"{name} must hold {length} entries, got {list(shape)}")
+  return shape
 
 
-def _check_flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
+def _flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
   if err_flag is None:
     return 0
   if err_flag.dtype != torch.int32 or err_flag.device != kv.device or err_flag.numel() < 1:
     raise ValueError("err_flag must be an int32 tensor on the pages' device")
   return err_flag.data_ptr()
+
+
+def _new_like(q: torch.Tensor) -> torch.Tensor:
+  return torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
 def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -508,128 +514,139 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
   cos_sin writes nothing for its token and sets err_flag (int32, on the device)
   to 1.
   """
-  tokens = k.shape[0] if k.dim() else 0
-  _check_heads(kv, "k", k, tokens, kv.heads)
-  _check_heads(kv, "v", v, tokens, kv.heads)
-  _check_index("slots", slots, torch.int64, 1, kv.device)
-  if slots.shape[0] != tokens:
-    raise ValueError(f"slots must hold {tokens} entries")
-  flag = _check_flag(kv, err_flag)
+  shape = k.shape
+  if len(shape) != 3 or shape[1:] != (kv.heads, kv.head_dim):
+    raise ValueError(f"k must be [tokens, {kv.heads}, {kv.head_dim}], got {list(shape)}")
+  tokens = shape[0]
   a = _native.KvAppendArgs()
+  a.k_token_stride, a.k_head_stride, _ = _heads(kv, "k", k, shape)
+  a.v_token_stride, a.v_head_stride, _ = _heads(kv, "v", v, shape)
+  _index(kv, "slots", slots, torch.int64, 1, tokens)
   a.k, a.v, a.slots, a.tokens = k.data_ptr(), v.data_ptr(), slots.data_ptr(), tokens
-  a.k_token_stride, a.k_head_stride, _ = k.stride()
-  a.v_token_stride, a.v_head_stride, _ = v.stride()
   if cos_sin is not None:
-    _check_index("positions", positions, torch.int64, 1, kv.device)
-    _check_index("cos_sin", cos_sin, torch.float32, 2, kv.device)
-    if positions.shape[0] != tokens:
-      raise ValueError(f"positions must hold {tokens} entries")
-    a.positions, a.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
-    a.max_position, a.rotary = cos_sin.shape
-    a.cos_sin_stride = cos_sin.stride(0) if a.max_position > 1 else a.rotary
-    a.interleaved = bool(interleaved)
-    if a.max_position == 0:
+    _index(kv, "positions", positions, torch.int64, 1, tokens)
+    rows, rotary = _index(kv, "cos_sin", cos_sin, torch.float32, 2, None)
+    if rows == 0:
       raise ValueError("cos_sin has no rows")
+    a.positions, a.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
+    a.max_position, a.rotary = rows, rotary
+    a.cos_sin_stride = cos_sin.stride(0) if rows > 1 else rotary
+    a.interleaved = bool(interleaved)
   elif interleaved or positions is not None:
     raise ValueError("positions and interleaved need cos_sin")
   if q_weight is not None or k_weight is not None:
     w = q_weight if q_weight is not None else k_weight
     if w.dtype not in (kv.dtype, torch.float32):
       raise ValueError("norm weights must be float32 or of the pages' dtype")
+    if q_weight is not None and q is None:
+      raise ValueError("q_weight needs q")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
       if t is None:
         continue
-      _check_index(name, t, w.dtype, 1, kv.device)
-      if t.shape[0] != kv.head_dim:
-        raise ValueError(f"{name} must hold {kv.head_dim} entries")
+      _index(kv, name, t, w.dtype, 1, kv.head_dim)
       if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires grad: the paged cache operators have no backward pass")
-    a.q_weight = q_weight.data_ptr() if q_weight is not None else 0
-    a.k_weight = k_weight.data_ptr() if k_weight is not None else 0
+      setattr(a, name, t.data_ptr())
     a.weight_dtype = _TORCH_TO_TS[w.dtype]
     a.eps = eps
-    if q_weight is not None and q is None:
-      raise ValueError("q_weight needs q")
   if q is not None:
-    _check_heads(kv, "q", q, tokens, None)
+    heads = q.shape[1] if q.dim() == 3 else 0
+    if heads == 0:
+      raise ValueError(f"q must be [{tokens}, heads, {kv.head_dim}], got {list(q.shape)}")
+    shape = (tokens, heads, kv.head_dim)
+    a.q_token_stride, a.q_head_stride, _ = _heads(kv, "q", q, shape)
     if q_out is None:
-      with _on(stream):
-        q_out = torch.empty(q.shape, dtype=kv.dtype, device=kv.device)
+      if stream is None:
+        q_out = _new_like(q)
+      else:
+        with torch.cuda.stream(stream):  # what a call allocates belongs to its stream
+          q_out = _new_like(q)
+      a.q_out_token_stride, a.q_out_head_stride = heads * kv.head_dim, kv.head_dim
       a.zero_padding = 1
     else:
-      _check_heads(kv, "q_out", q_out, tokens, q.shape[1])
-    a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-    a.q_token_stride, a.q_head_stride, _ = q.stride()
-    a.q_out_token_stride, a.q_out_head_stride, _ = q_out.stride()
-    if a.q_heads == 0:
-      raise ValueError("q needs at least one head")
+      a.q_out_token_stride, a.q_out_head_stride, _ = _heads(kv, "q_out", q_out, shape)
+    a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), heads
   elif q_out is not None:
     raise ValueError("q_out needs q")
-  _native.check(_native.lib().ts_kv_append(kv._index, kv._ref, ctypes.byref(a), flag,
-                                           _stream(stream, kv.device)), "kv_append: ")
+  rc = _native.lib().ts_kv_append(kv._index, kv._ref, ctypes.byref(a), _flag(kv, err_flag),
+                                  torch._C._cuda_getCurrentRawStream(kv._index)
+                                  if stream is None else stream.cuda_stream)
+  if rc:
+    _native.check(rc, "kv_append: ")
   return q_out
 
 
 def _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, out, return_lse,
                err_flag, stream):
-  if q.dim() == 3:
-    batch, q_heads, dim = q.shape
+  shape = q.shape
+  if len(shape) == 3:
+    batch, q_heads, dim = shape
     new = 1
-  elif q.dim() == 4:
-    batch, new, q_heads, dim = q.shape
+  elif len(shape) == 4:
+    batch, new, q_heads, dim = shape
   else:
     raise ValueError("q must be [batch, q_heads, head_dim] or [batch, new_tokens, q_heads, "
                      "head_dim]")
   if dim != kv.head_dim or q_heads == 0:
     raise ValueError(f"q heads must have {kv.head_dim} elements")
-  _check_like(kv, "q", q)
-  _check_index("block_table", block_table, torch.int32, 2, kv.device)
-  _check_index("seq_lens", seq_lens, torch.int32, 1, kv.device)
-  if block_table.shape[0] != batch or seq_lens.shape[0] != batch:
-    raise ValueError(f"block_table and seq_lens must hold {batch} sequences")
-  flag = _check_flag(kv, err_flag)
   a = _native.AttentionArgs()
+  strides = _heads(kv, "q", q, shape)
+  blocks = _index(kv, "block_table", block_table, torch.int32, 2, batch)[1]
+  _index(kv, "seq_lens", seq_lens, torch.int32, 1, batch)
   a.q, a.batch, a.new_tokens, a.q_heads = q.data_ptr(), batch, new, q_heads
-  strides = q.stride()
   # a dimension of one element is never stepped over: its stride says nothing
   a.q_batch_stride = strides[0] if batch > 1 else 0
   a.q_token_stride = strides[1] if new > 1 else 0
   a.q_head_stride = strides[-2] if q_heads > 1 else 0
-  a.block_table, a.max_blocks = block_table.data_ptr(), block_table.shape[1]
+  a.block_table, a.max_blocks = block_table.data_ptr(), blocks
   a.block_table_stride = block_table.stride(0) if batch > 1 else 0
   a.seq_lens = seq_lens.data_ptr()
   a.scale = dim ** -0.5 if scale is None else scale
+  prefix_blocks = 0
   if prefix_table is not None:
-    _check_index("prefix_table", prefix_table, torch.int32, 1, kv.device)
-    a.prefix_table, a.prefix_blocks = prefix_table.data_ptr(), prefix_table.shape[0]
+    prefix_blocks, = _index(kv, "prefix_table", prefix_table, torch.int32, 1, None)
+    a.prefix_table, a.prefix_blocks = prefix_table.data_ptr(), prefix_blocks
     if isinstance(prefix_len, torch.Tensor):
       if prefix_len.dtype != torch.int32 or prefix_len.device != kv.device or (
           prefix_len.numel() != 1):
         raise ValueError("prefix_len must be an int or one int32 on the pages' device")
       a.prefix_len_dev, a.prefix_len = prefix_len.data_ptr(), 2**31 - 1
     else:
-      if not 0 <= prefix_len <= a.prefix_blocks * kv.block_tokens:
+      if not 0 <= prefix_len <= prefix_blocks * kv.block_tokens:
         raise ValueError(f"prefix_table does not hold {prefix_len} tokens")
       a.prefix_len = prefix_len
   if out is not None:
-    _check_like(kv, "out", out)
-    if out.shape != q.shape or not out.is_contiguous():
-      raise ValueError("out must be contiguous and of q's shape")
+    _heads(kv, "out", out, shape)
+    if not out.is_contiguous():
+      raise ValueError("out must be contiguous")
   lib = _native.lib()
-  nbytes = ctypes.c_uint64()
-  _native.check(lib.ts_paged_attention_workspace(kv._index, kv._ref, ctypes.byref(a),
-                                                 ctypes.byref(nbytes)), "attention: ")
-  with _on(stream):
+  # the workspace's size follows from the shapes alone
+  key = (batch, new, q_heads, prefix_blocks > 0)
+  nbytes = kv._workspace.get(key)
+  if nbytes is None:
+    n = ctypes.c_uint64()
+    _native.check(lib.ts_paged_attention_workspace(kv._index, kv._ref, ctypes.byref(a),
+                                                   ctypes.byref(n)), "attention: ")
+    nbytes = n.value
+    if len(kv._workspace) >= 1024:
+      kv._workspace.clear()
+    kv._workspace[key] = nbytes
+  lse = None
+  # what a call allocates belongs to its stream
+  with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
     if out is None:
-      out = torch.empty(q.shape, dtype=kv.dtype, device=kv.device)
-    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=kv.device) if return_lse else None
-    work = torch.empty(nbytes.value, dtype=torch.uint8, device=kv.device)
+      out = _new_like(q)
+    if return_lse:
+      lse = q.new_empty(shape[:-1], dtype=torch.float32)
+      a.lse = lse.data_ptr()
+    work = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
   a.out = out.data_ptr()
-  if return_lse:
-    a.lse = lse.data_ptr()
-  _native.check(lib.ts_paged_attention(kv._index, kv._ref, ctypes.byref(a), work.data_ptr(),
-                                       nbytes.value, flag, _stream(stream, kv.device)),
-                "attention: ")
+  rc = lib.ts_paged_attention(kv._index, kv._ref, ctypes.byref(a), work.data_ptr(), nbytes,
+                              _flag(kv, err_flag),
+                              torch._C._cuda_getCurrentRawStream(kv._index)
+                              if stream is None else stream.cuda_stream)
+  if rc:
+    _native.check(rc, "attention: ")
   return (out, lse) if return_lse else out
 
 
