@@ -51,7 +51,9 @@ __device__ __forceinline__ bool token_place(const AppendParams& p, int64_t t, bo
   const int64_t slot = reinterpret_cast<const int64_t*>(p.a.slots)[t];
   *pos = rot ? reinterpret_cast<const int64_t*>(p.a.positions)[t] : 0;
   if (slot < 0) return false;
-  const int64_t pg = slot / p.kv.block_tokens;
+  // pages and block_tokens fit 31 bits, a slot usually 32: a short division
+  const int64_t pg = slot <= UINT32_MAX ? int64_t(uint32_t(slot) / uint32_t(p.kv.block_tokens))
+                                        : slot / p.kv.block_tokens;
   if (pg >= p.kv.pages || (rot && (*pos < 0 || *pos >= p.a.max_position))) {
     if (p.err != nullptr) *reinterpret_cast<volatile int*>(p.err) = 1;
     return false;
@@ -189,139 +191,221 @@ __device__ __forceinline__ void weights8(uint64_t w, int f32, int e, float* f) {
   }
 }
 
-enum Rotation { kNone = 0, kHalves = 1, kPairs = 2 };
-constexpr int kHeadsAhead = 3;  // head vectors a lane holds before it works on the first
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
 
-// A CTA per token; kLanes = head_dim / 8 lanes hold a head, 16 bytes each, so
-// a warp takes 32 / kLanes heads at a time and a lane meets the same elements
-// of every head: its cosines and sines are loaded once per token.  Rotated
-// halves are 8-element pieces of another lane of the same head (one shuffle
-// per element); interleaved pairs lie within a lane.  All of a lane's head
-// vectors are loaded before the first is used, and before the slot and
-// position they depend on are known.
+enum Rotation { kNone = 0, kHalves = 1, kPairs = 2 };
+constexpr int kAhead = 8;   // units a warp has in flight
+constexpr int kUnitBytes = 512;
+
+// kLanes = head_dim / 8 lanes hold a head, 16 bytes each, so a warp takes
+// 32 / kLanes heads at a time (a unit) and a lane meets the same elements of
+// every head of a token.  Norm and rotation are one product sum per element,
+//   y_e = (x_e A_e + x_mate(e) B_e) / sqrt(mean(x^2) + eps),
+//   A_e = w_e cos, B_e = -+ w_mate(e) sin,
+// whose A and B stay in registers over a token's query heads, and over its
+// key heads.  Units travel through shared memory (cp.async, a ring per warp):
+// what is in flight costs no registers, and the mates of rotated halves,
+// another lane's 8 elements, are read from there; those of interleaved pairs
+// are in the lane.
+//
+// `split` warps share a token, chosen by the host: decode steps spread a
+// token's heads over eight warps to shorten the one chain of dependent loads;
+// prompts give a warp all heads of a token, so that the chain and the
+// coefficients are paid once per token and the loads of later heads run under
+// the work on earlier ones.
 template <typename T, int kLanes, int kRot, bool kNorm>
-__global__ void __launch_bounds__(256) append_vec_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(256, 3)
+    append_vec_kernel(const __grid_constant__ AppendParams p, const int split) {
   constexpr int kHeads = 32 / kLanes;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int j = lane % kLanes;
-  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 31;
+  const int64_t wid = int64_t(blockIdx.x) * (blockDim.x >> 5) +
+                      __shfl_sync(~0u, int(threadIdx.x >> 5), 0);
+  const int64_t t = wid / split;
+  if (t >= p.a.tokens) return;
+  const int j = lane % kLanes, sub = lane / kLanes;
   const int hq = p.a.q != 0 ? int(p.a.q_heads) : 0;
   const int hk = int(p.kv.heads);
-  const int heads = hq + 2 * hk;
-  const T* q = reinterpret_cast<const T*>(p.a.q) + t * p.a.q_token_stride + j * 8;
-  const T* k = reinterpret_cast<const T*>(p.a.k) + t * p.a.k_token_stride + j * 8;
-  const T* v = reinterpret_cast<const T*>(p.a.v) + t * p.a.v_token_stride + j * 8;
-  T* qo = reinterpret_cast<T*>(p.a.q_out) + t * p.a.q_out_token_stride + j * 8;
-  const int step = warps * kHeads;
+  const int uq = (hq + kHeads - 1) / kHeads, uk = (hk + kHeads - 1) / kHeads;
+  const int units = uq + 2 * uk;
+  int u = int(wid - t * split);
 
-  int4 x[kHeadsAhead];
-  auto load = [&](int h0) {
+  __shared__ __align__(16) uint8_t rings[8][kAhead][kUnitBytes];
+  uint8_t(*ring)[kUnitBytes] = rings[threadIdx.x >> 5];
+  const uint32_t here = uint32_t(__cvta_generic_to_shared(ring)) + lane * 16;
+  // Walks this lane's pieces of the warp's units: running addresses, set anew
+  // where the queries end and where the keys end.
+  struct Walk {
+    T* at;
+    int64_t step;
+    int unit, next, head, heads;  // `next`: first unit of the next kind
+  };
+  const int stride = split * kHeads;  // heads between two units of the warp
+  auto enter = [&](Walk& w, const T* qb, int64_t qs, const T* kb, int64_t ks, const T* vb,
+                   int64_t vs) {
+    const int kind = w.unit < uq ? 0 : (w.unit < uq + uk ? 1 : 2);
+    w.head = (w.unit - (kind > 0 ? uq : 0) - (kind > 1 ? uk : 0)) * kHeads + sub;
+    w.heads = kind == 0 ? hq : hk;
+    w.next = uq + kind * uk;
+    const int64_t one = kind == 0 ? qs : (kind == 1 ? ks : vs);
+    w.at = const_cast<T*>((kind == 0 ? qb : (kind == 1 ? kb : vb)) + w.head * one + j * 8);
+    w.step = stride * one;
+  };
+  Walk in{};
+  in.unit = u;
+  const T* qb = reinterpret_cast<const T*>(p.a.q) + t * p.a.q_token_stride;
+  const T* kb = reinterpret_cast<const T*>(p.a.k) + t * p.a.k_token_stride;
+  const T* vb = reinterpret_cast<const T*>(p.a.v) + t * p.a.v_token_stride;
+  enter(in, qb, p.a.q_head_stride, kb, p.a.k_head_stride, vb, p.a.v_head_stride);
+  // queues the next unit; units past the last one are empty
+  auto load = [&](int slot) {
+    if (in.unit < units) {
+      if (in.head < in.heads)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(here + slot * kUnitBytes),
+                     "l"(in.at)
+                     : "memory");
+      in.unit += split;
+      in.head += stride;
+      in.at += in.step;
+      if (in.unit >= in.next)
+        enter(in, qb, p.a.q_head_stride, kb, p.a.k_head_stride, vb, p.a.v_head_stride);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 #pragma unroll
-    for (int i = 0; i < kHeadsAhead; ++i) {
-      const int h = h0 + i * step;
-      if (h < heads) {
-        const T* src = h < hq ? q + h * p.a.q_head_stride
-                              : (h < hq + hk ? k + (h - hq) * p.a.k_head_stride
-                                             : v + (h - hq - hk) * p.a.v_head_stride);
-        x[i] = __ldcs(reinterpret_cast<const int4*>(src));
+  for (int i = 0; i < kAhead - 1; ++i) load(i);
+  int64_t page = 0, off = 0, pos = 0;
+  const bool live = token_place(p, t, kRot != kNone, &page, &off, &pos);
+  T* qo = reinterpret_cast<T*>(p.a.q_out) + t * p.a.q_out_token_stride;
+  if (!live) {
+    if (p.a.zero_padding)
+      for (; u < uq; u += split)
+        if (u * kHeads + sub < hq)
+          *reinterpret_cast<int4*>(qo + (u * kHeads + sub) * p.a.q_out_head_stride + j * 8) =
+              make_int4(0, 0, 0, 0);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    return;
+  }
+  const T* kd =
+      reinterpret_cast<T*>(p.kv.k_ptr) + page * p.kv.k_page_stride + off * p.kv.k_token_stride;
+  const T* vd =
+      reinterpret_cast<T*>(p.kv.v_ptr) + page * p.kv.v_page_stride + off * p.kv.v_token_stride;
+  Walk out{};
+  out.unit = u;
+  enter(out, qo, p.a.q_out_head_stride, kd, p.kv.k_head_stride, vd, p.kv.v_head_stride);
+
+  // where this lane's elements find their angles and mates
+  int mate = j;          // the lane of the head with the mates (halves)
+  int angle = 0;
+  bool turns = false, second = false;
+  const int half = kRot != kNone ? int(p.a.rotary) / 2 : 0;
+  if (kRot == kPairs) {
+    turns = j * 8 < 2 * half;
+    angle = j * 4;
+  } else if (kRot == kHalves) {
+    turns = j * 4 < half;
+    second = j * 8 >= half;
+    angle = (second ? j * 8 - half : j * 8);
+    if (turns) mate = second ? j - half / 8 : j + half / 8;
+  }
+  const float* row = reinterpret_cast<const float*>(p.a.cos_sin) + pos * p.a.cos_sin_stride + angle;
+  float2 ca[4], cb[4];
+  auto coefficients = [&](uint64_t w) {
+    float wm[8];
+    float* ca1 = reinterpret_cast<float*>(ca);
+    float* cb1 = reinterpret_cast<float*>(cb);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ca1[e] = wm[e] = 1.f;
+    if (kNorm && w != 0) {
+      weights8<T>(w, p.a.weight_dtype == TS_DTYPE_F32, j * 8, ca1);
+      if (kRot == kHalves) weights8<T>(w, p.a.weight_dtype == TS_DTYPE_F32, mate * 8, wm);
+      if (kRot == kPairs)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wm[e] = ca1[e ^ 1];
+    }
+    if (kRot != kNone && turns) {
+#pragma unroll
+      for (int i = 0; i < (kRot == kPairs ? 4 : 8); i += 4) {
+        const float4 c = __ldg(reinterpret_cast<const float4*>(row + i));
+        const float4 s = __ldg(reinterpret_cast<const float4*>(row + half + i));
+        const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          if (kRot == kPairs) {
+            ca1[2 * a] *= cv[a];
+            ca1[2 * a + 1] *= cv[a];
+            cb1[2 * a] = -wm[2 * a] * sv[a];
+            cb1[2 * a + 1] = wm[2 * a + 1] * sv[a];
+          } else {
+            ca1[i + a] *= cv[a];
+            cb1[i + a] = second ? wm[i + a] * sv[a] : -wm[i + a] * sv[a];
+          }
+        }
       }
     }
   };
-  int h0 = warp * kHeads + lane / kLanes;
-  load(h0);
-  int64_t page = 0, off = 0, pos = 0;
-  const bool live = token_place(p, t, kRot != kNone, &page, &off, &pos);
-  if (!live) {
-    if (p.a.zero_padding)
-      for (int h = h0; h < hq; h += step)
-        *reinterpret_cast<int4*>(qo + h * p.a.q_out_head_stride) = make_int4(0, 0, 0, 0);
-    return;
-  }
-  T* kd = reinterpret_cast<T*>(p.kv.k_ptr) + page * p.kv.k_page_stride + off * p.kv.k_token_stride +
-          j * 8;
-  T* vd = reinterpret_cast<T*>(p.kv.v_ptr) + page * p.kv.v_page_stride + off * p.kv.v_token_stride +
-          j * 8;
-  // this lane's cosines and sines, and the lane of its pairs' other halves
-  constexpr int kAngles = kRot == kPairs ? 4 : 8;
-  float c[kAngles], s[kAngles];
-  int mate = lane;
-  bool turns = false, second = false;
-  if (kRot != kNone) {
-    const int half = int(p.a.rotary) / 2;
-    const float* row = reinterpret_cast<const float*>(p.a.cos_sin) + pos * p.a.cos_sin_stride;
-    int at;
-    if (kRot == kPairs) {
-      turns = j * 8 < int(p.a.rotary);
-      at = j * 4;
-    } else {
-      const int half_lanes = half / 8;
-      turns = j < 2 * half_lanes;
-      second = j >= half_lanes;
-      at = (second ? j - half_lanes : j) * 8;
-      if (turns) mate = second ? lane - half_lanes : lane + half_lanes;
-    }
-    if (turns) {
-#pragma unroll
-      for (int i = 0; i < kAngles / 4; ++i) {
-        *reinterpret_cast<float4*>(c + 4 * i) =
-            __ldg(reinterpret_cast<const float4*>(row + at) + i);
-        *reinterpret_cast<float4*>(s + 4 * i) =
-            __ldg(reinterpret_cast<const float4*>(row + half + at) + i);
+  int upto = 0;  // units before it have the coefficients that are held
+  uint64_t w = 0;
+  for (int slot = 0; out.unit < units; slot = slot + 1 == kAhead ? 0 : slot + 1) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+    __syncwarp();  // the unit is here, and every lane is done with the one before
+    load(slot == 0 ? kAhead - 1 : slot - 1);
+    int4 y = *reinterpret_cast<const int4*>(ring[slot] + lane * 16);
+    if ((kNorm || kRot != kNone) && out.unit < uq + uk) {
+      if (out.unit >= upto) {
+        w = out.unit < uq ? p.a.q_weight : p.a.k_weight;
+        upto = out.next;
+        coefficients(w);
       }
-    }
-  }
-  // every lane of a warp makes the same rounds: the shuffles need them all
-  for (int base = warp * kHeads; base < heads; base += kHeadsAhead * step, h0 += kHeadsAhead * step) {
-    if (base != warp * kHeads) load(h0);
+      float2 f[4], o[4];
+      unpack8(y, reinterpret_cast<float*>(f), T{});
+      float2 inv = make_float2(1.f, 1.f);
+      if (kNorm && w != 0) {
+        float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kHeadsAhead; ++i) {
-      if (base + i * step >= heads) break;
-      const int h = h0 + i * step;
-      const bool is_q = h < hq, is_k = !is_q && h < hq + hk;
-      if ((kNorm || kRot != kNone) && base + i * step < hq + hk) {
-        float f[8];
-        unpack8(x[i], f, T{});
-        if (kNorm) {
-          const uint64_t w = is_q ? p.a.q_weight : p.a.k_weight;
-          float ss = 0.f;
+        for (int e = 0; e < 4; ++e) ss = fma2(f[e], f[e], ss);
+        float sum = ss.x + ss.y;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
-#pragma unroll
-          for (int m = kLanes / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(~0u, ss, m);
-          if (w != 0 && (is_q || is_k)) {
-            const float inv = rsqrtf(ss * (1.f / (8 * kLanes)) + p.a.eps);
-            float g[8];
-            weights8<T>(w, p.a.weight_dtype == TS_DTYPE_F32, j * 8, g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = f[e] * inv * g[e];
-          }
-        }
-        if (kRot == kHalves) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float o = __shfl_sync(~0u, f[e], mate);
-            if (turns) f[e] = second ? f[e] * c[e] + o * s[e] : f[e] * c[e] - o * s[e];
-          }
-        } else if (kRot == kPairs) {
-          if (turns) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = f[2 * e], b = f[2 * e + 1];
-              f[2 * e] = a * c[e % kAngles] - b * s[e % kAngles];
-              f[2 * e + 1] = b * c[e % kAngles] + a * s[e % kAngles];
-            }
-          }
-        }
-        if (is_q || is_k) x[i] = pack8(f, T{});
+        for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(~0u, sum, m);
+        inv.x = inv.y = rsqrtf(sum * (1.f / (8 * kLanes)) + p.a.eps);
       }
-      if (h < heads) {
-        T* dst = is_q ? qo + h * p.a.q_out_head_stride
-                      : (is_k ? kd + (h - hq) * p.kv.k_head_stride
-                              : vd + (h - hq - hk) * p.kv.v_head_stride);
-        *reinterpret_cast<int4*>(dst) = x[i];
+      if (kRot == kHalves) {
+        unpack8(*reinterpret_cast<const int4*>(ring[slot] + (sub * kLanes + mate) * 16),
+                reinterpret_cast<float*>(o), T{});
+      } else if (kRot == kPairs) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = make_float2(f[e].y, f[e].x);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = mul2(f[e], ca[e]);
+        if (kRot != kNone && turns) f[e] = fma2(o[e], cb[e], f[e]);
+        if (kNorm) f[e] = mul2(f[e], inv);
+      }
+      y = pack8(reinterpret_cast<const float*>(f), T{});
     }
+    if (out.head < out.heads) *reinterpret_cast<int4*>(out.at) = y;
+    out.unit += split;
+    out.head += stride;
+    out.at += out.step;
+    if (out.unit >= out.next && out.unit < units)
+      enter(out, qo, p.a.q_out_head_stride, kd, p.kv.k_head_stride, vd, p.kv.v_head_stride);
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // The vector kernel's rule: heads of 64, 128 or 256 elements, every address and
@@ -344,29 +428,35 @@ bool vector_ok(const AppendParams& p) {
 }
 
 template <typename T, int kLanes>
-void launch_vec(const AppendParams& p, cudaStream_t s) {
+void launch_vec(const AppendParams& p, int device, cudaStream_t s) {
   constexpr int kHeads = 32 / kLanes;
-  const int heads = int(p.a.q != 0 ? p.a.q_heads : 0) + 2 * int(p.kv.heads);
-  const int warps = std::min(8, (heads + kHeads - 1) / kHeads);
+  // As many warps per token as fill the GPU (24 warps an SM), at most one per
+  // group of heads and eight.
+  const int64_t fill = int64_t(sm_count(device)) * 24 / p.a.tokens;
+  const int hq = int(p.a.q != 0 ? p.a.q_heads : 0), hk = int(p.kv.heads);
+  const int groups = (hq + kHeads - 1) / kHeads + 2 * ((hk + kHeads - 1) / kHeads);
+  const int split = int(std::max<int64_t>(1, std::min<int64_t>({fill, groups, 8})));
   const bool norm = p.a.q_weight || p.a.k_weight;
-  const dim3 grid(static_cast<unsigned>(p.a.tokens)), block(warps * 32);
+  const int64_t warps = p.a.tokens * split;
+  const int block = 32 * int(std::min<int64_t>(8, warps));
+  const unsigned grid = unsigned((warps * 32 + block - 1) / block);
   if (!p.a.cos_sin)
-    norm ? append_vec_kernel<T, kLanes, kNone, true><<<grid, block, 0, s>>>(p)
-         : append_vec_kernel<T, kLanes, kNone, false><<<grid, block, 0, s>>>(p);
+    norm ? append_vec_kernel<T, kLanes, kNone, true><<<grid, block, 0, s>>>(p, split)
+         : append_vec_kernel<T, kLanes, kNone, false><<<grid, block, 0, s>>>(p, split);
   else if (p.a.interleaved)
-    norm ? append_vec_kernel<T, kLanes, kPairs, true><<<grid, block, 0, s>>>(p)
-         : append_vec_kernel<T, kLanes, kPairs, false><<<grid, block, 0, s>>>(p);
+    norm ? append_vec_kernel<T, kLanes, kPairs, true><<<grid, block, 0, s>>>(p, split)
+         : append_vec_kernel<T, kLanes, kPairs, false><<<grid, block, 0, s>>>(p, split);
   else
-    norm ? append_vec_kernel<T, kLanes, kHalves, true><<<grid, block, 0, s>>>(p)
-         : append_vec_kernel<T, kLanes, kHalves, false><<<grid, block, 0, s>>>(p);
+    norm ? append_vec_kernel<T, kLanes, kHalves, true><<<grid, block, 0, s>>>(p, split)
+         : append_vec_kernel<T, kLanes, kHalves, false><<<grid, block, 0, s>>>(p, split);
 }
 
 template <typename T>
 int launch_append(const AppendParams& p, int device, cudaStream_t s) {
   if (vector_ok(p)) {
-    p.kv.head_dim == 64    ? launch_vec<T, 8>(p, s)
-    : p.kv.head_dim == 128 ? launch_vec<T, 16>(p, s)
-                           : launch_vec<T, 32>(p, s);
+    p.kv.head_dim == 64    ? launch_vec<T, 8>(p, device, s)
+    : p.kv.head_dim == 128 ? launch_vec<T, 16>(p, device, s)
+                           : launch_vec<T, 32>(p, device, s);
     TS_CUDA_RET(cudaGetLastError(), "kv append launch");
     return TS_OK;
   }
