@@ -10,7 +10,7 @@
 // A unit is (256 query rows, KV head).  A CTA takes an equal, contiguous share
 // of all 128-key tiles of all units (shares are cut on the device, from the
 // prefix length there); a share that cuts a unit leaves partials (m, l, acc),
-// joined per row by join_kernel.  Roles of the ten warps:
+// joined per row by join_kernel.  Roles of the warps:
 //
 //   warps 0-3, 4-7  one query row per thread, 128 rows each (halves A and B):
 //                   S from TMEM, running maximum and sum, P = 2^(S - m) back to
@@ -48,7 +48,7 @@
 namespace tsb {
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
 constexpr uint32_t kWaitRounds = 1u << 24;  // try_waits (each suspends for a while): seconds
 
 template <int D>
@@ -146,12 +146,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t* r, uint32_t addr) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
-      "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      TS_W8(r, 0), TS_W8(r, 8), TS_W8(r, 16), TS_W8(r, 24)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : TS_R8(r, 0), TS_R8(r, 8)
+      : "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
@@ -186,6 +186,25 @@ struct InstrDesc {
                                     uint32_t(128 >> 4) << 24;
 };
 
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float ax, float ay, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(ax), "f"(ay), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -258,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int x = 0; x < 2; ++x) {
       bar_init(q_full + 8 * x, 128);
       bar_init(s_full + 8 * x, 1);
-      bar_init(p_ready + 8 * x, 128);
+      bar_init(p_ready + 8 * x, 4);
       bar_init(o_full + 8 * x, 1);
     }
     *gone = 0;
@@ -277,7 +296,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int bt = int(p.kv.block_tokens);
   Segment seg;
 
-  if (warp == 8) {
+  // The softmax warps hold 128 scores each; the loading and issuing warpgroup
+  // gives up registers for them: 2 x 128 x 208 + 128 x 88 = 384 x 168.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
     // -- loads ----------------------------------------------------------------
     const int pieces = kPrefixTile / p.piece;
     uint32_t n = 0;  // tiles loaded, K and V counted apart
@@ -314,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (warp == 9) {
+    } else if (warp == 9) {
     // -- matrix products --------------------------------------------------------
     constexpr uint32_t kIdescS = InstrDesc<T, kPrefixTile, false>::value;
     constexpr uint32_t kIdescO = InstrDesc<T, D, true>::value;
@@ -390,7 +413,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         n += more ? 2 : 1;
       }
     }
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // -- softmax ----------------------------------------------------------------
     const int x = warp >> 2;               // half
     const int r = threadIdx.x & 127;       // row of the half
@@ -446,13 +471,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++s_n;
         if (!ok) break;
         fence_after();
-        float s[kPrefixTile];
+        uint32_t s[kPrefixTile];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_ld32(reinterpret_cast<uint32_t*>(s) + 32 * c, ts + 32 * c);
+        for (int c = 0; c < 4; ++c) tmem_ld32(s + 32 * c, ts + 32 * c);
         tmem_wait_ld();
         const int t0 = (seg.tile + j) * kPrefixTile;
         if (hole || t0 + kPrefixTile > len) {
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int t = t0 + 32 * c + lane;
             bool in = t < len;
@@ -462,13 +487,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const uint32_t mask = __ballot_sync(~0u, in);
 #pragma unroll
-            for (int k = 0; k < kPrefixTile; ++k)
-              if (k / 32 == c && !((mask >> (k % 32)) & 1)) s[k] = -INFINITY;
+            for (int k = 0; k < 32; ++k)
+              if (!((mask >> k) & 1)) s[32 * c + k] = 0xff800000u;  // -inf
           }
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 4; k < kPrefixTile; ++k) mx[k % 4] = fmaxf(mx[k % 4], s[k]);
+        for (int k = 0; k < kPrefixTile; k += 2)
+          mx[k / 2 % 4] = fmaxf(fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
+                                mx[k / 2 % 4]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         const bool grew = top > m + 8.f;
         if (__any_sync(~0u, grew)) {
@@ -477,36 +504,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= f;
           if (j > 0) {
             // the products up to the last tile are done: s_full was committed after them
-            uint32_t o[32];
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              tmem_ld32(o, to + 32 * c);
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o, to + 16 * c);
               tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st32(to + 32 * c, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(to + 16 * c, o);
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float base = m == -INFINITY ? 0.f : -m;
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+        const float2 base2 = make_float2(base, base);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const float a = ex2(fmaf(s[32 * c + 2 * k], p.scale_log2, -base));
-            const float b = ex2(fmaf(s[32 * c + 2 * k + 1], p.scale_log2, -base));
-            sum[k % 2 * 2] += a;
-            sum[k % 2 * 2 + 1] += b;
-            pk[k] = pack2(a, b, T{});
+            float2 e = fma2(__uint_as_float(s[32 * c + 2 * k]),
+                            __uint_as_float(s[32 * c + 2 * k + 1]), scale2, base2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[k % 2] = add2(sum[k % 2], e);
+            pk[k] = pack2(e.x, e.y, T{});
           }
           tmem_st16(ts + 16 * c, pk);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
         tmem_wait_st();
         fence_before();
-        bar_arrive(p_ready + 8 * x);
+        __syncwarp();
+        if (lane == 0) bar_arrive(p_ready + 8 * x);
       }
       if (!ok) break;
       ok = bar_wait(o_full + 8 * x, o_n & 1, gone);
