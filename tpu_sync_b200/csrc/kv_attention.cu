@@ -61,6 +61,7 @@ struct WalkParams {
   float* pre_ml;
   int* err;
   int ctas;
+  int block_shift;    // log2(block_tokens), or -1
   // the prefix part when prefix_attention.cu does it: its partition and partials
   int tensor_ctas;    // 0: it does not
   int tensor_row_tiles;
@@ -82,109 +83,133 @@ __device__ __forceinline__ int tokens_of(const WalkParams& p, int64_t b, bool* b
   return int(n < 0 ? 0 : (n > cap ? cap : n));
 }
 
-__device__ __forceinline__ int64_t tiles_of(const WalkParams& p, int64_t b, bool* bad) {
-  const int64_t per = b < p.a.batch ? int64_t(p.row_tiles_own) * p.kv.heads
-                                    : int64_t(p.row_tiles_pre) * p.kv.heads;
-  return int64_t((tokens_of(p, b, bad) + kTile - 1) / kTile) * per;
-}
+// Work is counted in units of a tile's time: an item of nt tiles costs nt + 2,
+// for its queries and the join of its four warps (2.4 us beside 0.95 us a tile
+// measured for a CTA alone, 1.5 us a tile when all of them share HBM).
+// Without that a CTA with ten short items ran 18 us past the median of 85 us
+// (64 sequences of 17..4096 tokens).  Totals fit 31 bits (checked on the host).
+constexpr int kItemCost = 2;
 
-// Sum over sequences [0, end) of their tiles; every lane of the warp gets it.
-__device__ __forceinline__ int64_t tiles_before(const WalkParams& p, int64_t end) {
-  int64_t sum = 0;
-  bool bad, any = false;
-  for (int64_t b = threadIdx.x & 31; b < end; b += 32) {
-    sum += tiles_of(p, b, &bad);
-    any = any || bad;
-  }
-  if (any) raise(p.err);
+__device__ __forceinline__ int tiles_in(int len) { return (len + kTile - 1) / kTile; }
+__device__ __forceinline__ int cost_of(const WalkParams& p, bool own, int len) {
+  const int nt = tiles_in(len);
+  return nt > 0 ? (nt + kItemCost) * (own ? p.row_tiles_own : p.row_tiles_pre) * int(p.kv.heads)
+                : 0;
+}
+__device__ __forceinline__ int warp_sum(int x) {
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(~0u, sum, m);
-  return sum;
-}
-
-// CTA w of n takes tiles [total * w / n, total * (w + 1) / n), and n is cut to
-// the tiles there are, so that no CTA of them is without a tile.
-__device__ __forceinline__ int64_t sharers(int64_t total, int ctas) {
-  return total < ctas ? total : ctas;
+  for (int m = 16; m > 0; m >>= 1) x += __shfl_xor_sync(~0u, x, m);
+  return x;
 }
 
 // Position in the CTA's share: the item (sequence, row tile, KV head) and the
 // tiles [tile, end) of it that are this CTA's.
 struct Cursor {
-  int64_t left;    // tiles of the share from `tile` on
-  int64_t b;
-  int sub;         // row tile * heads + head
+  int left;        // units of the share after this item's
+  int b;           // sequence; batch: the shared prefix
+  int rt, head;
   int tile, end;
   int len;         // tokens of the sequence
   int nt;          // tiles of the item
 
-  __device__ __forceinline__ void open(const WalkParams& p) {
-    // enter sequence b (skipping empty ones); sub and tile are set
-    bool bad;
-    for (; b < p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0); ++b) {
-      len = tokens_of(p, b, &bad);
-      nt = (len + kTile - 1) / kTile;
-      if (nt > 0) return clip();
-    }
-    left = 0;
+  __device__ __forceinline__ bool done() const { return tile >= end; }
+  // the share's tiles of this item, from unit u of it on (its cost comes first)
+  __device__ __forceinline__ void take(int u) {
+    const int to = min(nt + kItemCost, u + left);
+    left -= to - u;
+    tile = max(u, kItemCost) - kItemCost;
+    end = to - kItemCost;
   }
-  __device__ __forceinline__ void clip() {
-    const int64_t rest = nt - tile;
-    end = tile + int(rest < left ? rest : left);
+  __device__ __forceinline__ int seqs(const WalkParams& p) const {
+    return int(p.a.batch) + (p.row_tiles_pre > 0 ? 1 : 0);
   }
-  // the first share tile: global tile index lo
-  __device__ __forceinline__ void start(const WalkParams& p, int64_t lo, int64_t count) {
-    left = count;
-    b = 0;
-    sub = tile = end = len = nt = 0;
-    if (count <= 0) return;
-    const int lane = threadIdx.x & 31;
-    int64_t base = 0;
-    const int64_t seqs = p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0);
-    for (int64_t b0 = 0; b0 < seqs; b0 += 32) {
-      bool bad;
-      const int64_t mine = b0 + lane < seqs ? tiles_of(p, b0 + lane, &bad) : 0;
-      int64_t run = mine;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int64_t up = __shfl_up_sync(~0u, run, m);
-        if (lane >= m) run += up;
-      }
-      const unsigned past = __ballot_sync(~0u, base + run > lo);
-      if (past) {
-        const int at = __ffs(past) - 1;
-        b = b0 + at;
-        const int64_t in_seq = lo - base - __shfl_sync(~0u, run - mine, at);
-        bool ignore;
-        len = tokens_of(p, b, &ignore);
-        nt = (len + kTile - 1) / kTile;
-        sub = int(in_seq / nt);
-        tile = int(in_seq - int64_t(sub) * nt);
-        clip();
-        return;
-      }
-      base += __shfl_sync(~0u, run, 31);
-    }
-    left = 0;
-  }
-  __device__ __forceinline__ bool done() const { return left <= 0; }
-  __device__ __forceinline__ int subs(const WalkParams& p) const {
-    return (b < p.a.batch ? p.row_tiles_own : p.row_tiles_pre) * int(p.kv.heads);
-  }
-  // past this item's tiles of the share
+  // after this item's tiles
   __device__ __forceinline__ void next_item(const WalkParams& p) {
-    left -= end - tile;
+    tile = end = 0;
     if (left <= 0) return;
-    tile = 0;
-    if (++sub == subs(p)) {
-      sub = 0;
-      ++b;
-      open(p);
-    } else {
-      clip();
+    if (++head == int(p.kv.heads)) {
+      head = 0;
+      if (++rt == (b < p.a.batch ? p.row_tiles_own : p.row_tiles_pre)) {
+        rt = 0;
+        bool bad;
+        do {
+          if (++b >= seqs(p)) return;
+          len = tokens_of(p, b, &bad);
+        } while (len == 0);
+        nt = tiles_in(len);
+      }
     }
+    take(0);
   }
 };
+
+constexpr int kLensHeld = 4;  // lengths a lane keeps: batches up to 128 are read once
+
+// Finds the CTA's share and its first item; done() when it has none.
+__device__ __forceinline__ Cursor start_cursor(const WalkParams& p) {
+  Cursor c{};
+  const int lane = threadIdx.x & 31;
+  const int seqs = c.seqs(p);
+  int held[kLensHeld];
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < kLensHeld; ++k) {
+    bool now = false;
+    const int i = 32 * k + lane;
+    held[k] = i < seqs ? tokens_of(p, i, &now) : 0;
+    bad = bad || now;
+  }
+  int sum = 0;
+#pragma unroll
+  for (int k = 0; k < kLensHeld; ++k) sum += cost_of(p, 32 * k + lane < p.a.batch, held[k]);
+  for (int i = 32 * kLensHeld + lane; i < seqs; i += 32) {
+    bool now;
+    sum += cost_of(p, i < p.a.batch, tokens_of(p, i, &now));
+    bad = bad || now;
+  }
+  if (bad) raise(p.err);
+  const Cut cut(warp_sum(sum), p.ctas);
+  const int w = blockIdx.x;
+  if (w >= cut.ctas) return c;
+  const int lo = cut.start(w);
+  c.left = cut.start(w + 1) - lo;
+  int base = 0;
+  for (int k = 0; 32 * k < seqs; ++k) {
+    int len = 0;
+    bool ignore;
+    const int i = 32 * k + lane;
+    if (k < kLensHeld) {
+#pragma unroll
+      for (int h = 0; h < kLensHeld; ++h)
+        if (h == k) len = held[h];
+    } else if (i < seqs) {
+      len = tokens_of(p, i, &ignore);
+    }
+    const int cost = cost_of(p, i < p.a.batch, len);
+    int run = cost;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int up = __shfl_up_sync(~0u, run, m);
+      if (lane >= m) run += up;
+    }
+    const unsigned past = __ballot_sync(~0u, base + run > lo);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      c.b = 32 * k + at;
+      c.len = __shfl_sync(~0u, len, at);
+      c.nt = tiles_in(c.len);
+      const int in_seq = lo - base - __shfl_sync(~0u, run - cost, at);
+      const int item = c.nt + kItemCost;
+      const int sub = int(uint32_t(in_seq) / uint32_t(item));
+      c.rt = int(uint32_t(sub) / uint32_t(p.kv.heads));
+      c.head = sub - c.rt * int(p.kv.heads);
+      c.take(in_seq - sub * item);
+      return c;
+    }
+    base += __shfl_sync(~0u, run, 31);
+  }
+  return c;
+}
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return uint32_t(__cvta_generic_to_shared(p));
@@ -261,10 +286,19 @@ __host__ __device__ constexpr int walk_smem() {
   return kWarps * kStages * stage_bytes<D>() + join_floats<D>() * 4 + kWarps * kStages * 4;
 }
 
-// Row r of an item: which query (token index over the batch, head).
-__device__ __forceinline__ int64_t row_token(const WalkParams& p, const Cursor& c, int row) {
-  const int64_t base = c.b < p.a.batch ? c.b * p.a.new_tokens : 0;
-  return base + row / p.group;
+// Row r of an item: sequence b's new token j, query head g of the KV head.
+struct Row {
+  int b, j, g;
+};
+__device__ __forceinline__ Row row_of(const WalkParams& p, const Cursor& c, int row) {
+  Row r;
+  const int n = int(p.a.new_tokens);
+  const int tok = int(uint32_t(row) / uint32_t(p.group));
+  r.g = row - tok * p.group;
+  const int b = n == 1 ? tok : int(uint32_t(tok) / uint32_t(n));
+  r.j = tok - b * n;
+  r.b = c.b < p.a.batch ? c.b : b;  // an own item's rows are of one sequence: b is 0
+  return r;
 }
 
 template <typename T, int D, int MT>
@@ -283,18 +317,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
   // it, this one may itself run early: it reads nothing that kernel writes, and
   // waits for it before it ends, so that join_kernel's wait covers both.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t seqs = p.a.batch + (p.row_tiles_pre > 0 ? 1 : 0);
-  const int64_t total = tiles_before(p, seqs);
-  const int64_t ctas = sharers(total, p.ctas);
-  if (blockIdx.x >= ctas) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
-  const int64_t lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
-  Cursor ld, cu;
-  cu.start(p, lo, hi - lo);
-  ld = cu;
+  Cursor cu = start_cursor(p);
+  Cursor ld = cu;
   int ld_tile = ld.tile;
+  // table entries [window, window + 32) of the sequence being loaded, one a lane
+  int window = -1, entry = 0, window_seq = -1;
+  const int bt = int(p.kv.block_tokens);
 
   // Queues the warp's 16 tokens of tile ld_tile into ring stage `st`.
   auto load = [&](int st) {
@@ -302,45 +330,65 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
       cp_commit();
       return;
     }
-    const int head = ld.sub % int(p.kv.heads);
     const int t0 = ld_tile * kTile + warp * kWarpTokens;
-    // lanes 0..15 place one token each
-    const int t = t0 + (lane & 15);
-    const int blk = t / int(p.kv.block_tokens);
-    const int off = t - blk * int(p.kv.block_tokens);
-    bool ok = t < ld.len;
-    int page = 0;
-    if (ok) {
-      const int32_t* table = ld.b < p.a.batch
-          ? reinterpret_cast<const int32_t*>(p.a.block_table) + ld.b * p.a.block_table_stride
-          : reinterpret_cast<const int32_t*>(p.a.prefix_table);
-      page = table[blk];
-      if (page < 0 || page >= p.kv.pages) {
-        raise(p.err);
-        ok = false;
-        page = 0;
-      }
-    }
-    const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
-    if (lane == 0) masks[st] = mask;
-    const uint64_t ka = p.kv.k_ptr + uint64_t(page * p.kv.k_page_stride +
-                                              off * p.kv.k_token_stride +
-                                              head * p.kv.k_head_stride) * 2;
-    const uint64_t va = p.kv.v_ptr + uint64_t(page * p.kv.v_page_stride +
-                                              off * p.kv.v_token_stride +
-                                              head * p.kv.v_head_stride) * 2;
     const uint32_t kdst = ring + st * stage_bytes<D>();
     const uint32_t vdst = kdst + kWarpTokens * kRowBytes;
     const int c = lane % kChunks;
     constexpr int kPer = 32 / kChunks;  // tokens a warp's 32 lanes copy at once
+    // lanes 0..15 place one token each
+    const int t = t0 + (lane & 15);
+    const int blk = p.block_shift >= 0 ? t >> p.block_shift : int(uint32_t(t) / uint32_t(bt));
+    const int off = t - blk * bt;
+    bool ok = t < ld.len;
+    const int first = __shfl_sync(~0u, blk, 0);
+    // 16 tokens touch at most 16 entries: one window holds them
+    if (ld.b != window_seq || first < window || first + 16 > window + 32) {
+      window = first;
+      window_seq = ld.b;
+      const int32_t* table =
+          ld.b < p.a.batch
+              ? reinterpret_cast<const int32_t*>(p.a.block_table) + ld.b * p.a.block_table_stride
+              : reinterpret_cast<const int32_t*>(p.a.prefix_table);
+      const int last = p.block_shift >= 0 ? (ld.len - 1) >> p.block_shift : (ld.len - 1) / bt;
+      entry = window + lane <= last ? __ldg(table + window + lane) : 0;
+    }
+    const int page = __shfl_sync(~0u, entry, blk - window);
+    if (ok && (page < 0 || page >= p.kv.pages)) {
+      raise(p.err);
+      ok = false;
+    }
+    const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
+    if (lane == 0) masks[st] = mask;
+    const T* kp = reinterpret_cast<const T*>(p.kv.k_ptr) + ld.head * p.kv.k_head_stride;
+    const T* vp = reinterpret_cast<const T*>(p.kv.v_ptr) + ld.head * p.kv.v_head_stride;
+    if (mask == 0xffffu && bt % kWarpTokens == 0) {
+      // all in one page: one address, even steps
+      const int r0 = lane / kChunks;
+      const T* kr = kp + page * p.kv.k_page_stride + (__shfl_sync(~0u, off, 0) + r0) * p.kv.k_token_stride + c * 8;
+      const T* vr = vp + page * p.kv.v_page_stride + (__shfl_sync(~0u, off, 0) + r0) * p.kv.v_token_stride + c * 8;
+      const int64_t ks = kPer * p.kv.k_token_stride, vs = kPer * p.kv.v_token_stride;
 #pragma unroll
-    for (int i = 0; i < kWarpTokens / kPer; ++i) {
-      const int r = i * kPer + lane / kChunks;
-      const uint64_t kr = __shfl_sync(~0u, ka, r), vr = __shfl_sync(~0u, va, r);
-      const bool in = (mask >> r) & 1;
-      const uint32_t at = r * kRowBytes + ((c ^ (r & 7)) << 4);
-      cp_async16(kdst + at, reinterpret_cast<const void*>((in ? kr : p.kv.k_ptr) + c * 16), in);
-      cp_async16(vdst + at, reinterpret_cast<const void*>((in ? vr : p.kv.v_ptr) + c * 16), in);
+      for (int i = 0; i < kWarpTokens / kPer; ++i) {
+        const int r = i * kPer + r0;
+        const uint32_t at = r * kRowBytes + ((c ^ (r & 7)) << 4);
+        cp_async16(kdst + at, kr, true);
+        cp_async16(vdst + at, vr, true);
+        kr += ks;
+        vr += vs;
+      }
+    } else {
+      const int64_t ko = page * p.kv.k_page_stride + off * p.kv.k_token_stride;
+      const int64_t vo = page * p.kv.v_page_stride + off * p.kv.v_token_stride;
+#pragma unroll
+      for (int i = 0; i < kWarpTokens / kPer; ++i) {
+        const int r = i * kPer + lane / kChunks;
+        const int64_t kr = __shfl_sync(~0u, ko, r), vr = __shfl_sync(~0u, vo, r);
+        const bool in = (mask >> r) & 1;
+        const uint32_t at = r * kRowBytes + ((c ^ (r & 7)) << 4);
+        // a source that is not read still is an address of the pages
+        cp_async16(kdst + at, in ? kp + kr + c * 8 : reinterpret_cast<const T*>(p.kv.k_ptr), in);
+        cp_async16(vdst + at, in ? vp + vr + c * 8 : reinterpret_cast<const T*>(p.kv.v_ptr), in);
+      }
     }
     cp_commit();
     if (++ld_tile == ld.end) {
@@ -354,8 +402,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
   int st = 0;
 
   while (!cu.done()) {
-    const int head = cu.sub % int(p.kv.heads);
-    const int row0 = (cu.sub / int(p.kv.heads)) * kRows;
+    const int head = cu.head;
+    const int row0 = cu.rt * kRows;
     const bool own = cu.b < p.a.batch;
     const int n_rows = own ? p.rows_own : p.rows_pre;
     // the query rows as mma A fragments, and what each of this thread's rows sees
@@ -371,12 +419,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
         const T* src = nullptr;
         vis[mt][hf] = cu.len;
         if (in) {
-          const int64_t tok = row_token(p, cu, row);
-          const int64_t b = tok / p.a.new_tokens, j = tok - b * p.a.new_tokens;
-          const int hq = head * p.group + row % p.group;
-          src = reinterpret_cast<const T*>(p.a.q) + b * p.a.q_batch_stride +
-                j * p.a.q_token_stride + hq * p.a.q_head_stride;
-          if (own) vis[mt][hf] = cu.len - int(p.a.new_tokens) + 1 + int(j);
+          const Row q = row_of(p, cu, row);
+          src = reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
+                q.j * p.a.q_token_stride + (head * p.group + q.g) * p.a.q_head_stride;
+          if (own) vis[mt][hf] = cu.len - int(p.a.new_tokens) + 1 + q.j;
         }
         vis_min = min(vis_min, vis[mt][hf]);
 #pragma unroll
@@ -554,8 +600,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
             da = p.slots_acc + (slot * kRows + rl) * D;
             dm = p.slots_ml + (slot * kRows + rl) * 2;
           } else {
-            const int64_t out_row = row_token(p, cu, row) * p.a.q_heads +
-                                    head * p.group + row % p.group;
+            const Row q = row_of(p, cu, row);
+            const int64_t out_row = (int64_t(q.b) * p.a.new_tokens + q.j) * p.a.q_heads +
+                                    head * p.group + q.g;
             if (own && p.a.prefix_blocks == 0) {
               // the whole row: the result itself
               const float li = l[mt][hf];
@@ -599,17 +646,15 @@ struct Part {
   }
 };
 
-// The part of a row (row rl of an item's `rows`) whose item holds the tiles
-// [start, start + nt) of `total`, shared by `ctas` CTAs.
-__device__ __forceinline__ Part part_of(int64_t total, int64_t ctas, int64_t start, int nt,
-                                        int rows, int rl, const float* slots_acc,
-                                        const float* slots_ml, const float* whole_acc,
-                                        const float* whole_ml, int64_t out_row) {
+// The part of a row (row rl of an item's `rows`) whose item holds the units
+// [first, last] of the cut.
+__device__ __forceinline__ Part part_of(const Cut& cut, int first, int last, int rows, int rl,
+                                        const float* slots_acc, const float* slots_ml,
+                                        const float* whole_acc, const float* whole_ml,
+                                        int64_t out_row) {
   Part r{};
-  if (nt == 0) return r;
-  // owner of tile t: the CTA whose share holds it
-  const int64_t w0 = ((start + 1) * ctas - 1) / total;
-  const int64_t w1 = ((start + nt) * ctas - 1) / total;
+  if (last < first) return r;
+  const int64_t w0 = cut.owner(first), w1 = cut.owner(last);
   r.count = int(w1 - w0) + 1;
   if (r.count == 1) {
     r.acc = whole_acc;
@@ -634,48 +679,49 @@ template <typename T, int D, int MT, int kSplit>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkParams p) {
   constexpr int kRows = 16 * MT, kPer = D / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t n_rows = p.a.batch * p.a.new_tokens * p.a.q_heads;
-  const int64_t out_row = kSplit == 1 ? int64_t(blockIdx.x) * 4 + warp : int64_t(blockIdx.x);
+  const int n_rows = int(p.a.batch * p.a.new_tokens * p.a.q_heads);
+  const int out_row = kSplit == 1 ? int(blockIdx.x) * 4 + warp : int(blockIdx.x);
   if (out_row >= n_rows) return;
-  const int tok = int(out_row / p.a.q_heads);
-  const int hq = int(out_row) - tok * int(p.a.q_heads);
-  const int b = tok / int(p.a.new_tokens);
-  const int head = hq / p.group;
-  const int64_t heads = p.kv.heads;
+  const int q_heads = int(p.a.q_heads), heads = int(p.kv.heads), batch = int(p.a.batch);
+  const int tok = int(uint32_t(out_row) / uint32_t(q_heads));
+  const int hq = out_row - tok * q_heads;
+  const int b = int(uint32_t(tok) / uint32_t(p.a.new_tokens));
+  const int head = int(uint32_t(hq) / uint32_t(p.group));
+  const int g = hq - head * p.group;
+  // units of all sequences, and of those before b
+  int total = 0, before = 0;
   bool bad;
-  // tiles of all sequences, and of those before b
-  int64_t total = 0, before = 0;
-  for (int i = lane; i < p.a.batch; i += 32) {
-    const int64_t t = tiles_of(p, i, &bad);
-    total += t;
-    before += i < b ? t : 0;
+  for (int i = lane; i < batch; i += 32) {
+    const int cost = cost_of(p, true, tokens_of(p, i, &bad));
+    total += cost;
+    before += i < b ? cost : 0;
   }
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) {
-    total += __shfl_xor_sync(~0u, total, k);
-    before += __shfl_xor_sync(~0u, before, k);
-  }
-  const int64_t own_total = total;
-  if (p.row_tiles_pre > 0) total += tiles_of(p, p.a.batch, &bad);
+  total = warp_sum(total);
+  before = warp_sum(before);
+  const int prefix = p.a.prefix_blocks > 0 ? tokens_of(p, batch, &bad) : 0;
+  const int pre_first = total;
+  if (p.row_tiles_pre > 0) total += cost_of(p, false, prefix);
 
-  const int64_t ctas = sharers(total, p.ctas);
-  const int nt = (tokens_of(p, b, &bad) + kTile - 1) / kTile;
-  const int own_row = (tok - b * int(p.a.new_tokens)) * p.group + hq % p.group;
-  const Part own = part_of(total, ctas, before + (own_row / kRows * heads + head) * nt, nt, kRows,
-                           own_row % kRows, p.slots_acc, p.slots_ml, p.own_acc, p.own_ml, out_row);
+  const Cut cut(total, p.ctas);
+  const int nt = tiles_in(tokens_of(p, b, &bad));
+  const int own_row = (tok - b * int(p.a.new_tokens)) * p.group + g;
+  int first = before + (own_row / kRows * heads + head) * (nt + kItemCost) + kItemCost;
+  const Part own = part_of(cut, first, first + nt - 1, kRows, own_row % kRows, p.slots_acc,
+                           p.slots_ml, p.own_acc, p.own_ml, out_row);
   if (p.a.prefix_blocks == 0 && own.count == 1) return;  // written by walk_kernel
-  const int64_t row = int64_t(tok) * p.group + hq % p.group;
+  const int row = tok * p.group + g;
   Part pre{};
   if (p.row_tiles_pre > 0) {
-    const int n = (tokens_of(p, p.a.batch, &bad) + kTile - 1) / kTile;
-    pre = part_of(total, ctas, own_total + (row / kRows * heads + head) * n, n, kRows,
-                  int(row % kRows), p.slots_acc, p.slots_ml, p.pre_acc, p.pre_ml, out_row);
+    const int n = tiles_in(prefix);
+    first = pre_first + (row / kRows * heads + head) * (n + kItemCost) + kItemCost;
+    pre = part_of(cut, first, first + n - 1, kRows, row % kRows, p.slots_acc, p.slots_ml,
+                  p.pre_acc, p.pre_ml, out_row);
   } else if (p.tensor_ctas > 0) {
-    const int n = (tokens_of(p, p.a.batch, &bad) + kPrefixTile - 1) / kPrefixTile;
-    const int64_t all = int64_t(n) * p.tensor_row_tiles * heads;
-    pre = part_of(all, sharers(all, p.tensor_ctas), (row / kPrefixRows * heads + head) * n, n,
-                  kPrefixRows, int(row % kPrefixRows), p.tensor_acc, p.tensor_ml, p.pre_acc,
-                  p.pre_ml, out_row);
+    const int n = (prefix + kPrefixTile - 1) / kPrefixTile;
+    first = (row / kPrefixRows * heads + head) * n;
+    pre = part_of(Cut(n * p.tensor_row_tiles * heads, p.tensor_ctas), first, first + n - 1,
+                  kPrefixRows, row % kPrefixRows, p.tensor_acc, p.tensor_ml, p.pre_acc, p.pre_ml,
+                  out_row);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -748,7 +794,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkP
     }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  T* out = reinterpret_cast<T*>(p.a.out) + out_row * D + lane * kPer;
+  T* out = reinterpret_cast<T*>(p.a.out) + int64_t(out_row) * D + lane * kPer;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2)
     *reinterpret_cast<uint32_t*>(out + e) = Ops<T>::pack(o[e] * inv, o[e + 1] * inv);
@@ -792,6 +838,15 @@ int check_attention(const ts_paged_kv* kv, const ts_attention_args* args) {
   if (a.max_blocks > INT32_MAX / 2 / kv->block_tokens ||
       a.prefix_blocks > INT32_MAX / 2 / kv->block_tokens)
     return set_error(TS_INVALID_ARGUMENT, "block tables hold too many tokens");
+  // units of work are counted in 31 bits: items times their tiles
+  const double rows = double(a.new_tokens) * double(a.q_heads / kv->heads);
+  const double own_items = double(a.batch) * kv->heads * (rows / 16 + 1);
+  const double pre_items = double(kv->heads) * (a.batch * rows / 16 + 1);
+  const double bt = double(kv->block_tokens);
+  if (own_items * (a.max_blocks * bt / kTile + 1 + kItemCost) +
+          (a.prefix_blocks > 0 ? pre_items * (a.prefix_blocks * bt / kTile + 1 + kItemCost) : 0) >
+      double(INT32_MAX))
+    return set_error(TS_INVALID_ARGUMENT, "batch, heads and table capacity too large for one call");
   if (!(a.scale > 0.f) || !std::isfinite(a.scale))
     return set_error(TS_INVALID_ARGUMENT, "scale must be finite and positive");
   return TS_OK;
@@ -931,6 +986,9 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
   p.pre_ml = reinterpret_cast<float*>(base + w.pre_ml);
   p.err = err_flag;
   p.ctas = w.ctas;
+  p.block_shift = (kv->block_tokens & (kv->block_tokens - 1)) == 0
+                      ? __builtin_ctzll(uint64_t(kv->block_tokens))
+                      : -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (w.tensor) {
     tsb::PrefixParams t{};

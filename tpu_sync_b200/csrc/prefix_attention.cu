@@ -224,14 +224,12 @@ struct Segment {
   int unit, tile, count;
 };
 struct Shares {
-  int64_t lo, hi;
-  int nt;
+  int lo, hi, nt;
   __device__ __forceinline__ bool next(Segment* s) {
     if (lo >= hi) return false;
-    s->unit = int(lo / nt);
-    s->tile = int(lo - int64_t(s->unit) * nt);
-    const int64_t left = hi - lo;
-    s->count = int(left < nt - s->tile ? left : nt - s->tile);
+    s->unit = int(uint32_t(lo) / uint32_t(nt));
+    s->tile = lo - s->unit * nt;
+    s->count = min(hi - lo, nt - s->tile);
     lo += s->count;
     return true;
   }
@@ -261,13 +259,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int heads = int(p.kv.heads);
   Shares shares{};
   shares.nt = (len + kPrefixTile - 1) / kPrefixTile;
-  const int64_t total = int64_t(shares.nt) * p.row_tiles * heads;
+  const Cut cut(shares.nt * p.row_tiles * heads, p.ctas);
   if (bad && blockIdx.x == 0 && threadIdx.x == 0 && p.err)
     *reinterpret_cast<volatile int*>(p.err) = 1;
-  const int64_t ctas = total < p.ctas ? total : p.ctas;
-  if (blockIdx.x >= ctas) return;
-  shares.lo = total * blockIdx.x / ctas;
-  shares.hi = total * (blockIdx.x + 1) / ctas;
+  if (blockIdx.x >= cut.ctas) return;
+  shares.lo = cut.start(blockIdx.x);
+  shares.hi = cut.start(blockIdx.x + 1);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -437,8 +434,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int row = row0 + rr;
           int4 v = make_int4(0, 0, 0, 0);
           if (row < p.rows) {
-            const int64_t tok = row / p.group;
-            const int64_t b = tok / p.a.new_tokens, jj = tok - b * p.a.new_tokens;
+            const int tok = int(uint32_t(row) / uint32_t(p.group));
+            const int b = int(uint32_t(tok) / uint32_t(p.a.new_tokens));
+            const int jj = tok - b * int(p.a.new_tokens);
             v = *reinterpret_cast<const int4*>(
                 reinterpret_cast<const T*>(p.a.q) + b * p.a.q_batch_stride +
                 jj * p.a.q_token_stride +
@@ -550,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float *da = nullptr, *dm = nullptr;
       if (row < p.rows) {
         if (seg.count == shares.nt) {
-          const int64_t tok = row / p.group;
+          const int tok = int(uint32_t(row) / uint32_t(p.group));
           const int64_t out_row = tok * p.a.q_heads + head * p.group + row - tok * p.group;
           da = p.whole_acc + out_row * D;
           dm = p.whole_ml + out_row * 2;

@@ -29,6 +29,23 @@ struct PrefixParams {
   int* err;
 };
 
+// CTA w of n takes units [w q + min(w, r), ...) of the total = q n + r; n is
+// cut to the units there are, so that every CTA has one.
+struct Cut {
+  int ctas, q, r;
+  __device__ __forceinline__ Cut(int total, int most) {
+    ctas = total < most ? total : most;
+    q = ctas > 0 ? int(uint32_t(total) / uint32_t(ctas)) : 0;
+    r = total - q * ctas;
+  }
+  __device__ __forceinline__ int start(int w) const { return q * w + min(w, r); }
+  __device__ __forceinline__ int owner(int unit) const {
+    const int big = r * (q + 1);
+    return unit < big ? int(uint32_t(unit) / uint32_t(q + 1))
+                      : r + int(uint32_t(unit - big) / uint32_t(q));
+  }
+};
+
 // Whether the kernel takes this page geometry (else the walk over 64-token
 // tiles reads the prefix too).
 bool prefix_geometry_ok(const ts_paged_kv& kv);
