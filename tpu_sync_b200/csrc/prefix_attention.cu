@@ -18,7 +18,7 @@
 //                   accumulator is rescaled only when a maximum grew by more
 //                   than 2^8: m is any common reference, so the result is the
 //                   same, and P stays below 2^8.
-//   warp 8          page lookups and TMA loads of K and V tiles into a ring.
+//   warps 8, 10     page lookups and TMA loads of K and of V tiles into a ring.
 //   warp 9          all tcgen05.mma: while one half's softmax runs, the other
 //                   half's products do.
 //
@@ -56,7 +56,7 @@ struct Shape {
   static constexpr int kTileBytes = kPrefixTile * D * 2;  // a K or V tile
   static constexpr int kStages = D == 128 ? 5 : 9;
   static constexpr int kQBytes = kPrefixRows * D * 2;
-  static constexpr int kBars = 2 * kStages + 8;
+  static constexpr int kBars = 2 * kStages + 12;
   static constexpr int kSmem = kQBytes + kStages * kTileBytes + kBars * 8 + 16 + 1024;
 };
 
@@ -93,6 +93,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
   return __all_sync(~0u, ok);
 }
 
+// The same for one thread.
+__device__ __forceinline__ bool bar_wait_one(uint32_t bar, uint32_t parity, volatile int* gone) {
+  bool ok = bar_try(bar, parity);
+  for (uint32_t i = 0; !ok && i < kWaitRounds && !*gone; ++i) ok = bar_try(bar, parity);
+  if (!ok) *gone = 1;
+  return ok;
+}
+
 __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
                                        int token, int head, int page) {
   asm volatile(
@@ -112,6 +120,14 @@ __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
       : "memory");
+}
+// One lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
 }
 // D[tmem] (+)= A B, both operands in shared memory
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
@@ -205,6 +221,31 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+__device__ __forceinline__ float2 pair(float x) { return make_float2(x, x); }
+// The largest of three; NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x on the multiply-add pipe, for -126 <= x < 128 (smaller x count as -126,
+// which next to a row's maximum is nothing): x = i + f with |f| <= 1/2, 2^f by
+// the polynomial of degree 4 with the least relative error there (2.6e-6, by
+// Remez exchange), i added to its exponent.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+  const float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = add2(x, pair(kRound));
+  const float2 i = add2(t, pair(-kRound));
+  const float2 f = fma2(i.x, i.y, pair(-1.f), x);
+  float2 y = fma2(f.x, f.y, pair(0.009570102207362652f), pair(0.05591785907745361f));
+  y = fma2(y.x, y.y, f, pair(0.240247443318367f));
+  y = fma2(y.x, y.y, f, pair(0.6931217908859253f));
+  y = fma2(y.x, y.y, f, pair(0.9999992847442627f));
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -247,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* ctl = smem + S::kQBytes + S::kStages * S::kTileBytes;
   const uint32_t bars = smem_u32(ctl);
   const uint32_t full = bars, empty = bars + 8 * S::kStages, q_full = bars + 16 * S::kStages,
-                 s_full = q_full + 16, p_ready = q_full + 32, o_full = q_full + 48;
+                 s_full = q_full + 16, p_ready = q_full + 32, o_full = q_full + 64, v_cut = q_full + 80;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 8 * S::kBars);
   volatile int* gone = reinterpret_cast<volatile int*>(ctl + 8 * S::kBars + 4);
 
@@ -274,9 +315,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int x = 0; x < 2; ++x) {
       bar_init(q_full + 8 * x, 128);
       bar_init(s_full + 8 * x, 1);
-      bar_init(p_ready + 8 * x, 4);
+      bar_init(p_ready + 16 * x, 4);  // keys 0-63 of the tile
+      bar_init(p_ready + 16 * x + 8, 4);
       bar_init(o_full + 8 * x, 1);
     }
+    bar_init(v_cut, 1);
     *gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -297,119 +340,152 @@ __global__ void __launch_bounds__(kThreads, 1)
   // gives up registers for them: 2 x 128 x 208 + 128 x 88 = 384 x 168.
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8) {
-    // -- loads ----------------------------------------------------------------
-    const int pieces = kPrefixTile / p.piece;
-    uint32_t n = 0;  // tiles loaded, K and V counted apart
-    bool ok = true;
-    while (ok && shares.next(&seg)) {
-      const int head = seg.unit % heads;
-      for (int j = 0; ok && j < seg.count; ++j) {
-        // lane i < pieces places piece i; the page past the last one loads zeros
-        int page = int(p.kv.pages), off = 0;
-        const int t = (seg.tile + j) * kPrefixTile + lane * p.piece;
-        if (lane < pieces && t < len) {
-          const int blk = t / bt;
-          off = t - blk * bt;
-          const int id = table[blk];
-          if (id >= 0 && id < p.kv.pages) {
-            page = id;
-          } else if (p.err) {
-            *reinterpret_cast<volatile int*>(p.err) = 1;
+    if (warp == 8 || warp == 10) {
+      // -- loads: warp 8 the K tiles, warp 10 the V tiles ------------------------
+      const int pieces = kPrefixTile / p.piece;
+      const CUtensorMap* map = warp == 8 ? &kmap : &vmap;
+      uint32_t n = warp == 8 ? 0 : 1;  // ring position: K and V tiles alternate
+      bool ok = true;
+      while (ok && shares.next(&seg)) {
+        const int head = seg.unit % heads;
+        // lane i < pieces places piece i of a tile; what is past the length, or of
+        // no page, loads zeros: the page after the last one
+        auto place = [&](int tile, int* off) {
+          const int t = tile * kPrefixTile + lane * p.piece;
+          int page = int(p.kv.pages);
+          *off = 0;
+          if (lane < pieces && t < len) {
+            const int blk = int(uint32_t(t) / uint32_t(bt));
+            *off = t - blk * bt;
+            page = __ldg(table + blk);
           }
-        }
-        for (int kv = 0; kv < 2; ++kv, ++n) {
-          const uint32_t st = n % S::kStages, round = n / S::kStages;
-          ok = bar_wait(empty + 8 * st, (round & 1) ^ 1, gone);
-          if (!ok) break;
-          if (lane == 0) bar_expect(full + 8 * st, S::kTileBytes);
+          return page;
+        };
+        int off, page = place(seg.tile, &off);
+        for (int j = 0; ok && j < seg.count; ++j, n += 2) {
+          if (page < 0 || page > p.kv.pages ||
+              (page == p.kv.pages && lane < pieces &&
+               (seg.tile + j) * kPrefixTile + lane * p.piece < len)) {
+            if (p.err) *reinterpret_cast<volatile int*>(p.err) = 1;
+            page = int(p.kv.pages);
+          }
+          int next_off = 0, next = 0;
+          if (j + 1 < seg.count) next = place(seg.tile + j + 1, &next_off);
+          const uint32_t st = n % S::kStages;
+          if (n >= S::kStages) {
+            // the stage's last tile was released with group g
+            const uint32_t g = (n - S::kStages + 1) / 2;
+            ok = bar_wait(empty + 8 * (g % S::kStages), (g / S::kStages) & 1, gone);
+            if (!ok) break;
+          }
+          if (elect()) bar_expect(full + 8 * st, S::kTileBytes);
           __syncwarp();
-          if (lane < pieces) {
-            const uint32_t dst = ring + st * S::kTileBytes + lane * p.piece * 128;
+          const uint32_t dst = ring + st * S::kTileBytes;
+          for (int i = 0; i < pieces; ++i) {
+            const int pg = __shfl_sync(~0u, page, i), of = __shfl_sync(~0u, off, i);
+            if (elect()) {
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h)
-              tma_4d(dst + h * kPrefixTile * 128, kv ? &vmap : &kmap, full + 8 * st, h * 64, off,
-                     head, page);
+              for (int h = 0; h < D / 64; ++h)
+                tma_4d(dst + i * p.piece * 128 + h * kPrefixTile * 128, map, full + 8 * st, h * 64,
+                       of, head, pg);
+            }
+            __syncwarp();
+          }
+          page = next;
+          off = next_off;
+          const int past = len - (seg.tile + j) * kPrefixTile;  // keys of this tile that count
+          if (warp == 10 && past < kPrefixTile) {
+            // V rows past the length: whatever the page holds must not meet a weight of 0
+            ok = bar_wait(full + 8 * st, (n / S::kStages) & 1, gone);
+            if (!ok) break;
+            for (int i = lane; i < (kPrefixTile - past) * (D / 64) * 8; i += 32) {
+              const int r = past + i / (D / 64 * 8), c = i % (D / 64 * 8);
+              const uint32_t at = dst + (c / 8) * kPrefixTile * 128 + r * 128 + (c % 8) * 16;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(v_cut);
           }
         }
       }
-    }
-    } else if (warp == 9) {
-    // -- matrix products --------------------------------------------------------
-    constexpr uint32_t kIdescS = InstrDesc<T, kPrefixTile, false>::value;
-    constexpr uint32_t kIdescO = InstrDesc<T, D, true>::value;
-    uint32_t n = 0;              // ring position (as the loads')
-    uint32_t q_n[2] = {0, 0}, p_n[2] = {0, 0};
-    bool ok = true;
-    auto scores = [&](int x, uint32_t st) {
-      if (lane == 0) {
-        const uint32_t a = q_smem + x * 128 * 128, b = ring + st * S::kTileBytes;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          // 64 elements (four steps) per 128-byte block
-          const uint64_t ad = smem_desc(a + (k / 4) * kPrefixRows * 128 + (k % 4) * 32, 16);
-          const uint64_t bd = smem_desc(b + (k / 4) * kPrefixTile * 128 + (k % 4) * 32, 16);
-          mma_ss(tmem_s + 128 * x, ad, bd, kIdescS, k > 0);
+    } else if (warp == 9 && elect()) {
+      // -- matrix products, all by one thread -------------------------------------
+      constexpr uint32_t kIdescS = InstrDesc<T, kPrefixTile, false>::value;
+      constexpr uint32_t kIdescO = InstrDesc<T, D, true>::value;
+      // descriptors of tile 0 of each operand; the 14-bit addresses count 16 bytes
+      const uint64_t q_desc = smem_desc(q_smem, 16), k_desc = smem_desc(ring, 16),
+                     v_desc = smem_desc(ring, kPrefixTile * 128);
+      uint32_t n = 0;                   // ring position: K0 V0 K1 V1 ...
+      uint32_t st = 0, st_phase = 0;    // n % kStages, n / kStages
+      uint32_t q_n[2] = {0, 0}, p_n[2] = {0, 0}, cuts = 0;
+      bool ok = true;
+      auto advance = [&] {
+        ++n;
+        if (++st == S::kStages) {
+          st = 0;
+          ++st_phase;
         }
+      };
+      auto scores = [&](int x) {
+        const uint64_t a = q_desc + x * (128 * 128 / 16), b = k_desc + st * (S::kTileBytes / 16);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)  // 64 elements (four steps) per 128-byte block
+          mma_ss(tmem_s + 128 * x, a + ((k / 4) * kPrefixRows * 128 + (k % 4) * 32) / 16,
+                 b + ((k / 4) * kPrefixTile * 128 + (k % 4) * 32) / 16, kIdescS, k > 0);
         commit(s_full + 8 * x);
-      }
-      __syncwarp();
-    };
-    while (ok && shares.next(&seg)) {
-      const int rt = seg.unit / heads;
-      const int halves = p.rows - rt * kPrefixRows > 128 ? 2 : 1;
-      ok = bar_wait(full + 8 * (n % S::kStages), (n / S::kStages) & 1, gone);
-      for (int x = 0; ok && x < halves; ++x) {
-        ok = bar_wait(q_full + 8 * x, q_n[x] & 1, gone);
-        ++q_n[x];
-        fence_after();
-        if (ok) scores(x, n % S::kStages);
-      }
-      if (lane == 0) commit(empty + 8 * (n % S::kStages));
-      ++n;
-      for (int j = 0; ok && j < seg.count; ++j) {
-        const uint32_t vst = n % S::kStages;
-        ok = bar_wait(full + 8 * vst, (n / S::kStages) & 1, gone);
-        const int past = len - (seg.tile + j) * kPrefixTile;  // keys of this tile that count
-        if (ok && past < kPrefixTile) {
-          // V rows past the length: whatever the page holds must not meet a weight of 0
-          for (int i = lane; i < (kPrefixTile - past) * (D / 64) * 8; i += 32) {
-            const int r = past + i / (D / 64 * 8), c = i % (D / 64 * 8);
-            const uint32_t at = ring + vst * S::kTileBytes + (c / 8) * kPrefixTile * 128 +
-                                r * 128 + (c % 8) * 16;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        __syncwarp();
-        const bool more = j + 1 < seg.count;
+      };
+      // Group g = V tile j and K tile j + 1 (and the last V tile with the next
+      // segment's first K tile): read for the last time by the products up to
+      // here, released by one commit.
+      auto release = [&] { commit(empty + 8 * ((n / 2) % S::kStages)); };
+      while (ok && shares.next(&seg)) {
+        const int rt = seg.unit / heads;
+        const int halves = p.rows - rt * kPrefixRows > 128 ? 2 : 1;
+        ok = bar_wait_one(full + 8 * st, st_phase & 1, gone);
         for (int x = 0; ok && x < halves; ++x) {
-          ok = bar_wait(p_ready + 8 * x, p_n[x] & 1, gone);
-          ++p_n[x];
+          ok = bar_wait_one(q_full + 8 * x, q_n[x] & 1, gone);
+          ++q_n[x];
           fence_after();
-          if (!ok) break;
-          if (lane == 0) {
+          if (ok) scores(x);
+        }
+        release();
+        advance();
+        for (int j = 0; ok && j < seg.count; ++j) {
+          const uint64_t vb = v_desc + st * (S::kTileBytes / 16);
+          ok = bar_wait_one(full + 8 * st, st_phase & 1, gone);
+          if (len - (seg.tile + j) * kPrefixTile < kPrefixTile) {
+            ok = ok && bar_wait_one(v_cut, cuts & 1, gone);
+            ++cuts;
+          }
+          advance();  // to the next K tile (or the next segment's)
+          const bool more = j + 1 < seg.count;
+          for (int x = 0; ok && x < halves; ++x) {
 #pragma unroll
-            for (int k = 0; k < kPrefixTile / 16; ++k)
-              mma_ts(tmem_o + D * x, tmem_s + 128 * x + 8 * k,
-                     smem_desc(ring + vst * S::kTileBytes + k * 16 * 128, kPrefixTile * 128),
-                     kIdescO, j > 0 || k > 0);
-            if (!more) commit(o_full + 8 * x);
+            for (int h = 0; h < 2; ++h) {
+              ok = ok && bar_wait_one(p_ready + 16 * x + 8 * h, p_n[x] & 1, gone);
+              if (!ok) break;
+              fence_after();
+#pragma unroll
+              for (int k = 4 * h; k < 4 * h + 4; ++k)
+                mma_ts(tmem_o + D * x, tmem_s + 128 * x + 8 * k, vb + k * (16 * 128 / 16), kIdescO,
+                       j > 0 || k > 0);
+            }
+            ++p_n[x];
+            if (!ok) break;
+            if (more) {
+              if (x == 0) ok = bar_wait_one(full + 8 * st, st_phase & 1, gone);
+              if (ok) scores(x);
+            } else {
+              commit(o_full + 8 * x);
+            }
           }
-          __syncwarp();
           if (more) {
-            if (x == 0)
-              ok = bar_wait(full + 8 * ((n + 1) % S::kStages), ((n + 1) / S::kStages) & 1, gone);
-            if (ok) scores(x, (n + 1) % S::kStages);
+            release();
+            advance();
           }
         }
-        if (lane == 0) {
-          commit(empty + 8 * vst);
-          if (more) commit(empty + 8 * ((n + 1) % S::kStages));
-        }
-        n += more ? 2 : 1;
       }
-    }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -428,24 +504,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       {
         constexpr int kC = D / 8;
         const int c = r % kC;
-#pragma unroll 8
+        int4 v[kC];
+#pragma unroll
         for (int i = 0; i < kC; ++i) {
-          const int rr = i * (128 / kC) + r / kC;
-          const int row = row0 + rr;
-          int4 v = make_int4(0, 0, 0, 0);
+          const int row = row0 + i * (128 / kC) + r / kC;
+          v[i] = make_int4(0, 0, 0, 0);
           if (row < p.rows) {
             const int tok = int(uint32_t(row) / uint32_t(p.group));
-            const int b = int(uint32_t(tok) / uint32_t(p.a.new_tokens));
+            const int b = p.a.new_tokens == 1 ? tok : int(uint32_t(tok) / uint32_t(p.a.new_tokens));
             const int jj = tok - b * int(p.a.new_tokens);
-            v = *reinterpret_cast<const int4*>(
+            v[i] = *reinterpret_cast<const int4*>(
                 reinterpret_cast<const T*>(p.a.q) + b * p.a.q_batch_stride +
                 jj * p.a.q_token_stride +
                 (head * p.group + row - tok * p.group) * p.a.q_head_stride + c * 8);
           }
+        }
+#pragma unroll
+        for (int i = 0; i < kC; ++i) {
+          const int rr = i * (128 / kC) + r / kC;
           const uint32_t at = q_smem + (c / 8) * kPrefixRows * 128 + (x * 128 + rr) * 128 +
                               (((c % 8) ^ (rr & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y),
-                       "r"(v.z), "r"(v.w)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x),
+                       "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
                        : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -474,7 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 4; ++c) tmem_ld32(s + 32 * c, ts + 32 * c);
         tmem_wait_ld();
         const int t0 = (seg.tile + j) * kPrefixTile;
-        if (hole || t0 + kPrefixTile > len) {
+        const bool masked = hole || t0 + kPrefixTile > len;
+        if (masked) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int t = t0 + 32 * c + lane;
@@ -492,9 +573,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int k = 0; k < kPrefixTile; k += 2)
-          mx[k / 2 % 4] = fmaxf(fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
-                                mx[k / 2 % 4]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+          mx[k / 2 % 4] = max3(__uint_as_float(s[k]), __uint_as_float(s[k + 1]), mx[k / 2 % 4]);
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * p.scale_log2;
+        if (!(top < INFINITY)) m = NAN;  // a score is NaN or infinite: so is the row
         const bool grew = top > m + 8.f;
         if (__any_sync(~0u, grew)) {
           const float f = grew ? ex2(m - top) : 1.f;
@@ -513,30 +594,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : -m;
-        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-        const float2 base2 = make_float2(base, base);
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        const float2 scale2 = pair(p.scale_log2), base2 = pair(m == -INFINITY ? 0.f : -m);
+        float2 sum[2] = {pair(0.f), pair(0.f)};
+        // 32 keys of the row; the first half of the tile's keys goes to the
+        // tensor cores while the second is worked on
+        auto keys = [&](int c, bool spread) {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             float2 e = fma2(__uint_as_float(s[32 * c + 2 * k]),
                             __uint_as_float(s[32 * c + 2 * k + 1]), scale2, base2);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
+            if (spread && k % 4 == 3) {
+              e = ex2_fma(e);
+            } else {
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+            }
             sum[k % 2] = add2(sum[k % 2], e);
             pk[k] = pack2(e.x, e.y, T{});
           }
           tmem_st16(ts + 16 * c, pk);
+          if (c % 2 == 1) {
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(p_ready + 16 * x + 8 * (c / 2));
+          }
+        };
+        // Masked tiles need exact zeros; in the others a quarter of the
+        // exponentials leave the special function unit (16 a cycle and SM, the
+        // scarcest next to the tensor cores) for the multiply-add pipe.
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) keys(c, false);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) keys(c, true);
         }
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
-        tmem_wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(p_ready + 8 * x);
       }
       if (!ok) break;
       ok = bar_wait(o_full + 8 * x, o_n & 1, gone);
@@ -586,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 100; ++i) __nanosleep(100000);
     __syncthreads();
   }
+  __syncwarp();
   if (warp == 9)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
