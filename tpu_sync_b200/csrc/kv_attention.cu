@@ -145,39 +145,38 @@ struct Cursor {
 
 constexpr int kLensHeld = 4;  // lengths a lane keeps: batches up to 128 are read once
 
-// Finds the CTA's share and its first item; done() when it has none.
-__device__ __forceinline__ Cursor start_cursor(const WalkParams& p) {
-  Cursor c{};
-  const int lane = threadIdx.x & 31;
-  const int seqs = c.seqs(p);
+// The lengths of the batch (and, as sequence `batch`, of a prefix that the
+// walk reads), the first 128 of them held by the warp's lanes, and the cut of
+// all units between CTAs.
+struct Lengths {
   int held[kLensHeld];
-  bool bad = false;
+  int seqs;
+  __device__ __forceinline__ Cut read(const WalkParams& p, bool flag) {
+    const int lane = threadIdx.x & 31;
+    seqs = int(p.a.batch) + (p.row_tiles_pre > 0 ? 1 : 0);
+    bool bad = false;
 #pragma unroll
-  for (int k = 0; k < kLensHeld; ++k) {
-    bool now = false;
-    const int i = 32 * k + lane;
-    held[k] = i < seqs ? tokens_of(p, i, &now) : 0;
-    bad = bad || now;
-  }
-  int sum = 0;
+    for (int k = 0; k < kLensHeld; ++k) {
+      bool now = false;
+      const int i = 32 * k + lane;
+      held[k] = i < seqs ? tokens_of(p, i, &now) : 0;
+      bad = bad || now;
+    }
+    int sum = 0;
 #pragma unroll
-  for (int k = 0; k < kLensHeld; ++k) sum += cost_of(p, 32 * k + lane < p.a.batch, held[k]);
-  for (int i = 32 * kLensHeld + lane; i < seqs; i += 32) {
-    bool now;
-    sum += cost_of(p, i < p.a.batch, tokens_of(p, i, &now));
-    bad = bad || now;
+    for (int k = 0; k < kLensHeld; ++k) sum += cost_of(p, 32 * k + lane < p.a.batch, held[k]);
+    for (int i = 32 * kLensHeld + lane; i < seqs; i += 32) {
+      bool now;
+      sum += cost_of(p, i < p.a.batch, tokens_of(p, i, &now));
+      bad = bad || now;
+    }
+    if (flag && bad) raise(p.err);
+    return Cut(warp_sum(sum), p.ctas);
   }
-  if (bad) raise(p.err);
-  const Cut cut(warp_sum(sum), p.ctas);
-  const int w = blockIdx.x;
-  if (w >= cut.ctas) return c;
-  const int lo = cut.start(w);
-  c.left = cut.start(w + 1) - lo;
-  int base = 0;
-  for (int k = 0; 32 * k < seqs; ++k) {
+  __device__ __forceinline__ int get(const WalkParams& p, int k) const {
     int len = 0;
     bool ignore;
-    const int i = 32 * k + lane;
+    const int i = 32 * k + (threadIdx.x & 31);
     if (k < kLensHeld) {
 #pragma unroll
       for (int h = 0; h < kLensHeld; ++h)
@@ -185,29 +184,62 @@ __device__ __forceinline__ Cursor start_cursor(const WalkParams& p) {
     } else if (i < seqs) {
       len = tokens_of(p, i, &ignore);
     }
-    const int cost = cost_of(p, i < p.a.batch, len);
+    return len;
+  }
+};
+
+// The item that holds a unit (there is one), and the unit's place in it.
+struct Item {
+  int b, rt, head, len, nt, u;
+};
+__device__ __forceinline__ Item item_at(const WalkParams& p, const Lengths& lens, int unit) {
+  Item it{};
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int k = 0; 32 * k < lens.seqs; ++k) {
+    const int len = lens.get(p, k);
+    const int cost = cost_of(p, 32 * k + lane < p.a.batch, len);
     int run = cost;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
       const int up = __shfl_up_sync(~0u, run, m);
       if (lane >= m) run += up;
     }
-    const unsigned past = __ballot_sync(~0u, base + run > lo);
+    const unsigned past = __ballot_sync(~0u, base + run > unit);
     if (past) {
       const int at = __ffs(past) - 1;
-      c.b = 32 * k + at;
-      c.len = __shfl_sync(~0u, len, at);
-      c.nt = tiles_in(c.len);
-      const int in_seq = lo - base - __shfl_sync(~0u, run - cost, at);
-      const int item = c.nt + kItemCost;
+      it.b = 32 * k + at;
+      it.len = __shfl_sync(~0u, len, at);
+      it.nt = tiles_in(it.len);
+      const int in_seq = unit - base - __shfl_sync(~0u, run - cost, at);
+      const int item = it.nt + kItemCost;
       const int sub = int(uint32_t(in_seq) / uint32_t(item));
-      c.rt = int(uint32_t(sub) / uint32_t(p.kv.heads));
-      c.head = sub - c.rt * int(p.kv.heads);
-      c.take(in_seq - sub * item);
-      return c;
+      it.u = in_seq - sub * item;
+      it.rt = int(uint32_t(sub) / uint32_t(p.kv.heads));
+      it.head = sub - it.rt * int(p.kv.heads);
+      return it;
     }
     base += __shfl_sync(~0u, run, 31);
   }
+  return it;
+}
+
+// The CTA's share; done() when it has none.
+__device__ __forceinline__ Cursor start_cursor(const WalkParams& p) {
+  Cursor c{};
+  Lengths lens;
+  const Cut cut = lens.read(p, true);
+  const int w = blockIdx.x;
+  if (w >= cut.ctas) return c;
+  const int lo = cut.start(w);
+  const Item it = item_at(p, lens, lo);
+  c.left = cut.start(w + 1) - lo;
+  c.b = it.b;
+  c.rt = it.rt;
+  c.head = it.head;
+  c.len = it.len;
+  c.nt = it.nt;
+  c.take(it.u);
   return c;
 }
 
@@ -290,14 +322,14 @@ __host__ __device__ constexpr int walk_smem() {
 struct Row {
   int b, j, g;
 };
-__device__ __forceinline__ Row row_of(const WalkParams& p, const Cursor& c, int row) {
+__device__ __forceinline__ Row row_of(const WalkParams& p, int seq, int row) {
   Row r;
   const int n = int(p.a.new_tokens);
   const int tok = int(uint32_t(row) / uint32_t(p.group));
   r.g = row - tok * p.group;
   const int b = n == 1 ? tok : int(uint32_t(tok) / uint32_t(n));
   r.j = tok - b * n;
-  r.b = c.b < p.a.batch ? c.b : b;  // an own item's rows are of one sequence: b is 0
+  r.b = seq < p.a.batch ? seq : b;  // an own item's rows are of one sequence: b is 0
   return r;
 }
 
@@ -419,7 +451,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
         const T* src = nullptr;
         vis[mt][hf] = cu.len;
         if (in) {
-          const Row q = row_of(p, cu, row);
+          const Row q = row_of(p, cu.b, row);
           src = reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
                 q.j * p.a.q_token_stride + (head * p.group + q.g) * p.a.q_head_stride;
           if (own) vis[mt][hf] = cu.len - int(p.a.new_tokens) + 1 + q.j;
@@ -600,7 +632,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
             da = p.slots_acc + (slot * kRows + rl) * D;
             dm = p.slots_ml + (slot * kRows + rl) * 2;
           } else {
-            const Row q = row_of(p, cu, row);
+            const Row q = row_of(p, cu.b, row);
             const int64_t out_row = (int64_t(q.b) * p.a.new_tokens + q.j) * p.a.q_heads +
                                     head * p.group + q.g;
             if (own && p.a.prefix_blocks == 0) {
@@ -671,105 +703,61 @@ __device__ __forceinline__ Part part_of(const Cut& cut, int first, int last, int
   return r;
 }
 
-// kSplit warps per query row join the partials of its own part and of its
-// prefix part.  Rows that walk_kernel finished itself are left alone; rows
-// whose sequence is empty are written here.  All that depends on the lengths
-// alone is done before waiting for the kernels that write the partials.
-template <typename T, int D, int MT, int kSplit>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkParams p) {
-  constexpr int kRows = 16 * MT, kPer = D / 32;
+// Joins the partials of one query row's own part and prefix part by kSplit
+// warps (a whole CTA if that is more than one), in a fixed order, and writes
+// the row.  A warp takes kAtOnce partials at a time (its own of every kSplit),
+// all loads of them before the first is used.
+template <typename T, int D, int kSplit, int kAtOnce>
+__device__ __forceinline__ void join_row(const WalkParams& p, const Part& own, const Part& pre,
+                                         int64_t out_row) {
+  constexpr int kPer = D / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n_rows = int(p.a.batch * p.a.new_tokens * p.a.q_heads);
-  const int out_row = kSplit == 1 ? int(blockIdx.x) * 4 + warp : int(blockIdx.x);
-  if (out_row >= n_rows) return;
-  const int q_heads = int(p.a.q_heads), heads = int(p.kv.heads), batch = int(p.a.batch);
-  const int tok = int(uint32_t(out_row) / uint32_t(q_heads));
-  const int hq = out_row - tok * q_heads;
-  const int b = int(uint32_t(tok) / uint32_t(p.a.new_tokens));
-  const int head = int(uint32_t(hq) / uint32_t(p.group));
-  const int g = hq - head * p.group;
-  // units of all sequences, and of those before b
-  int total = 0, before = 0;
-  bool bad;
-  for (int i = lane; i < batch; i += 32) {
-    const int cost = cost_of(p, true, tokens_of(p, i, &bad));
-    total += cost;
-    before += i < b ? cost : 0;
-  }
-  total = warp_sum(total);
-  before = warp_sum(before);
-  const int prefix = p.a.prefix_blocks > 0 ? tokens_of(p, batch, &bad) : 0;
-  const int pre_first = total;
-  if (p.row_tiles_pre > 0) total += cost_of(p, false, prefix);
-
-  const Cut cut(total, p.ctas);
-  const int nt = tiles_in(tokens_of(p, b, &bad));
-  const int own_row = (tok - b * int(p.a.new_tokens)) * p.group + g;
-  int first = before + (own_row / kRows * heads + head) * (nt + kItemCost) + kItemCost;
-  const Part own = part_of(cut, first, first + nt - 1, kRows, own_row % kRows, p.slots_acc,
-                           p.slots_ml, p.own_acc, p.own_ml, out_row);
-  if (p.a.prefix_blocks == 0 && own.count == 1) return;  // written by walk_kernel
-  const int row = tok * p.group + g;
-  Part pre{};
-  if (p.row_tiles_pre > 0) {
-    const int n = tiles_in(prefix);
-    first = pre_first + (row / kRows * heads + head) * (n + kItemCost) + kItemCost;
-    pre = part_of(cut, first, first + n - 1, kRows, row % kRows, p.slots_acc, p.slots_ml,
-                  p.pre_acc, p.pre_ml, out_row);
-  } else if (p.tensor_ctas > 0) {
-    const int n = (prefix + kPrefixTile - 1) / kPrefixTile;
-    first = (row / kPrefixRows * heads + head) * n;
-    pre = part_of(Cut(n * p.tensor_row_tiles * heads, p.tensor_ctas), first, first + n - 1,
-                  kPrefixRows, row % kPrefixRows, p.tensor_acc, p.tensor_ml, p.pre_acc, p.pre_ml,
-                  out_row);
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  // 32 partials at a time (this warp's of every kSplit): their weights, then
-  // their rows
   float m = -INFINITY, l = 0.f;
   float o[kPer] = {};
   const int n = own.count + pre.count;
-  const int mine = kSplit == 1 ? n : (n - warp + kSplit - 1) / kSplit;
-  for (int i0 = 0; i0 < mine; i0 += 32) {
-    const int i = kSplit == 1 ? i0 + lane : (i0 + lane) * kSplit + warp;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    const float* acc = nullptr;
-    if (i < n) {
-      const bool first = i < own.count;
-      const int64_t at = first ? own.row(i) : pre.row(i - own.count);
-      ml = *reinterpret_cast<const float2*>((first ? own.ml : pre.ml) + at * 2);
-      acc = (first ? own.acc : pre.acc) + at * D;
+  for (int i0 = kSplit == 1 ? 0 : warp; i0 < n; i0 += kAtOnce * kSplit) {
+    float2 ml[kAtOnce];
+    float v[kAtOnce][kPer];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int i = i0 + k * kSplit;
+      ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[k][e] = 0.f;
+      if (i < n) {
+        const bool first = i < own.count;
+        const int64_t at = first ? own.row(i) : pre.row(i - own.count);
+        ml[k] = *reinterpret_cast<const float2*>((first ? own.ml : pre.ml) + at * 2);
+        const float* src = (first ? own.acc : pre.acc) + at * D + lane * kPer;
+        if constexpr (kPer == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src);
+          v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(src);
+          v[k][0] = x.x, v[k][1] = x.y;
+        }
+      }
     }
-    float top = ml.x;
+    float mn = m;
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
-    const float mn = fmaxf(m, top);
+    for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, ml[k].x);
     const float base = mn == -INFINITY ? 0.f : mn;
-    const float w = ex2(ml.x - base), corr = ex2(m - base);
-    float lw = ml.y * w;
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) lw += __shfl_xor_sync(~0u, lw, k);
-    l = l * corr + lw;
+    const float corr = ex2(m - base);
     m = mn;
+    l *= corr;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) o[e] *= corr;
-    const int count = min(32, mine - i0);
-#pragma unroll 8
-    for (int k = 0; k < count; ++k) {
-      const float wk = __shfl_sync(~0u, w, k);
-      const float* src = reinterpret_cast<const float*>(
-          __shfl_sync(~0u, reinterpret_cast<uint64_t>(acc), k)) + lane * kPer;
 #pragma unroll
-      for (int e = 0; e < kPer; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + e);
-        o[e] += v.x * wk;
-        o[e + 1] += v.y * wk;
-      }
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float w = ex2(ml[k].x - base);
+      l += ml[k].y * w;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] += v[k][e] * w;
     }
   }
   if constexpr (kSplit > 1) {
     __shared__ float part[kSplit][D + 2];
+    __syncthreads();  // the row before has been read
 #pragma unroll
     for (int e = 0; e < kPer; ++e) part[warp][lane * kPer + e] = o[e];
     if (lane == 0) {
@@ -794,12 +782,133 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkP
     }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  T* out = reinterpret_cast<T*>(p.a.out) + int64_t(out_row) * D + lane * kPer;
+  T* out = reinterpret_cast<T*>(p.a.out) + out_row * D + lane * kPer;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2)
     *reinterpret_cast<uint32_t*>(out + e) = Ops<T>::pack(o[e] * inv, o[e + 1] * inv);
   if (p.a.lse && lane == 0)
     reinterpret_cast<float*>(p.a.lse)[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Without a prefix: walk_kernel wrote the rows of every item one CTA did alone,
+// so only the items cut between CTAs are left, at most one per boundary.  CTA w
+// finds those its walk share has a part of, and does every count-th row of an
+// item that count CTAs share; it also writes its share of the empty sequences.
+// All that depends on the lengths alone is done before waiting for the walk.
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(128) join_cut_kernel(const __grid_constant__ WalkParams p) {
+  constexpr int kRows = 16 * MT;
+  const int w = blockIdx.x;
+  Lengths lens;
+  const Cut cut = lens.read(p, false);
+  const int heads = int(p.a.q_heads), n_new = int(p.a.new_tokens);
+  for (int b = w; b < p.a.batch; b += gridDim.x) {
+    bool ignore;
+    if (tokens_of(p, b, &ignore) != 0) continue;
+    const int64_t rows = int64_t(n_new) * heads, at = b * rows;
+    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.a.out) + at * D);
+    for (int64_t i = threadIdx.x; i < rows * D / 8; i += blockDim.x) out[i] = make_uint4(0, 0, 0, 0);
+    if (p.a.lse)
+      for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+        reinterpret_cast<float*>(p.a.lse)[at + i] = -INFINITY;
+  }
+  if (w >= cut.ctas) return;
+  const int lo = cut.start(w), hi = cut.start(w + 1);
+  const Item it[2] = {item_at(p, lens, lo), item_at(p, lens, hi - 1)};
+  const int first[2] = {lo - it[0].u + kItemCost, hi - 1 - it[1].u + kItemCost};  // first tiles
+  Part part[2];
+  int from[2], rows[2];  // this CTA's rows of each: from, from + count, ...
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    part[i] = part_of(cut, first[i], first[i] + it[i].nt - 1, kRows, 0, p.slots_acc, p.slots_ml,
+                      p.own_acc, p.own_ml, 0);
+    from[i] = w - cut.owner(first[i]);
+    const int all = min(kRows, p.rows_own - it[i].rt * kRows);
+    const int count = part[i].count;
+    rows[i] = count > 1 && from[i] >= 0 && from[i] < count
+                  ? (max(0, all - from[i]) + count - 1) / count
+                  : 0;
+  }
+  if (first[0] == first[1]) rows[1] = 0;  // one item holds the whole share
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  auto join = [&](int i, int k, bool together) {
+    const int rl = from[i] + k * part[i].count;
+    const Row q = row_of(p, it[i].b, it[i].rt * kRows + rl);
+    Part own = part[i];
+    own.first += rl;
+    own.next += rl;
+    const int64_t out_row = (int64_t(q.b) * n_new + q.j) * heads + it[i].head * p.group + q.g;
+    if (together)
+      join_row<T, D, 4, 10>(p, own, Part{}, out_row);
+    else
+      join_row<T, D, 1, 4>(p, own, Part{}, out_row);
+  };
+  // Rows of many partials (one long sequence) by all four warps, the others by
+  // a warp each.
+  const bool many[2] = {part[0].count > 8, part[1].count > 8};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (many[i])
+      for (int k = 0; k < rows[i]; ++k) join(i, k, true);
+  const int few0 = many[0] ? 0 : rows[0], few1 = many[1] ? 0 : rows[1];
+  for (int k = threadIdx.x >> 5; k < few0 + few1; k += 4)
+    if (k < few0)
+      join(0, k, false);
+    else
+      join(1, k - few0, false);
+}
+
+// With a prefix: kSplit warps per query row join its own part and its prefix
+// part.
+template <typename T, int D, int MT, int kSplit>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkParams p) {
+  constexpr int kRows = 16 * MT;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n_rows = int(p.a.batch * p.a.new_tokens * p.a.q_heads);
+  const int out_row = kSplit == 1 ? int(blockIdx.x) * 4 + warp : int(blockIdx.x);
+  if (out_row >= n_rows) return;
+  const int q_heads = int(p.a.q_heads), heads = int(p.kv.heads), batch = int(p.a.batch);
+  const int tok = int(uint32_t(out_row) / uint32_t(q_heads));
+  const int hq = out_row - tok * q_heads;
+  const int b = int(uint32_t(tok) / uint32_t(p.a.new_tokens));
+  const int head = int(uint32_t(hq) / uint32_t(p.group));
+  const int g = hq - head * p.group;
+  // units of all sequences, and of those before b
+  int total = 0, before = 0;
+  bool bad;
+  for (int i = lane; i < batch; i += 32) {
+    const int cost = cost_of(p, true, tokens_of(p, i, &bad));
+    total += cost;
+    before += i < b ? cost : 0;
+  }
+  total = warp_sum(total);
+  before = warp_sum(before);
+  const int prefix = tokens_of(p, batch, &bad);
+  const int pre_first = total;
+  if (p.row_tiles_pre > 0) total += cost_of(p, false, prefix);
+
+  const Cut cut(total, p.ctas);
+  const int nt = tiles_in(tokens_of(p, b, &bad));
+  const int own_row = (tok - b * int(p.a.new_tokens)) * p.group + g;
+  int first = before + (own_row / kRows * heads + head) * (nt + kItemCost) + kItemCost;
+  const Part own = part_of(cut, first, first + nt - 1, kRows, own_row % kRows, p.slots_acc,
+                           p.slots_ml, p.own_acc, p.own_ml, out_row);
+  const int row = tok * p.group + g;
+  Part pre{};
+  if (p.row_tiles_pre > 0) {
+    const int n = tiles_in(prefix);
+    first = pre_first + (row / kRows * heads + head) * (n + kItemCost) + kItemCost;
+    pre = part_of(cut, first, first + n - 1, kRows, row % kRows, p.slots_acc, p.slots_ml,
+                  p.pre_acc, p.pre_ml, out_row);
+  } else if (p.tensor_ctas > 0) {
+    const int n = (prefix + kPrefixTile - 1) / kPrefixTile;
+    first = (row / kPrefixRows * heads + head) * (n + kPrefixUnitCost) + kPrefixUnitCost;
+    pre = part_of(Cut(prefix_units(n, p.tensor_row_tiles * heads), p.tensor_ctas), first,
+                  first + n - 1, kPrefixRows, row % kPrefixRows, p.tensor_acc, p.tensor_ml,
+                  p.pre_acc, p.pre_ml, out_row);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  join_row<T, D, kSplit, 4>(p, own, pre, out_row);
 }
 
 // Launches on `s`; `early`: may start while the kernel before it in the stream
@@ -903,11 +1012,16 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
   TS_CUDA_RET(launch_on(walk_kernel<T, D, MT>, unsigned(p.ctas), kWarps * 32, walk_smem<D>(), s,
                         p.tensor_ctas > 0, p),
               "attention launch");
-  // Few items leave many partials to each row, which then takes four warps.
+  if (p.a.prefix_blocks == 0) {
+    TS_CUDA_RET(launch_on(join_cut_kernel<T, D, MT>, unsigned(p.ctas), 128, 0, s, true, p),
+                "attention join launch");
+    return TS_OK;
+  }
+  // Few units leave many partials to each row, which then takes four warps.
   const int64_t rows = p.a.batch * p.a.new_tokens * p.a.q_heads;
   const int64_t items = p.a.batch * p.row_tiles_own * p.kv.heads +
                         int64_t(p.row_tiles_pre) * p.kv.heads;
-  const bool many = p.ctas >= 8 * items;
+  const bool many = p.ctas >= 8 * items || p.tensor_ctas >= 8 * p.tensor_row_tiles * p.kv.heads;
   TS_CUDA_RET(launch_on(many ? join_kernel<T, D, MT, 4> : join_kernel<T, D, MT, 1>,
                         unsigned(many ? rows : (rows + 3) / 4), 128, 0, s, true, p),
               "attention join launch");

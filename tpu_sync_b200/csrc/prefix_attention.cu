@@ -228,24 +228,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x on the multiply-add pipe, for -126 <= x < 128 (smaller x count as -126,
-// which next to a row's maximum is nothing): x = i + f with |f| <= 1/2, 2^f by
-// the polynomial of degree 4 with the least relative error there (2.6e-6, by
-// Remez exchange), i added to its exponent.
-__device__ __forceinline__ float2 ex2_fma(float2 x) {
-  const float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 t = add2(x, pair(kRound));
-  const float2 i = add2(t, pair(-kRound));
-  const float2 f = fma2(i.x, i.y, pair(-1.f), x);
-  float2 y = fma2(f.x, f.y, pair(0.009570102207362652f), pair(0.05591785907745361f));
-  y = fma2(y.x, y.y, f, pair(0.240247443318367f));
-  y = fma2(y.x, y.y, f, pair(0.6931217908859253f));
-  y = fma2(y.x, y.y, f, pair(0.9999992847442627f));
-  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
-}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -267,12 +249,16 @@ struct Segment {
 struct Shares {
   int lo, hi, nt;
   __device__ __forceinline__ bool next(Segment* s) {
-    if (lo >= hi) return false;
-    s->unit = int(uint32_t(lo) / uint32_t(nt));
-    s->tile = lo - s->unit * nt;
-    s->count = min(hi - lo, nt - s->tile);
-    lo += s->count;
-    return true;
+    while (lo < hi) {
+      s->unit = int(uint32_t(lo) / uint32_t(nt + kPrefixUnitCost));
+      const int from = lo - s->unit * (nt + kPrefixUnitCost);
+      const int to = min(nt + kPrefixUnitCost, from + hi - lo);
+      lo += to - from;
+      s->tile = max(from, kPrefixUnitCost) - kPrefixUnitCost;
+      s->count = to - kPrefixUnitCost - s->tile;
+      if (s->count > 0) return true;
+    }
+    return false;
   }
 };
 
@@ -300,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int heads = int(p.kv.heads);
   Shares shares{};
   shares.nt = (len + kPrefixTile - 1) / kPrefixTile;
-  const Cut cut(shares.nt * p.row_tiles * heads, p.ctas);
+  const Cut cut(prefix_units(shares.nt, p.row_tiles * heads), p.ctas);
   if (bad && blockIdx.x == 0 && threadIdx.x == 0 && p.err)
     *reinterpret_cast<volatile int*>(p.err) = 1;
   if (blockIdx.x >= cut.ctas) return;
@@ -494,37 +480,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = threadIdx.x & 127;       // row of the half
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // this warp's TMEM lanes
     const uint32_t ts = tmem_s + 128 * x + lanes, to = tmem_o + D * x + lanes;
+    // this warp's 32 rows of the queries, and its scratch when they are done with
+    const uint32_t mine = q_smem + (x * 128 + (warp & 3) * 32) * 128;
     uint32_t s_n = 0, o_n = 0;
     bool ok = true;
     while (ok && shares.next(&seg)) {
       const int head = seg.unit % heads, rt = seg.unit / heads;
       const int row0 = rt * kPrefixRows + x * 128;
       if (x == 1 && row0 >= p.rows) continue;
-      // this half's queries into shared memory: 16 bytes a thread, rows swizzled
+      // The queries of this warp's 32 rows into shared memory, swizzled: a lane
+      // places one row, then kC lanes copy a row together.
       {
-        constexpr int kC = D / 8;
-        const int c = r % kC;
+        constexpr int kC = D / 8, kPer = 32 / kC;
+        const int row = row0 + r;
+        int64_t at = -1;
+        if (row < p.rows) {
+          const int tok = int(uint32_t(row) / uint32_t(p.group));
+          const int b = p.a.new_tokens == 1 ? tok : int(uint32_t(tok) / uint32_t(p.a.new_tokens));
+          at = b * p.a.q_batch_stride + (tok - b * p.a.new_tokens) * p.a.q_token_stride +
+               (head * p.group + row - tok * p.group) * p.a.q_head_stride;
+        }
+        const int c = lane % kC;
         int4 v[kC];
 #pragma unroll
         for (int i = 0; i < kC; ++i) {
-          const int row = row0 + i * (128 / kC) + r / kC;
+          const int64_t from = __shfl_sync(~0u, at, i * kPer + lane / kC);
           v[i] = make_int4(0, 0, 0, 0);
-          if (row < p.rows) {
-            const int tok = int(uint32_t(row) / uint32_t(p.group));
-            const int b = p.a.new_tokens == 1 ? tok : int(uint32_t(tok) / uint32_t(p.a.new_tokens));
-            const int jj = tok - b * int(p.a.new_tokens);
-            v[i] = *reinterpret_cast<const int4*>(
-                reinterpret_cast<const T*>(p.a.q) + b * p.a.q_batch_stride +
-                jj * p.a.q_token_stride +
-                (head * p.group + row - tok * p.group) * p.a.q_head_stride + c * 8);
-          }
+          if (from >= 0)
+            v[i] = *reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.a.q) + from + c * 8);
         }
 #pragma unroll
         for (int i = 0; i < kC; ++i) {
-          const int rr = i * (128 / kC) + r / kC;
-          const uint32_t at = q_smem + (c / 8) * kPrefixRows * 128 + (x * 128 + rr) * 128 +
+          const int rr = i * kPer + lane / kC;
+          const uint32_t to = mine + (c / 8) * kPrefixRows * 128 + rr * 128 +
                               (((c % 8) ^ (rr & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x),
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[i].x),
                        "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
                        : "memory");
         }
@@ -554,8 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 4; ++c) tmem_ld32(s + 32 * c, ts + 32 * c);
         tmem_wait_ld();
         const int t0 = (seg.tile + j) * kPrefixTile;
-        const bool masked = hole || t0 + kPrefixTile > len;
-        if (masked) {
+        if (hole || t0 + kPrefixTile > len) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int t = t0 + 32 * c + lane;
@@ -596,20 +585,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float2 scale2 = pair(p.scale_log2), base2 = pair(m == -INFINITY ? 0.f : -m);
         float2 sum[2] = {pair(0.f), pair(0.f)};
-        // 32 keys of the row; the first half of the tile's keys goes to the
-        // tensor cores while the second is worked on
-        auto keys = [&](int c, bool spread) {
+        // the first half of the tile's keys goes to the tensor cores while the
+        // second is worked on
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             float2 e = fma2(__uint_as_float(s[32 * c + 2 * k]),
                             __uint_as_float(s[32 * c + 2 * k + 1]), scale2, base2);
-            if (spread && k % 4 == 3) {
-              e = ex2_fma(e);
-            } else {
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-            }
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
             sum[k % 2] = add2(sum[k % 2], e);
             pk[k] = pack2(e.x, e.y, T{});
           }
@@ -620,16 +606,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) bar_arrive(p_ready + 16 * x + 8 * (c / 2));
           }
-        };
-        // Masked tiles need exact zeros; in the others a quarter of the
-        // exponentials leave the special function unit (16 a cycle and SM, the
-        // scarcest next to the tensor cores) for the multiply-add pipe.
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) keys(c, false);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) keys(c, true);
         }
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
@@ -639,35 +615,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++o_n;
       if (!ok) break;
       fence_after();
-      // the row's partial
+      // The rows' partials: turned in shared memory (the queries' place, which
+      // the products are done with), so that eight lanes write 128 bytes of a row.
       const int row = row0 + r;
-      float *da = nullptr, *dm = nullptr;
+      int64_t to_row = -1;  // first element of this lane's row
+      const bool whole = seg.count == shares.nt;
       if (row < p.rows) {
-        if (seg.count == shares.nt) {
-          const int tok = int(uint32_t(row) / uint32_t(p.group));
-          const int64_t out_row = tok * p.a.q_heads + head * p.group + row - tok * p.group;
-          da = p.whole_acc + out_row * D;
-          dm = p.whole_ml + out_row * 2;
-        } else {
-          const int64_t slot = (int64_t(blockIdx.x) * 2 + (seg.tile == 0 ? 1 : 0)) * kPrefixRows +
-                               x * 128 + r;
-          da = p.slots_acc + slot * D;
-          dm = p.slots_ml + slot * 2;
-        }
-        *reinterpret_cast<float2*>(dm) = make_float2(m, l);
+        const int tok = int(uint32_t(row) / uint32_t(p.group));
+        to_row = whole ? tok * p.a.q_heads + head * p.group + row - tok * p.group
+                       : (int64_t(blockIdx.x) * 2 + (seg.tile == 0 ? 1 : 0)) * kPrefixRows +
+                             x * 128 + r;
+        *reinterpret_cast<float2*>((whole ? p.whole_ml : p.slots_ml) + to_row * 2) =
+            make_float2(m, l);
       }
-#pragma unroll
+      float* acc = whole ? p.whole_acc : p.slots_acc;
+#pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(o, to + 32 * c);
         tmem_wait_ld();
-        if (da) {
+        const uint32_t buf = mine + (c & 1) * (D / 64 - 1) * kPrefixRows * 128;
+        __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            *reinterpret_cast<uint4*>(da + 32 * c + 4 * k) =
-                make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        for (int k = 0; k < 8; ++k)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 +
+                                                                       ((k ^ (lane & 7)) << 4)),
+                       "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
+                       : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = 4 * i + lane / 8, k = lane % 8;
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(buf + rr * 128 + ((k ^ (rr & 7)) << 4))
+                       : "memory");
+          const int64_t dst = __shfl_sync(~0u, to_row, rr);
+          if (dst >= 0) *reinterpret_cast<uint4*>(acc + dst * D + 32 * c + 4 * k) = v;
         }
       }
+      __syncwarp();
       fence_before();
     }
   }

@@ -46,6 +46,13 @@ struct Cut {
   }
 };
 
+// Units of work of the prefix: a unit of nt tiles costs nt + 2 tiles' time, for
+// its queries' way in and its partials' way out.
+constexpr int kPrefixUnitCost = 2;
+__host__ __device__ __forceinline__ int prefix_units(int nt, int units) {
+  return nt > 0 ? (nt + kPrefixUnitCost) * units : 0;
+}
+
 // Whether the kernel takes this page geometry (else the walk over 64-token
 // tiles reads the prefix too).
 bool prefix_geometry_ok(const ts_paged_kv& kv);
