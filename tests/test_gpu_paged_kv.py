@@ -439,13 +439,16 @@ def test_bad_pages_of_a_prefix_with_many_rows(cuda, d, bt, dt):
 
 @pytest.mark.parametrize("prefix", [1, 127, 128, 129, 255, 1023, 20000])
 def test_prefix_lengths_with_many_rows(cuda, prefix):
-  """Tile ends, one key, and more tiles than CTAs; 130 rows and 1040 rows per KV head."""
-  for hq, hk, count in ((13, 1, 10), (26, 1, 40)):
+  """Tile ends, one key, and more tiles than CTAs; 130, 1040 and 5600 rows per KV head,
+  so that one CTA also does many short units after one another."""
+  err = torch.zeros(1, dtype=torch.int32, device="cuda")
+  for hq, hk, count in ((13, 1, 10), (26, 1, 40), (8, 1, 700)):
     lens = [(3 * i) % 7 for i in range(count)]
     pools, table, lens_t, ptable, q, own, shared = build(prefix, BF, hq, hk, 128, 16, True, 1,
                                                          lens, prefix)
     out, lse = ops.shared_prefix_attention(ops.PagedKV(*pools, head_major=True), q, ptable, prefix,
-                                           table, lens_t, return_lse=True)
+                                           table, lens_t, return_lse=True, err_flag=err)
+    assert int(err) == 0
     check(out, lse, q, own, shared, lens, hk, BF)
 
 

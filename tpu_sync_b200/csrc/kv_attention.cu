@@ -26,6 +26,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <numeric>
@@ -470,6 +471,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
       }
     }
     vis_min = __reduce_min_sync(~0u, vis_min);
+    // halves of eight rows that hold any (one for up to eight query heads)
+    const int halves = min(2 * MT, (n_rows - row0 + 7) / 8);
 
     float acc[MT][D / 8][4];
     float m[MT][2], l[MT][2];
@@ -484,16 +487,23 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
 
     for (int tile = cu.tile; tile < cu.end; ++tile) {
       cp_wait<kStages - 2>();
-      __syncwarp();
+      __syncwarp();  // the stage is here, and every lane is done with the one before
       const uint32_t kb = ring + st * stage_bytes<D>();
       const uint32_t vb = kb + kWarpTokens * kRowBytes;
       const uint32_t mask = masks[st];
       const int t0 = tile * kTile + warp * kWarpTokens;
-      float s[MT][2][4];
+      // 16 rows: two accumulators of the scores, for even and odd steps, halve
+      // the chain of products (32 rows are two chains anyway)
+      constexpr int kChains = MT == 1 ? 2 : 1;
+      float s[kChains][MT][2][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int c = 0; c < kChains; ++c)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[mt][i][0] = s[mt][i][1] = s[mt][i][2] = s[mt][i][3] = 0.f;
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[c][mt][i][e] = 0.f;
       // S = Q K^T: lane addresses rows (tokens) 0-7 / 8-15 and the two halves of 16 elements
       {
         const int r = (lane & 7) + ((lane >> 4) << 3);
@@ -504,10 +514,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
           ldsm4(b, kb + r * kRowBytes + (((2 * ks + hb) ^ (r & 7)) << 4));
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            Ops<T>::mma(s[mt][0], qf[mt][ks], b[0], b[1]);
-            Ops<T>::mma(s[mt][1], qf[mt][ks], b[2], b[3]);
+            Ops<T>::mma(s[ks % kChains][mt][0], qf[mt][ks], b[0], b[1]);
+            Ops<T>::mma(s[ks % kChains][mt][1], qf[mt][ks], b[2], b[3]);
           }
         }
+      }
+      // The stage read in the round before is free: its refill runs under the
+      // products.
+      {
+        const int fill = st + kStages - 1;
+        load(fill >= kStages ? fill - kStages : fill);
       }
       const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
       uint32_t pf[MT][4];
@@ -515,10 +531,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          float x[4] = {s[mt][0][2 * hf], s[mt][0][2 * hf + 1], s[mt][1][2 * hf],
-                        s[mt][1][2 * hf + 1]};
+          pf[mt][hf] = pf[mt][hf + 2] = 0;
+          if (2 * mt + hf >= halves) continue;
+          float x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] *= p.scale_log2;
+          for (int i = 0; i < 4; ++i) {
+            x[i] = s[0][mt][i / 2][2 * hf + i % 2];
+            if (kChains > 1) x[i] += s[kChains - 1][mt][i / 2][2 * hf + i % 2];
+            x[i] *= p.scale_log2;
+          }
           if (!whole) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -565,9 +586,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
           }
         }
       }
-      __syncwarp();  // every lane has read the stage before it is filled again
-      int fill = st + kStages - 1;
-      load(fill >= kStages ? fill - kStages : fill);
       if (++st == kStages) st = 0;
     }
 
@@ -587,6 +605,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
         if (warp >= step && warp < 2 * step) {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
+            if (2 * mt + hf >= halves) break;
             float* row = buf + (hf * 8 + g) * (D + 4);
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
@@ -599,6 +618,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
         if (warp < step) {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
+            if (2 * mt + hf >= halves) break;
             const float* row = buf + (hf * 8 + g) * (D + 4);
             const float2 ml = *reinterpret_cast<const float2*>(row + D);
             const float mn = fmaxf(m[mt][hf], ml.x);
@@ -720,24 +740,28 @@ __device__ __forceinline__ void join_row(const WalkParams& p, const Part& own, c
     float v[kAtOnce][kPer];
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      const int i = i0 + k * kSplit;
-      ml[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) v[k][e] = 0.f;
-      if (i < n) {
-        const bool first = i < own.count;
-        const int64_t at = first ? own.row(i) : pre.row(i - own.count);
-        ml[k] = *reinterpret_cast<const float2*>((first ? own.ml : pre.ml) + at * 2);
-        const float* src = (first ? own.acc : pre.acc) + at * D + lane * kPer;
-        if constexpr (kPer == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src);
-          v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(src);
-          v[k][0] = x.x, v[k][1] = x.y;
-        }
+      // past the last one: that one again, with no weight (a load under a
+      // condition of its own would wait for the one before)
+      const int i = min(i0 + k * kSplit, n - 1);
+      const bool first = i < own.count;
+      const int64_t at = first ? own.row(i) : pre.row(i - own.count);
+      ml[k] = *reinterpret_cast<const float2*>((first ? own.ml : pre.ml) + at * 2);
+      const float* src = (first ? own.acc : pre.acc) + at * D + lane * kPer;
+      if constexpr (kPer == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        v[k][0] = x.x, v[k][1] = x.y;
       }
     }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (i0 + k * kSplit >= n) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[k][e] = 0.f;
+      }
     float mn = m;
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, ml[k].x);
@@ -908,7 +932,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkP
                   p.pre_acc, p.pre_ml, out_row);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  join_row<T, D, kSplit, 4>(p, own, pre, out_row);
+  join_row<T, D, kSplit, 8>(p, own, pre, out_row);
 }
 
 // Launches on `s`; `early`: may start while the kernel before it in the stream
@@ -959,6 +983,18 @@ int check_attention(const ts_paged_kv* kv, const ts_attention_args* args) {
   if (!(a.scale > 0.f) || !std::isfinite(a.scale))
     return set_error(TS_INVALID_ARGUMENT, "scale must be finite and positive");
   return TS_OK;
+}
+
+// CTAs of the prefix kernel: at least kPrefixShare units of work for each (by
+// the length the host knows), so that what every CTA pays once (about 7 us:
+// queries in, partials out) is not most of its time; the SMs left over run the
+// walk meanwhile.
+constexpr int kPrefixShare = 6;
+int prefix_ctas(const ts_paged_kv& kv, const ts_attention_args& a, int64_t row_tiles, int device) {
+  const int64_t len = std::min<int64_t>(a.prefix_len, a.prefix_blocks * kv.block_tokens);
+  const int64_t nt = (len + kPrefixTile - 1) / kPrefixTile;
+  const int64_t units = (nt + kPrefixUnitCost) * row_tiles * kv.heads;
+  return int(std::max<int64_t>(1, std::min<int64_t>(sm_count(device), units / kPrefixShare)));
 }
 
 struct Layout {
@@ -1021,7 +1057,7 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
   const int64_t rows = p.a.batch * p.a.new_tokens * p.a.q_heads;
   const int64_t items = p.a.batch * p.row_tiles_own * p.kv.heads +
                         int64_t(p.row_tiles_pre) * p.kv.heads;
-  const bool many = p.ctas >= 8 * items || p.tensor_ctas >= 8 * p.tensor_row_tiles * p.kv.heads;
+  const bool many = p.ctas >= 4 * items || p.tensor_ctas >= 24 * p.tensor_row_tiles * p.kv.heads;
   TS_CUDA_RET(launch_on(many ? join_kernel<T, D, MT, 4> : join_kernel<T, D, MT, 1>,
                         unsigned(many ? rows : (rows + 3) / 4), 128, 0, s, true, p),
               "attention join launch");
@@ -1113,7 +1149,7 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
     t.rows = p.rows_pre;
     t.row_tiles = (p.rows_pre + tsb::kPrefixRows - 1) / tsb::kPrefixRows;
     t.piece = int(std::gcd(kv->block_tokens, int64_t(tsb::kPrefixTile)));
-    t.ctas = tsb::sm_count(device);
+    t.ctas = tsb::prefix_ctas(*kv, a, t.row_tiles, device);
     t.slots_acc = reinterpret_cast<float*>(base + w.tensor_acc);
     t.slots_ml = reinterpret_cast<float*>(base + w.tensor_ml);
     t.whole_acc = p.pre_acc;

@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int pieces = kPrefixTile / p.piece;
       const CUtensorMap* map = warp == 8 ? &kmap : &vmap;
       uint32_t n = warp == 8 ? 0 : 1;  // ring position: K and V tiles alternate
+      uint32_t cuts = 0;
       bool ok = true;
       while (ok && shares.next(&seg)) {
         const int head = seg.unit % heads;
@@ -364,7 +365,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = bar_wait(empty + 8 * (g % S::kStages), (g / S::kStages) & 1, gone);
             if (!ok) break;
           }
-          if (elect()) bar_expect(full + 8 * st, S::kTileBytes);
+          // A V tile that ends past the length goes through a barrier of its own:
+          // whatever its page holds there must not meet a weight of 0, so it is
+          // handed on when those rows are zeroed.
+          const int past = len - (seg.tile + j) * kPrefixTile;  // keys of this tile that count
+          const bool cut = warp == 10 && past < kPrefixTile;
+          const uint32_t bar = cut ? v_cut : full + 8 * st;
+          if (elect()) bar_expect(bar, S::kTileBytes);
           __syncwarp();
           const uint32_t dst = ring + st * S::kTileBytes;
           for (int i = 0; i < pieces; ++i) {
@@ -372,17 +379,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (elect()) {
 #pragma unroll
               for (int h = 0; h < D / 64; ++h)
-                tma_4d(dst + i * p.piece * 128 + h * kPrefixTile * 128, map, full + 8 * st, h * 64,
+                tma_4d(dst + i * p.piece * 128 + h * kPrefixTile * 128, map, bar, h * 64,
                        of, head, pg);
             }
             __syncwarp();
           }
           page = next;
           off = next_off;
-          const int past = len - (seg.tile + j) * kPrefixTile;  // keys of this tile that count
-          if (warp == 10 && past < kPrefixTile) {
-            // V rows past the length: whatever the page holds must not meet a weight of 0
-            ok = bar_wait(full + 8 * st, (n / S::kStages) & 1, gone);
+          if (cut) {
+            ok = bar_wait(v_cut, cuts & 1, gone);
+            ++cuts;
             if (!ok) break;
             for (int i = lane; i < (kPrefixTile - past) * (D / 64) * 8; i += 32) {
               const int r = past + i / (D / 64 * 8), c = i % (D / 64 * 8);
@@ -391,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) bar_arrive(v_cut);
+            if (lane == 0) bar_arrive(full + 8 * st);
           }
         }
       }
@@ -404,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      v_desc = smem_desc(ring, kPrefixTile * 128);
       uint32_t n = 0;                   // ring position: K0 V0 K1 V1 ...
       uint32_t st = 0, st_phase = 0;    // n % kStages, n / kStages
-      uint32_t q_n[2] = {0, 0}, p_n[2] = {0, 0}, cuts = 0;
+      uint32_t q_n[2] = {0, 0}, p_n[2] = {0, 0};
       bool ok = true;
       auto advance = [&] {
         ++n;
@@ -440,10 +446,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; ok && j < seg.count; ++j) {
           const uint64_t vb = v_desc + st * (S::kTileBytes / 16);
           ok = bar_wait_one(full + 8 * st, st_phase & 1, gone);
-          if (len - (seg.tile + j) * kPrefixTile < kPrefixTile) {
-            ok = ok && bar_wait_one(v_cut, cuts & 1, gone);
-            ++cuts;
-          }
           advance();  // to the next K tile (or the next segment's)
           const bool more = j + 1 < seg.count;
           for (int x = 0; ok && x < halves; ++x) {
@@ -504,14 +506,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         int4 v[kC];
 #pragma unroll
         for (int i = 0; i < kC; ++i) {
+          // rows past the last one read the batch's first row: a load under a
+          // condition of its own would wait for the one before
           const int64_t from = __shfl_sync(~0u, at, i * kPer + lane / kC);
-          v[i] = make_int4(0, 0, 0, 0);
-          if (from >= 0)
-            v[i] = *reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.a.q) + from + c * 8);
+          v[i] = *reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.a.q) +
+                                                (from < 0 ? 0 : from) + c * 8);
         }
 #pragma unroll
         for (int i = 0; i < kC; ++i) {
           const int rr = i * kPer + lane / kC;
+          if (row0 + (warp & 3) * 32 + rr >= p.rows) v[i] = make_int4(0, 0, 0, 0);
           const uint32_t to = mine + (c / 8) * kPrefixRows * 128 + rr * 128 +
                               (((c % 8) ^ (rr & 7)) << 4);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[i].x),
