@@ -883,56 +883,62 @@ __global__ void __launch_bounds__(128) join_cut_kernel(const __grid_constant__ W
 }
 
 // With a prefix: kSplit warps per query row join its own part and its prefix
-// part.
+// part, row after row.  The grid is what fits on the SMs at once: a CTA that
+// starts late pays its way to the first row (about 5 us) on top.
+constexpr int kJoinCtas = 5;
 template <typename T, int D, int MT, int kSplit>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ WalkParams p) {
+__global__ void __launch_bounds__(128, kJoinCtas) join_kernel(const __grid_constant__ WalkParams p) {
   constexpr int kRows = 16 * MT;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n_rows = int(p.a.batch * p.a.new_tokens * p.a.q_heads);
-  const int out_row = kSplit == 1 ? int(blockIdx.x) * 4 + warp : int(blockIdx.x);
-  if (out_row >= n_rows) return;
   const int q_heads = int(p.a.q_heads), heads = int(p.kv.heads), batch = int(p.a.batch);
-  const int tok = int(uint32_t(out_row) / uint32_t(q_heads));
-  const int hq = out_row - tok * q_heads;
-  const int b = int(uint32_t(tok) / uint32_t(p.a.new_tokens));
-  const int head = int(uint32_t(hq) / uint32_t(p.group));
-  const int g = hq - head * p.group;
-  // units of all sequences, and of those before b
-  int total = 0, before = 0;
+  Lengths lens;
+  const Cut cut = lens.read(p, false);
   bool bad;
-  for (int i = lane; i < batch; i += 32) {
-    const int cost = cost_of(p, true, tokens_of(p, i, &bad));
-    total += cost;
-    before += i < b ? cost : 0;
-  }
-  total = warp_sum(total);
-  before = warp_sum(before);
   const int prefix = tokens_of(p, batch, &bad);
-  const int pre_first = total;
-  if (p.row_tiles_pre > 0) total += cost_of(p, false, prefix);
-
-  const Cut cut(total, p.ctas);
-  const int nt = tiles_in(tokens_of(p, b, &bad));
-  const int own_row = (tok - b * int(p.a.new_tokens)) * p.group + g;
-  int first = before + (own_row / kRows * heads + head) * (nt + kItemCost) + kItemCost;
-  const Part own = part_of(cut, first, first + nt - 1, kRows, own_row % kRows, p.slots_acc,
-                           p.slots_ml, p.own_acc, p.own_ml, out_row);
-  const int row = tok * p.group + g;
-  Part pre{};
-  if (p.row_tiles_pre > 0) {
-    const int n = tiles_in(prefix);
-    first = pre_first + (row / kRows * heads + head) * (n + kItemCost) + kItemCost;
-    pre = part_of(cut, first, first + n - 1, kRows, row % kRows, p.slots_acc, p.slots_ml,
-                  p.pre_acc, p.pre_ml, out_row);
-  } else if (p.tensor_ctas > 0) {
-    const int n = (prefix + kPrefixTile - 1) / kPrefixTile;
-    first = (row / kPrefixRows * heads + head) * (n + kPrefixUnitCost) + kPrefixUnitCost;
-    pre = part_of(Cut(prefix_units(n, p.tensor_row_tiles * heads), p.tensor_ctas), first,
-                  first + n - 1, kPrefixRows, row % kPrefixRows, p.tensor_acc, p.tensor_ml,
-                  p.pre_acc, p.pre_ml, out_row);
+  const int pre_nt = p.tensor_ctas > 0 ? (prefix + kPrefixTile - 1) / kPrefixTile : tiles_in(prefix);
+  const Cut pre_cut = p.tensor_ctas > 0
+                          ? Cut(prefix_units(pre_nt, p.tensor_row_tiles * heads), p.tensor_ctas)
+                          : cut;
+  const int step = kSplit == 1 ? int(gridDim.x) * 4 : int(gridDim.x);
+  bool waited = false;
+  for (int out_row = kSplit == 1 ? int(blockIdx.x) * 4 + warp : int(blockIdx.x); out_row < n_rows;
+       out_row += step) {
+    const int tok = int(uint32_t(out_row) / uint32_t(q_heads));
+    const int hq = out_row - tok * q_heads;
+    const int b = int(uint32_t(tok) / uint32_t(p.a.new_tokens));
+    const int head = int(uint32_t(hq) / uint32_t(p.group));
+    const int g = hq - head * p.group;
+    // units of the sequences before b, and of all (where a walked prefix begins)
+    int before = 0, all = 0, len = 0;
+    for (int k = 0; 32 * k < batch; ++k) {
+      const int i = 32 * k + lane, now = lens.get(p, k);
+      const int cost = i < batch ? cost_of(p, true, now) : 0;
+      before += i < b ? cost : 0;
+      all += cost;
+      if (k == b / 32) len = __shfl_sync(~0u, now, b % 32);
+    }
+    before = warp_sum(before);
+    const int nt = tiles_in(len);
+    const int own_row = (tok - b * int(p.a.new_tokens)) * p.group + g;
+    int first = before + (own_row / kRows * heads + head) * (nt + kItemCost) + kItemCost;
+    const Part own = part_of(cut, first, first + nt - 1, kRows, own_row % kRows, p.slots_acc,
+                             p.slots_ml, p.own_acc, p.own_ml, out_row);
+    const int row = tok * p.group + g;
+    Part pre{};
+    if (p.tensor_ctas > 0) {
+      first = (row / kPrefixRows * heads + head) * (pre_nt + kPrefixUnitCost) + kPrefixUnitCost;
+      pre = part_of(pre_cut, first, first + pre_nt - 1, kPrefixRows, row % kPrefixRows,
+                    p.tensor_acc, p.tensor_ml, p.pre_acc, p.pre_ml, out_row);
+    } else if (p.row_tiles_pre > 0) {
+      first = warp_sum(all) + (row / kRows * heads + head) * (pre_nt + kItemCost) + kItemCost;
+      pre = part_of(cut, first, first + pre_nt - 1, kRows, row % kRows, p.slots_acc, p.slots_ml,
+                    p.pre_acc, p.pre_ml, out_row);
+    }
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    waited = true;
+    join_row<T, D, kSplit, 8>(p, own, pre, out_row);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  join_row<T, D, kSplit, 8>(p, own, pre, out_row);
 }
 
 // Launches on `s`; `early`: may start while the kernel before it in the stream
@@ -1059,7 +1065,9 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
                         int64_t(p.row_tiles_pre) * p.kv.heads;
   const bool many = p.ctas >= 4 * items || p.tensor_ctas >= 24 * p.tensor_row_tiles * p.kv.heads;
   TS_CUDA_RET(launch_on(many ? join_kernel<T, D, MT, 4> : join_kernel<T, D, MT, 1>,
-                        unsigned(many ? rows : (rows + 3) / 4), 128, 0, s, true, p),
+                        unsigned(std::min<int64_t>(many ? rows : (rows + 3) / 4,
+                                                   int64_t(sm_count(device)) * kJoinCtas)),
+                        128, 0, s, true, p),
               "attention join launch");
   return TS_OK;
 }
