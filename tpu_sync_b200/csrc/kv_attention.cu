@@ -51,11 +51,11 @@ struct WalkParams {
   float scale_log2;   // scale * log2(e): softmax in powers of two
   int group;          // query heads per KV head
   int rows_own;       // rows of a sequence and KV head: new_tokens * group
-  int row_tiles_own;  // tiles of 16 * MT rows of them
+  int row_tiles_own;  // tiles of 8, 16 or 32 rows of them
   int rows_pre;       // rows of the shared prefix and a KV head: all sequences'
   int row_tiles_pre;  // 0: no prefix in this kernel
-  float* slots_acc;   // [ctas][2][16 * MT][D]: partials of items cut between CTAs
-  float* slots_ml;    // [ctas][2][16 * MT][2]
+  float* slots_acc;   // [ctas][2][rows of a tile][D]: partials of items cut between CTAs
+  float* slots_ml;    // [ctas][2][rows of a tile][2]
   float* own_acc;     // [rows][D]: own parts of a batch that has a prefix
   float* own_ml;      // [rows][2]
   float* pre_acc;     // [rows][D]: whole prefix parts
@@ -334,55 +334,50 @@ __device__ __forceinline__ Row row_of(const WalkParams& p, int seq, int row) {
   return r;
 }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_constant__ WalkParams p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, tg = lane & 3;
-  constexpr int kChunks = D / 8;          // 16-byte pieces of a head vector
-  constexpr int kRowBytes = D * 2;
-  constexpr int kRows = 16 * MT;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
-  float* join = reinterpret_cast<float*>(smem + kWarps * kStages * stage_bytes<D>());
-  uint32_t* masks = reinterpret_cast<uint32_t*>(join + join_floats<D>()) + warp * kStages;
+// A warp's loads: the 16 tokens it owns of each tile of the CTA's share, one
+// ring stage (K, then V) per tile, across items.
+template <typename T, int D>
+struct Loader {
+  static constexpr int kChunks = D / 8;  // 16-byte pieces of a head vector
+  static constexpr int kRowBytes = D * 2;
+  Cursor at;
+  int tile;
+  uint32_t ring;    // of this warp
+  uint32_t* masks;  // tokens of each stage that count, one bit each
+  // table entries [window, window + 32) of sequence window_seq, one a lane
+  int window, entry, window_seq;
 
-  // Lets join_kernel take SMs as they fall free.  With a prefix kernel before
-  // it, this one may itself run early: it reads nothing that kernel writes, and
-  // waits for it before it ends, so that join_kernel's wait covers both.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  Cursor cu = start_cursor(p);
-  Cursor ld = cu;
-  int ld_tile = ld.tile;
-  // table entries [window, window + 32) of the sequence being loaded, one a lane
-  int window = -1, entry = 0, window_seq = -1;
-  const int bt = int(p.kv.block_tokens);
+  __device__ __forceinline__ Loader(const Cursor& c, uint32_t r, uint32_t* m)
+      : at(c), tile(c.tile), ring(r), masks(m), window(-1), entry(0), window_seq(-1) {}
 
-  // Queues the warp's 16 tokens of tile ld_tile into ring stage `st`.
-  auto load = [&](int st) {
-    if (ld.done()) {
+  // Queues the next tile into stage `st` (an empty group past the last one).
+  __device__ __forceinline__ void load(const WalkParams& p, int st) {
+    if (at.done()) {
       cp_commit();
       return;
     }
-    const int t0 = ld_tile * kTile + warp * kWarpTokens;
+    const int bt = int(p.kv.block_tokens);
+    const int t0 = tile * kTile + int(threadIdx.x >> 5) * kWarpTokens;
     const uint32_t kdst = ring + st * stage_bytes<D>();
     const uint32_t vdst = kdst + kWarpTokens * kRowBytes;
+    const int lane = threadIdx.x & 31;
     const int c = lane % kChunks;
     constexpr int kPer = 32 / kChunks;  // tokens a warp's 32 lanes copy at once
     // lanes 0..15 place one token each
     const int t = t0 + (lane & 15);
     const int blk = p.block_shift >= 0 ? t >> p.block_shift : int(uint32_t(t) / uint32_t(bt));
     const int off = t - blk * bt;
-    bool ok = t < ld.len;
+    bool ok = t < at.len;
     const int first = __shfl_sync(~0u, blk, 0);
     // 16 tokens touch at most 16 entries: one window holds them
-    if (ld.b != window_seq || first < window || first + 16 > window + 32) {
+    if (at.b != window_seq || first < window || first + 16 > window + 32) {
       window = first;
-      window_seq = ld.b;
+      window_seq = at.b;
       const int32_t* table =
-          ld.b < p.a.batch
-              ? reinterpret_cast<const int32_t*>(p.a.block_table) + ld.b * p.a.block_table_stride
+          at.b < p.a.batch
+              ? reinterpret_cast<const int32_t*>(p.a.block_table) + at.b * p.a.block_table_stride
               : reinterpret_cast<const int32_t*>(p.a.prefix_table);
-      const int last = p.block_shift >= 0 ? (ld.len - 1) >> p.block_shift : (ld.len - 1) / bt;
+      const int last = p.block_shift >= 0 ? (at.len - 1) >> p.block_shift : (at.len - 1) / bt;
       entry = window + lane <= last ? __ldg(table + window + lane) : 0;
     }
     const int page = __shfl_sync(~0u, entry, blk - window);
@@ -392,8 +387,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
     }
     const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
     if (lane == 0) masks[st] = mask;
-    const T* kp = reinterpret_cast<const T*>(p.kv.k_ptr) + ld.head * p.kv.k_head_stride;
-    const T* vp = reinterpret_cast<const T*>(p.kv.v_ptr) + ld.head * p.kv.v_head_stride;
+    const T* kp = reinterpret_cast<const T*>(p.kv.k_ptr) + at.head * p.kv.k_head_stride;
+    const T* vp = reinterpret_cast<const T*>(p.kv.v_ptr) + at.head * p.kv.v_head_stride;
     if (mask == 0xffffu && bt % kWarpTokens == 0) {
       // all in one page: one address, even steps
       const int r0 = lane / kChunks;
@@ -424,14 +419,32 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
       }
     }
     cp_commit();
-    if (++ld_tile == ld.end) {
-      ld.next_item(p);
-      ld_tile = ld.tile;
+    if (++tile == at.end) {
+      at.next_item(p);
+      tile = at.tile;
     }
-  };
+  }
+};
 
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_constant__ WalkParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, tg = lane & 3;
+  constexpr int kRowBytes = D * 2;
+  constexpr int kRows = 16 * MT;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
+  float* join = reinterpret_cast<float*>(smem + kWarps * kStages * stage_bytes<D>());
+  uint32_t* masks = reinterpret_cast<uint32_t*>(join + join_floats<D>()) + warp * kStages;
+
+  // Lets join_kernel take SMs as they fall free.  With a prefix kernel before
+  // it, this one may itself run early: it reads nothing that kernel writes, and
+  // waits for it before it ends, so that join_kernel's wait covers both.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Cursor cu = start_cursor(p);
+  Loader<T, D> loader(cu, ring, masks);
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load(s);
+  for (int s = 0; s < kStages - 1; ++s) loader.load(p, s);
   int st = 0;
 
   while (!cu.done()) {
@@ -523,7 +536,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
       // products.
       {
         const int fill = st + kStages - 1;
-        load(fill >= kStages ? fill - kStages : fill);
+        loader.load(p, fill >= kStages ? fill - kStages : fill);
       }
       const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
       uint32_t pf[MT][4];
@@ -685,6 +698,247 @@ __global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_const
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Up to eight query rows of a KV head (one token of up to eight query heads,
+// the common decode step): the tokens are the rows of the products and the
+// queries their eight columns, S^T = K Q^T and O^T = V^T P^T, so no product
+// works on rows that are not there, and a thread holds half as many sums.
+// S^T's fragments become P^T's operand by a transposing register move.
+template <int D>
+__host__ __device__ constexpr int walk8_smem() {
+  return kWarps * kStages * stage_bytes<D>() + kWarps * kStages * 4;
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWarps * 32, 3)
+    walk8_kernel(const __grid_constant__ WalkParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, tg = lane & 3;
+  constexpr int kRowBytes = D * 2;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
+  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * stage_bytes<D>()) +
+                    warp * kStages;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // as in walk_kernel
+  Cursor cu = start_cursor(p);
+  Loader<T, D> loader(cu, ring, masks);
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) loader.load(p, s);
+  int st = 0;
+
+  // The queries as operand B (this thread: row g), and how many tokens this
+  // thread's two rows see.  Rows past the last one repeat it and are not written.
+  uint32_t qf[D / 16][2];
+  int vis[2], vis_min = 0;
+  auto load_queries = [&](const Cursor& c) {
+    const bool own = c.b < p.a.batch;
+    const int n_rows = own ? p.rows_own : p.rows_pre;
+    vis_min = INT32_MAX;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const Row q = row_of(p, c.b, min(c.rt * 8 + 2 * tg + e, n_rows - 1));
+      vis[e] = own ? c.len - int(p.a.new_tokens) + 1 + q.j : c.len;
+      vis_min = min(vis_min, vis[e]);
+    }
+    vis_min = __reduce_min_sync(~0u, vis_min);
+    const Row q = row_of(p, c.b, min(c.rt * 8 + g, n_rows - 1));
+    const T* src = reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
+                   q.j * p.a.q_token_stride + (c.head * p.group + q.g) * p.a.q_head_stride;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qf[ks][0] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg);
+      qf[ks][1] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg + 8);
+    }
+  };
+  if (!cu.done()) load_queries(cu);
+
+  while (!cu.done()) {
+    const int row0 = cu.rt * 8;
+    const bool own = cu.b < p.a.batch;
+    const int n_rows = own ? p.rows_own : p.rows_pre;
+    // acc[i]: elements 16 i + g and 16 i + g + 8 of rows 2 tg and 2 tg + 1
+    float acc[D / 16][4];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+
+    for (int tile = cu.tile; tile < cu.end; ++tile) {
+      cp_wait<kStages - 2>();
+      __syncwarp();  // the stage is here, and every lane is done with the one before
+      const uint32_t kb = ring + st * stage_bytes<D>();
+      const uint32_t vb = kb + kWarpTokens * kRowBytes;
+      const uint32_t mask = masks[st];
+      const int t0 = tile * kTile + warp * kWarpTokens;
+      // S^T = K Q^T in two accumulators, for even and odd steps
+      float s[2][4] = {};
+      {
+        const int r = lane & 15, hb = lane >> 4;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t a[4];
+          ldsm4(a, kb + r * kRowBytes + (((2 * ks + hb) ^ (r & 7)) << 4));
+          Ops<T>::mma(s[ks & 1], a, qf[ks][0], qf[ks][1]);
+        }
+      }
+      // The stage read in the round before is free: its refill runs under the
+      // products.
+      {
+        const int fill = st + kStages - 1;
+        loader.load(p, fill >= kStages ? fill - kStages : fill);
+      }
+      const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
+      float x[4], corr[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (s[0][i] + s[1][i]) * p.scale_log2;
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = g + (i >> 1) * 8;
+          if (!((mask >> tok) & 1) || t0 + tok >= vis[i & 1]) x[i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(x[e], x[e + 2]);
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
+        const float mn = fmaxf(m[e], mx);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        corr[e] = ex2(m[e] - base);
+        m[e] = mn;
+        x[e] = ex2(x[e] - base);
+        x[e + 2] = ex2(x[e + 2] - base);
+        l[e] = l[e] * corr[e] + x[e] + x[e + 2];
+      }
+      if (__any_sync(~0u, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          acc[i][0] *= corr[0];
+          acc[i][1] *= corr[1];
+          acc[i][2] *= corr[0];
+          acc[i][3] *= corr[1];
+        }
+      }
+      const uint32_t p0 = transpose8(Ops<T>::pack(x[0], x[1]));
+      const uint32_t p1 = transpose8(Ops<T>::pack(x[2], x[3]));
+      // O^T += V^T P^T
+      {
+        const int r = (lane & 7) + ((lane >> 4) << 3), hb = (lane >> 3) & 1;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t a[4];
+          ldsm4_t(a, vb + r * kRowBytes + (((2 * i + hb) ^ (r & 7)) << 4));
+          Ops<T>::mma(acc[i], a, p0, p1);
+        }
+      }
+      if (++st == kStages) st = 0;
+    }
+
+    // The next item's queries are on their way while this one is joined.
+    Cursor next = cu;
+    next.next_item(p);
+    if (!next.done()) load_queries(next);
+
+    // All four warps' parts through shared memory, each in its ring's stage that
+    // was read last and is not refilled before the next item's first tile; then
+    // 16 threads a row.
+    static_assert(8 * (D + 4) * 4 <= stage_bytes<D>(), "a warp's part fits a stage");
+    const int free_st = st == 0 ? kStages - 1 : st - 1;
+    auto part = [&](int w) {
+      return reinterpret_cast<float*>(smem + (w * kStages + free_st) * stage_bytes<D>());
+    };
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int k = 4; k < 32; k <<= 1) l[e] += __shfl_xor_sync(~0u, l[e], k);
+    __syncwarp();  // every lane is done with the stage
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float* row = part(warp) + (2 * tg + e) * (D + 4);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        row[16 * i + g] = acc[i][e];
+        row[16 * i + g + 8] = acc[i][e + 2];
+      }
+      if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[e], l[e]);
+    }
+    __syncthreads();
+    {
+      constexpr int kPer = D / 16;  // elements a thread joins
+      const int rl = threadIdx.x >> 4, at = (threadIdx.x & 15) * kPer;
+      const int row = row0 + rl;
+      if (row < n_rows) {
+        float2 ml[kWarps];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          ml[w] = *reinterpret_cast<const float2*>(part(w) + rl * (D + 4) + D);
+          mx = fmaxf(mx, ml[w].x);
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float o[kPer] = {}, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = ex2(ml[w].x - base);
+          sum += ml[w].y * f;
+          const float* src = part(w) + rl * (D + 4) + at;
+#pragma unroll
+          for (int i = 0; i < kPer; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src + i);
+            o[i] += v.x * f;
+            o[i + 1] += v.y * f;
+            o[i + 2] += v.z * f;
+            o[i + 3] += v.w * f;
+          }
+        }
+        const Row q = row_of(p, cu.b, row);
+        const int64_t out_row = (int64_t(q.b) * p.a.new_tokens + q.j) * p.a.q_heads +
+                                cu.head * p.group + q.g;
+        const bool complete = cu.tile == 0 && cu.end == cu.nt;
+        if (complete && own && p.a.prefix_blocks == 0) {
+          // the whole row: the result itself
+          const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+          T* out = reinterpret_cast<T*>(p.a.out) + out_row * D + at;
+#pragma unroll
+          for (int i = 0; i < kPer; i += 4)
+            *reinterpret_cast<uint2*>(out + i) =
+                make_uint2(Ops<T>::pack(o[i] * inv, o[i + 1] * inv),
+                           Ops<T>::pack(o[i + 2] * inv, o[i + 3] * inv));
+          if (p.a.lse && at == 0)
+            reinterpret_cast<float*>(p.a.lse)[out_row] =
+                sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+        } else {
+          float *da, *dm;
+          if (complete) {
+            da = (own ? p.own_acc : p.pre_acc) + out_row * D;
+            dm = (own ? p.own_ml : p.pre_ml) + out_row * 2;
+          } else {
+            const int64_t slot = (int64_t(blockIdx.x) * 2 + (cu.tile == 0 ? 1 : 0)) * 8 + rl;
+            da = p.slots_acc + slot * D;
+            dm = p.slots_ml + slot * 2;
+          }
+#pragma unroll
+          for (int i = 0; i < kPer; i += 4)
+            *reinterpret_cast<float4*>(da + at + i) =
+                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          if (at == 0) *reinterpret_cast<float2*>(dm) = make_float2(mx, sum);
+        }
+      }
+    }
+    __syncthreads();  // the parts have been read: the stages may be refilled
+    cu = next;
+  }
+  cp_wait<0>();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Where one part (own or prefix) of a query row lies: `count` partials, the
 // first at row `first`, the others from row `next` on, `step` rows apart (the
 // slots of consecutive CTAs).
@@ -819,9 +1073,8 @@ __device__ __forceinline__ void join_row(const WalkParams& p, const Part& own, c
 // finds those its walk share has a part of, and does every count-th row of an
 // item that count CTAs share; it also writes its share of the empty sequences.
 // All that depends on the lengths alone is done before waiting for the walk.
-template <typename T, int D, int MT>
+template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(128) join_cut_kernel(const __grid_constant__ WalkParams p) {
-  constexpr int kRows = 16 * MT;
   const int w = blockIdx.x;
   Lengths lens;
   const Cut cut = lens.read(p, false);
@@ -886,9 +1139,8 @@ __global__ void __launch_bounds__(128) join_cut_kernel(const __grid_constant__ W
 // part, row after row.  The grid is what fits on the SMs at once: a CTA that
 // starts late pays its way to the first row (about 5 us) on top.
 constexpr int kJoinCtas = 5;
-template <typename T, int D, int MT, int kSplit>
+template <typename T, int D, int kRows, int kSplit>
 __global__ void __launch_bounds__(128, kJoinCtas) join_kernel(const __grid_constant__ WalkParams p) {
-  constexpr int kRows = 16 * MT;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n_rows = int(p.a.batch * p.a.new_tokens * p.a.q_heads);
   const int q_heads = int(p.a.q_heads), heads = int(p.kv.heads), batch = int(p.a.batch);
@@ -1004,7 +1256,7 @@ int prefix_ctas(const ts_paged_kv& kv, const ts_attention_args& a, int64_t row_t
 }
 
 struct Layout {
-  int mt, ctas;
+  int rows, ctas;  // query rows of a tile of the walk, its CTAs
   bool tensor;  // the prefix part goes to the tensor-core kernel
   uint64_t slots_acc, slots_ml, own_acc, own_ml, pre_acc, pre_ml, tensor_acc, tensor_ml, bytes;
 };
@@ -1013,14 +1265,12 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   Layout w{};
   const int64_t group = a.q_heads / kv.heads;
   const int64_t rows = a.batch * a.new_tokens * a.q_heads;
-  // 32-row tiles read K and V half as often once the rows pass one 16-row
-  // tile; below that they only waste registers and matrix work.
+  // The smallest tile that holds a KV head's rows: more than 32 rows are read
+  // for in tiles of 32; a walked prefix counts the rows of the whole batch.
   const bool pre = a.prefix_blocks > 0;
   w.tensor = pre && a.batch * a.new_tokens * group > 32 && prefix_geometry_ok(kv);
-  w.mt = a.new_tokens * group > 16 ||
-                 (pre && !w.tensor && a.batch * a.new_tokens * group > 16)
-             ? 2
-             : 1;
+  const int64_t most = (pre && !w.tensor ? a.batch : 1) * a.new_tokens * group;
+  w.rows = most <= 8 ? 8 : (most <= 16 ? 16 : 32);
   w.ctas = 2 * sm_count(device);
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
@@ -1028,7 +1278,7 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
     at += (n * 4 + 255) / 256 * 256;
     return o;
   };
-  const uint64_t slot_rows = uint64_t(w.ctas) * 2 * 16 * w.mt;
+  const uint64_t slot_rows = uint64_t(w.ctas) * 2 * w.rows;
   w.slots_acc = take(slot_rows * kv.head_dim);
   w.slots_ml = take(slot_rows * 2);
   w.own_acc = take(pre ? rows * kv.head_dim : 0);
@@ -1042,20 +1292,34 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   return w;
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int kRows>
 int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
+  void (*walk)(WalkParams);
+  size_t smem;
+  if constexpr (kRows == 8) {
+    walk = walk8_kernel<T, D>;
+    smem = walk8_smem<D>();
+  } else {
+    walk = walk_kernel<T, D, kRows / 16>;
+    smem = walk_smem<D>();
+  }
   static bool ready[64] = {};
   if (device < 0 || device >= 64 || !ready[device]) {
-    TS_CUDA_RET(cudaFuncSetAttribute(walk_kernel<T, D, MT>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, walk_smem<D>()),
+    TS_CUDA_RET(cudaFuncSetAttribute(reinterpret_cast<const void*>(walk),
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
+                "attention shared memory");
+    // room beside two CTAs for one of the join that follows: its way to the
+    // partials then runs under the walk
+    TS_CUDA_RET(cudaFuncSetAttribute(reinterpret_cast<const void*>(walk),
+                                     cudaFuncAttributePreferredSharedMemoryCarveout,
+                                     cudaSharedmemCarveoutMaxShared),
                 "attention shared memory");
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  TS_CUDA_RET(launch_on(walk_kernel<T, D, MT>, unsigned(p.ctas), kWarps * 32, walk_smem<D>(), s,
-                        p.tensor_ctas > 0, p),
+  TS_CUDA_RET(launch_on(walk, unsigned(p.ctas), kWarps * 32, smem, s, p.tensor_ctas > 0, p),
               "attention launch");
   if (p.a.prefix_blocks == 0) {
-    TS_CUDA_RET(launch_on(join_cut_kernel<T, D, MT>, unsigned(p.ctas), 128, 0, s, true, p),
+    TS_CUDA_RET(launch_on(join_cut_kernel<T, D, kRows>, unsigned(p.ctas), 128, 0, s, true, p),
                 "attention join launch");
     return TS_OK;
   }
@@ -1064,7 +1328,7 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
   const int64_t items = p.a.batch * p.row_tiles_own * p.kv.heads +
                         int64_t(p.row_tiles_pre) * p.kv.heads;
   const bool many = p.ctas >= 4 * items || p.tensor_ctas >= 24 * p.tensor_row_tiles * p.kv.heads;
-  TS_CUDA_RET(launch_on(many ? join_kernel<T, D, MT, 4> : join_kernel<T, D, MT, 1>,
+  TS_CUDA_RET(launch_on(many ? join_kernel<T, D, kRows, 4> : join_kernel<T, D, kRows, 1>,
                         unsigned(std::min<int64_t>(many ? rows : (rows + 3) / 4,
                                                    int64_t(sm_count(device)) * kJoinCtas)),
                         128, 0, s, true, p),
@@ -1072,13 +1336,16 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
   return TS_OK;
 }
 
+template <typename T, int D>
+int launch_rows(const WalkParams& p, int rows, int device, cudaStream_t s) {
+  return rows == 8    ? launch_attention<T, D, 8>(p, device, s)
+         : rows == 16 ? launch_attention<T, D, 16>(p, device, s)
+                      : launch_attention<T, D, 32>(p, device, s);
+}
 template <typename T>
-int launch_attention(const WalkParams& p, int mt, int device, cudaStream_t s) {
-  if (p.kv.head_dim == 64)
-    return mt == 1 ? launch_attention<T, 64, 1>(p, device, s)
-                   : launch_attention<T, 64, 2>(p, device, s);
-  return mt == 1 ? launch_attention<T, 128, 1>(p, device, s)
-                 : launch_attention<T, 128, 2>(p, device, s);
+int launch_rows(const WalkParams& p, int rows, int device, cudaStream_t s) {
+  return p.kv.head_dim == 64 ? launch_rows<T, 64>(p, rows, device, s)
+                             : launch_rows<T, 128>(p, rows, device, s);
 }
 
 }  // namespace
@@ -1131,9 +1398,9 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
   p.scale_log2 = a.scale * tsb::kLog2e;
   p.group = int(a.q_heads / kv->heads);
   p.rows_own = int(a.new_tokens) * p.group;
-  p.row_tiles_own = (p.rows_own + 16 * w.mt - 1) / (16 * w.mt);
+  p.row_tiles_own = (p.rows_own + w.rows - 1) / w.rows;
   p.rows_pre = int(a.batch) * p.rows_own;
-  p.row_tiles_pre = a.prefix_blocks > 0 && !w.tensor ? (p.rows_pre + 16 * w.mt - 1) / (16 * w.mt)
+  p.row_tiles_pre = a.prefix_blocks > 0 && !w.tensor ? (p.rows_pre + w.rows - 1) / w.rows
                                                      : 0;
   uint8_t* base = static_cast<uint8_t*>(workspace);
   p.slots_acc = reinterpret_cast<float*>(base + w.slots_acc);
@@ -1170,6 +1437,6 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
     if (int rc = tsb::launch_prefix(t, device, s)) return rc;
   }
   return kv->dtype == TS_DTYPE_BF16
-             ? tsb::launch_attention<__nv_bfloat16>(p, w.mt, device, s)
-             : tsb::launch_attention<__half>(p, w.mt, device, s);
+             ? tsb::launch_rows<__nv_bfloat16>(p, w.rows, device, s)
+             : tsb::launch_rows<__half>(p, w.rows, device, s);
 }
