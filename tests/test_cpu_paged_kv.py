@@ -148,6 +148,16 @@ def test_attention_workspace_and_head_dim():
   assert attend(kv(), attention_args(new_tokens=0, q=0)) == _native.OK
 
 
+def test_packed_arguments_have_the_structures_layout():
+  assert ops._APPEND_ARGS.size == ctypes.sizeof(_native.KvAppendArgs)
+  assert ops._ATTENTION_ARGS.size == ctypes.sizeof(_native.AttentionArgs)
+  for packer, cls in ((ops._APPEND_ARGS, _native.KvAppendArgs),
+                      (ops._ATTENTION_ARGS, _native.AttentionArgs)):
+    values = list(range(3, 3 + len(cls._fields_)))
+    got = cls.from_buffer_copy(packer.pack(*values))
+    assert [getattr(got, name) for name, _ in cls._fields_] == values
+
+
 def test_wrappers_need_cuda_tensors():
   t = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
   with pytest.raises(ValueError, match="CUDA"):

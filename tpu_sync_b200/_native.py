@@ -330,13 +330,10 @@ _SIGS = {
     "ts_ipc_open": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.POINTER(_V)]),
     "ts_ipc_close": (ctypes.c_int, [ctypes.c_int, _V]),
     "ts_ipc_export": (ctypes.c_int, [_V, ctypes.c_char_p, c_u64_p]),
-    "ts_kv_append": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(PagedKvC),
-                                    ctypes.POINTER(KvAppendArgs), _V, _V]),
-    "ts_paged_attention_workspace": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(PagedKvC),
-                                                    ctypes.POINTER(AttentionArgs), c_u64_p]),
-    "ts_paged_attention": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(PagedKvC),
-                                          ctypes.POINTER(AttentionArgs), _V, ctypes.c_uint64,
-                                          _V, _V]),
+    # the argument structures by address: a byref() or packed bytes
+    "ts_kv_append": (ctypes.c_int, [ctypes.c_int, _V, _V, _V, _V]),
+    "ts_paged_attention_workspace": (ctypes.c_int, [ctypes.c_int, _V, _V, c_u64_p]),
+    "ts_paged_attention": (ctypes.c_int, [ctypes.c_int, _V, _V, _V, ctypes.c_uint64, _V, _V]),
     "ts_kv_relayout": (ctypes.c_int, [ctypes.c_int, _V, _V, ctypes.c_int,
                                       PageGeometry, PageGeometry, _V, ctypes.c_int64,
                                       _V, ctypes.c_int64, ctypes.c_int64,

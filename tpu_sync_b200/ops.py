@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 from typing import List, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -446,34 +447,37 @@ class PagedKV:
     self._workspace = {}  # bytes of attention workspace by shapes
 
 
-def _heads(kv: PagedKV, name: str, t: torch.Tensor, shape: Tuple[int, ...]) -> Tuple[int, ...]:
-  """Strides of a tensor of heads of this shape, checked."""
-  strides = t.stride()
-  if (t.shape == shape and t.dtype is kv.dtype and t.get_device() == kv._index and
-      (strides[-1] == 1 or shape[-1] <= 1) and not (t.requires_grad and torch.is_grad_enabled())):
-    return strides
+# The argument structures as bytes (one pack is cheaper than filling a ctypes
+# structure field by field): ts_kv_append_args, ts_attention_args.
+_APPEND_ARGS = struct.Struct("=22qifii")
+_ATTENTION_ARGS = struct.Struct("=17qfi")
+
+
+def _check_heads(kv: PagedKV, name: str, t: torch.Tensor, shape: Tuple[int, ...]) -> None:
+  """Raises what is wrong with a tensor of heads."""
   if t.shape != shape:
     raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
   if t.dtype != kv.dtype or t.device != kv.device:
     raise ValueError(f"{name} must have the pages' dtype and device")
-  if t.requires_grad and torch.is_grad_enabled():
-    raise ValueError(f"{name} requires grad: the paged cache operators have no backward pass")
-  raise ValueError(f"the last dimension of {name} must be contiguous")
-
-
-def _index(kv: PagedKV, name: str, t: torch.Tensor, dtype: torch.dtype, dims: int,
-           length: Optional[int]) -> Tuple[int, ...]:
-  """Shape of an index tensor, a table or a weight, checked; `length`: of its first dimension."""
-  if not isinstance(t, torch.Tensor):
-    raise ValueError(f"{name} must be a tensor")
-  shape = t.shape
-  if t.dtype is not dtype or len(shape) != dims or t.get_device() != kv._index:
-    raise ValueError(f"{name} must be a {dims}-dimensional {dtype} tensor on {kv.device}")
-  if t.stride()[-1] != 1 and shape[-1] > 1:
+  if t.stride(-1) != 1 and shape[-1] > 1:
     raise ValueError(f"the last dimension of {name} must be contiguous")
-  if length is not None and shape[0] != length:
-    raise ValueError(f"{name} must hold {length} entries, got {list(shape)}")
-  return shape
+
+
+def _check_index(kv: PagedKV, name: str, t: torch.Tensor, dtype: torch.dtype, dims: int,
+                 length: Optional[int]) -> None:
+  """The same for an index tensor, a table or a weight; `length`: of its first dimension."""
+  if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != dims or (
+      t.device != kv.device):
+    raise ValueError(f"{name} must be a {dims}-dimensional {dtype} tensor on {kv.device}")
+  if t.stride(-1) != 1 and t.shape[-1] > 1:
+    raise ValueError(f"the last dimension of {name} must be contiguous")
+  if length is not None and t.shape[0] != length:
+    raise ValueError(f"{name} must hold {length} entries, got {list(t.shape)}")
+
+
+def _check_grad(*tensors: Optional[torch.Tensor]) -> None:
+  if any(t is not None and t.requires_grad for t in tensors):
+    raise ValueError("an input requires grad: the paged cache operators have no backward pass")
 
 
 def _flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
@@ -484,8 +488,7 @@ def _flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
   return err_flag.data_ptr()
 
 
-def _new_like(q: torch.Tensor) -> torch.Tensor:
-  return torch.empty_like(q, memory_format=torch.contiguous_format)
+_HERE = contextlib.nullcontext()
 
 
 def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -514,62 +517,77 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
   cos_sin writes nothing for its token and sets err_flag (int32, on the device)
   to 1.
   """
+  index, dtype, dim = kv._index, kv.dtype, kv.head_dim
   shape = k.shape
-  if len(shape) != 3 or shape[1:] != (kv.heads, kv.head_dim):
-    raise ValueError(f"k must be [tokens, {kv.heads}, {kv.head_dim}], got {list(shape)}")
+  if len(shape) != 3 or shape[1] != kv.heads or shape[2] != dim:
+    raise ValueError(f"k must be [tokens, {kv.heads}, {dim}], got {list(shape)}")
   tokens = shape[0]
-  a = _native.KvAppendArgs()
-  a.k_token_stride, a.k_head_stride, _ = _heads(kv, "k", k, shape)
-  a.v_token_stride, a.v_head_stride, _ = _heads(kv, "v", v, shape)
-  _index(kv, "slots", slots, torch.int64, 1, tokens)
-  a.k, a.v, a.slots, a.tokens = k.data_ptr(), v.data_ptr(), slots.data_ptr(), tokens
+  ks, vs = k.stride(), v.stride()
+  if (k.dtype is not dtype or v.dtype is not dtype or v.shape != shape or
+      k.get_device() != index or v.get_device() != index or ks[2] != 1 or vs[2] != 1):
+    _check_heads(kv, "k", k, shape)
+    _check_heads(kv, "v", v, shape)
+  if (slots.dtype is not torch.int64 or slots.shape != (tokens,) or
+      slots.get_device() != index or slots.stride() != (1,)):
+    _check_index(kv, "slots", slots, torch.int64, 1, tokens)
+  table = places = rows = row_stride = rotary = 0
   if cos_sin is not None:
-    _index(kv, "positions", positions, torch.int64, 1, tokens)
-    rows, rotary = _index(kv, "cos_sin", cos_sin, torch.float32, 2, None)
+    if (not isinstance(positions, torch.Tensor) or positions.dtype is not torch.int64 or
+        positions.shape != (tokens,) or positions.get_device() != index or
+        positions.stride() != (1,)):
+      _check_index(kv, "positions", positions, torch.int64, 1, tokens)
+    _check_index(kv, "cos_sin", cos_sin, torch.float32, 2, None)
+    rows, rotary = cos_sin.shape
     if rows == 0:
       raise ValueError("cos_sin has no rows")
-    a.positions, a.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
-    a.max_position, a.rotary = rows, rotary
-    a.cos_sin_stride = cos_sin.stride(0) if rows > 1 else rotary
-    a.interleaved = bool(interleaved)
+    table, places = cos_sin.data_ptr(), positions.data_ptr()
+    row_stride = cos_sin.stride(0) if rows > 1 else rotary
   elif interleaved or positions is not None:
     raise ValueError("positions and interleaved need cos_sin")
+  wq = wk = weight_dtype = 0
   if q_weight is not None or k_weight is not None:
     w = q_weight if q_weight is not None else k_weight
-    if w.dtype not in (kv.dtype, torch.float32):
+    if w.dtype not in (dtype, torch.float32):
       raise ValueError("norm weights must be float32 or of the pages' dtype")
-    if q_weight is not None and q is None:
-      raise ValueError("q_weight needs q")
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-      if t is None:
-        continue
-      _index(kv, name, t, w.dtype, 1, kv.head_dim)
-      if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires grad: the paged cache operators have no backward pass")
-      setattr(a, name, t.data_ptr())
-    a.weight_dtype = _TORCH_TO_TS[w.dtype]
-    a.eps = eps
+    if q_weight is not None:
+      if q is None:
+        raise ValueError("q_weight needs q")
+      _check_index(kv, "q_weight", q_weight, w.dtype, 1, dim)
+      wq = q_weight.data_ptr()
+    if k_weight is not None:
+      _check_index(kv, "k_weight", k_weight, w.dtype, 1, dim)
+      wk = k_weight.data_ptr()
+    weight_dtype = _TORCH_TO_TS[w.dtype]
+  if torch.is_grad_enabled():
+    _check_grad(k, v, q, q_weight, k_weight, q_out)
+  q_ptr = out_ptr = heads = qt = qh = ot = oh = zero = 0
   if q is not None:
     heads = q.shape[1] if q.dim() == 3 else 0
     if heads == 0:
-      raise ValueError(f"q must be [{tokens}, heads, {kv.head_dim}], got {list(q.shape)}")
-    shape = (tokens, heads, kv.head_dim)
-    a.q_token_stride, a.q_head_stride, _ = _heads(kv, "q", q, shape)
+      raise ValueError(f"q must be [{tokens}, heads, {dim}], got {list(q.shape)}")
+    shape = (tokens, heads, dim)
+    qt, qh, last = q.stride()
+    if (q.shape != shape or q.dtype is not dtype or q.get_device() != index or last != 1):
+      _check_heads(kv, "q", q, shape)
     if q_out is None:
       if stream is None:
-        q_out = _new_like(q)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
       else:
         with torch.cuda.stream(stream):  # what a call allocates belongs to its stream
-          q_out = _new_like(q)
-      a.q_out_token_stride, a.q_out_head_stride = heads * kv.head_dim, kv.head_dim
-      a.zero_padding = 1
+          q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+      ot, oh, zero = heads * dim, dim, 1
     else:
-      a.q_out_token_stride, a.q_out_head_stride, _ = _heads(kv, "q_out", q_out, shape)
-    a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), heads
+      _check_heads(kv, "q_out", q_out, shape)
+      ot, oh, _ = q_out.stride()
+    q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
   elif q_out is not None:
     raise ValueError("q_out needs q")
-  rc = _native.lib().ts_kv_append(kv._index, kv._ref, ctypes.byref(a), _flag(kv, err_flag),
-                                  torch._C._cuda_getCurrentRawStream(kv._index)
+  args = _APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), q_ptr, out_ptr, ks[0], ks[1], vs[0], vs[1],
+                           qt, qh, ot, oh, tokens, heads, slots.data_ptr(), places, table, rows,
+                           row_stride, rotary, wq, wk, weight_dtype, eps, bool(interleaved), zero)
+  rc = _native.lib().ts_kv_append(index, kv._ref, args,
+                                  0 if err_flag is None else _flag(kv, err_flag),
+                                  torch._C._cuda_getCurrentRawStream(index)
                                   if stream is None else stream.cuda_stream)
   if rc:
     _native.check(rc, "kv_append: ")
@@ -589,61 +607,71 @@ def _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, ou
                      "head_dim]")
   if dim != kv.head_dim or q_heads == 0:
     raise ValueError(f"q heads must have {kv.head_dim} elements")
-  a = _native.AttentionArgs()
-  strides = _heads(kv, "q", q, shape)
-  blocks = _index(kv, "block_table", block_table, torch.int32, 2, batch)[1]
-  _index(kv, "seq_lens", seq_lens, torch.int32, 1, batch)
-  a.q, a.batch, a.new_tokens, a.q_heads = q.data_ptr(), batch, new, q_heads
-  # a dimension of one element is never stepped over: its stride says nothing
-  a.q_batch_stride = strides[0] if batch > 1 else 0
-  a.q_token_stride = strides[1] if new > 1 else 0
-  a.q_head_stride = strides[-2] if q_heads > 1 else 0
-  a.block_table, a.max_blocks = block_table.data_ptr(), blocks
-  a.block_table_stride = block_table.stride(0) if batch > 1 else 0
-  a.seq_lens = seq_lens.data_ptr()
-  a.scale = dim ** -0.5 if scale is None else scale
-  prefix_blocks = 0
+  index, dtype, device = kv._index, kv.dtype, kv.device
+  strides = q.stride()
+  if q.dtype is not dtype or q.get_device() != index or strides[-1] != 1:
+    _check_heads(kv, "q", q, shape)
+  if (block_table.dtype is not torch.int32 or block_table.dim() != 2 or
+      block_table.get_device() != index or block_table.shape[0] != batch or
+      block_table.stride(1) != 1):
+    _check_index(kv, "block_table", block_table, torch.int32, 2, batch)
+  if (seq_lens.dtype is not torch.int32 or seq_lens.shape != (batch,) or
+      seq_lens.get_device() != index or seq_lens.stride() != (1,)):
+    _check_index(kv, "seq_lens", seq_lens, torch.int32, 1, batch)
+  shared = blocks = length = length_ptr = 0
   if prefix_table is not None:
-    prefix_blocks, = _index(kv, "prefix_table", prefix_table, torch.int32, 1, None)
-    a.prefix_table, a.prefix_blocks = prefix_table.data_ptr(), prefix_blocks
+    _check_index(kv, "prefix_table", prefix_table, torch.int32, 1, None)
+    shared, blocks = prefix_table.data_ptr(), prefix_table.shape[0]
     if isinstance(prefix_len, torch.Tensor):
-      if prefix_len.dtype != torch.int32 or prefix_len.device != kv.device or (
+      if prefix_len.dtype != torch.int32 or prefix_len.device != device or (
           prefix_len.numel() != 1):
         raise ValueError("prefix_len must be an int or one int32 on the pages' device")
-      a.prefix_len_dev, a.prefix_len = prefix_len.data_ptr(), 2**31 - 1
+      length_ptr, length = prefix_len.data_ptr(), 2**31 - 1
     else:
-      if not 0 <= prefix_len <= prefix_blocks * kv.block_tokens:
+      length = prefix_len
+      if not 0 <= length <= blocks * kv.block_tokens:
         raise ValueError(f"prefix_table does not hold {prefix_len} tokens")
-      a.prefix_len = prefix_len
   if out is not None:
-    _heads(kv, "out", out, shape)
+    _check_heads(kv, "out", out, shape)
     if not out.is_contiguous():
       raise ValueError("out must be contiguous")
+  if torch.is_grad_enabled():
+    _check_grad(q, out)
   lib = _native.lib()
+
+  def pack(out_ptr, lse_ptr):
+    # a dimension of one element is never stepped over: its stride says nothing
+    return _ATTENTION_ARGS.pack(
+        q.data_ptr(), out_ptr, lse_ptr, strides[0] if batch > 1 else 0,
+        strides[1] if new > 1 else 0, strides[-2] if q_heads > 1 else 0, batch, new, q_heads,
+        block_table.data_ptr(), block_table.stride(0) if batch > 1 else 0, block_table.shape[1],
+        seq_lens.data_ptr(), shared, blocks, length, length_ptr,
+        dim ** -0.5 if scale is None else scale, 0)
+
   # the workspace's size follows from the shapes alone
-  key = (batch, new, q_heads, prefix_blocks > 0)
+  key = (batch, new, q_heads, blocks > 0)
   nbytes = kv._workspace.get(key)
   if nbytes is None:
     n = ctypes.c_uint64()
-    _native.check(lib.ts_paged_attention_workspace(kv._index, kv._ref, ctypes.byref(a),
-                                                   ctypes.byref(n)), "attention: ")
+    _native.check(lib.ts_paged_attention_workspace(index, kv._ref, pack(0, 0), ctypes.byref(n)),
+                  "attention: ")
     nbytes = n.value
     if len(kv._workspace) >= 1024:
       kv._workspace.clear()
     kv._workspace[key] = nbytes
   lse = None
   # what a call allocates belongs to its stream
-  with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+  with _HERE if stream is None else torch.cuda.stream(stream):
     if out is None:
-      out = _new_like(q)
+      out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if return_lse:
       lse = q.new_empty(shape[:-1], dtype=torch.float32)
-      a.lse = lse.data_ptr()
-    work = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
-  a.out = out.data_ptr()
-  rc = lib.ts_paged_attention(kv._index, kv._ref, ctypes.byref(a), work.data_ptr(), nbytes,
-                              _flag(kv, err_flag),
-                              torch._C._cuda_getCurrentRawStream(kv._index)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+  rc = lib.ts_paged_attention(index, kv._ref,
+                              pack(out.data_ptr(), lse.data_ptr() if return_lse else 0),
+                              work.data_ptr(), nbytes,
+                              0 if err_flag is None else _flag(kv, err_flag),
+                              torch._C._cuda_getCurrentRawStream(index)
                               if stream is None else stream.cuda_stream)
   if rc:
     _native.check(rc, "attention: ")
