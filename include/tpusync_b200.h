@@ -744,8 +744,10 @@ TS_API int ts_paged_attention_workspace(int device, const ts_paged_kv* kv,
  * values are held in 32 bits, probabilities rounded to the storages' dtype for
  * the matrix products.  Tokens of a table entry outside [0, pages) are left
  * out, lengths are cut to what their table holds, and either sets *err_flag
- * (device or host-mapped int, may be NULL) to 1.  What lies in pages past a
- * length is never used (it may be NaN).  head_dim is 64 or 128. */
+ * (device or host-mapped int, may be NULL) to 1; 2 says that a kernel gave up
+ * waiting for its own loads (its waits are bounded) and the result is not
+ * valid.  What lies in pages past a length is never used (it may be NaN).
+ * head_dim is 64 or 128. */
 TS_API int ts_paged_attention(int device, const ts_paged_kv* kv, const ts_attention_args* args,
                               void* workspace, uint64_t workspace_bytes, int* err_flag,
                               void* stream);

@@ -19,6 +19,9 @@ unused table entries) is NaN or out of range.
 """
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -318,6 +321,11 @@ PREFIX = [
     (8, 2, 128, 128, True, 4, 515, [4 + i for i in range(17)]),
     (8, 2, 128, 256, False, 1, 700, [4 + i for i in range(70)]),
     (32, 8, 128, 16, False, 1, 6000, [17, 33]),
+    # many rows and pages of other than a power of two tokens: loads of 8 and 16 tokens
+    (8, 1, 128, 24, False, 1, 500, [3, 0, 25, 49, 7]),
+    (12, 1, 64, 48, True, 1, 1111, [48, 1, 0, 2, 95, 96, 97]),
+    (10, 1, 128, 136, False, 2, 300, [2, 137, 0, 5, 1]),
+    (40, 1, 128, 20, False, 1, 260, [21, 3]),     # 20 tokens: not in whole groups of 8
 ]
 
 
@@ -536,6 +544,78 @@ def test_other_stream_and_repeatable(cuda):
   assert torch.equal(got, want)
 
 
+def test_calls_from_threads(cuda):
+  """Calls of several threads at once, each on its own stream, give the bits of one alone."""
+  import threading
+  lens = [70, 0, 333]
+  pools, table, lens_t, ptable, q, own, shared = build(16, FP, 16, 2, 64, 16, False, 1, lens, 500)
+  kv = ops.PagedKV(*pools)
+  want = ops.shared_prefix_attention(kv, q, ptable, 500, table, lens_t)
+  alone = ops.paged_attention(kv, q, table, lens_t)
+  torch.cuda.synchronize()
+  bad = []
+
+  def work():
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+      for _ in range(30):
+        a = ops.shared_prefix_attention(kv, q, ptable, 500, table, lens_t)
+        b = ops.paged_attention(kv, q, table, lens_t)
+        stream.synchronize()
+        if not (torch.equal(a, want) and torch.equal(b, alone)):
+          bad.append(1)
+
+  threads = [threading.Thread(target=work) for _ in range(4)]
+  for t in threads:
+    t.start()
+  for t in threads:
+    t.join()
+  assert not bad
+
+
+def test_first_call_is_captured(cuda):
+  """A process whose first call of each operator happens while its stream is captured."""
+  code = """
+import torch
+from tpu_sync_b200 import ops
+g = torch.Generator(device="cuda").manual_seed(1)
+pages = torch.randn(40, 16, 2, 64, generator=g, device="cuda").half()
+kv = ops.PagedKV(pages, pages.clone())
+q = torch.randn(20, 8, 64, generator=g, device="cuda").half()
+k = torch.randn(3, 2, 64, generator=g, device="cuda").half()
+slots = torch.tensor([5, 6, 200], device="cuda")
+table = torch.arange(40, device="cuda", dtype=torch.int32).view(20, 2)
+lens = torch.full((20,), 25, device="cuda", dtype=torch.int32)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+  ops.kv_append(kv, k, k, slots)
+  a = ops.paged_attention(kv, q, table, lens)
+  b = ops.shared_prefix_attention(kv, q, table[0], 30, table, lens)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(kv.k_pages.view(-1, 2, 64)[slots], k)
+assert torch.equal(a, ops.paged_attention(kv, q, table, lens))
+assert torch.equal(b, ops.shared_prefix_attention(kv, q, table[0], 30, table, lens))
+"""
+  root = Path(__file__).resolve().parents[1]
+  r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                     timeout=120)
+  assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_other_device_than_the_current_one(cuda):
+  pools, table, lens_t, ptable, q, own, shared = build(17, BF, 32, 8, 128, 16, False, 1, [90] * 9,
+                                                       300)
+  there = lambda t: t.to("cuda:1")
+  kv = ops.PagedKV(*[there(p) for p in pools])
+  out = ops.shared_prefix_attention(kv, there(q), there(ptable), 300, there(table), there(lens_t))
+  assert out.device == torch.device("cuda:1")
+  want = ops.shared_prefix_attention(ops.PagedKV(*pools), q, ptable, 300, table, lens_t)
+  assert torch.equal(out.cpu(), want.cpu())
+
+
 def test_two_graphs_with_new_lengths(cuda):
   """Captured calls replay with lengths, tables and queries changed in place; two graphs keep
   their workspaces apart."""
@@ -673,6 +753,8 @@ def test_refusals_on_the_device(cuda):
                (kp.float(), kp.float()), (kp.transpose(2, 3), kp.transpose(2, 3))):
     with pytest.raises(ValueError):
       ops.PagedKV(*args)
+  with pytest.raises(ValueError):
+    ops.PagedKV(kp.clone().requires_grad_(), kp)
   spread = kp[:1].expand(4, 16, 2, 128)
   with pytest.raises(_native.NativeError):
     ops.paged_attention(ops.PagedKV(spread, kp), q, table, lens)

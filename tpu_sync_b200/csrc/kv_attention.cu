@@ -310,6 +310,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// CTAs of the walk on an SM.
+__host__ __device__ constexpr int walk_ctas(int d, int rows) {
+  return d == 64 && rows <= 16 ? 3 : 2;
+}
 template <int D>
 __host__ __device__ constexpr int stage_bytes() { return 2 * kWarpTokens * D * 2; }  // K and V of a warp's tokens
 template <int D>
@@ -427,7 +431,8 @@ struct Loader {
 };
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kWarps * 32, 2) walk_kernel(const __grid_constant__ WalkParams p) {
+__global__ void __launch_bounds__(kWarps * 32, walk_ctas(D, 16 * MT))
+    walk_kernel(const __grid_constant__ WalkParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tg = lane & 3;
@@ -1089,7 +1094,11 @@ __global__ void __launch_bounds__(128) join_cut_kernel(const __grid_constant__ W
       for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
         reinterpret_cast<float*>(p.a.lse)[at + i] = -INFINITY;
   }
-  if (w >= cut.ctas) return;
+  if (w >= cut.ctas) {
+    // also where no CTA has a share: this kernel never ends before the walk
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int lo = cut.start(w), hi = cut.start(w + 1);
   const Item it[2] = {item_at(p, lens, lo), item_at(p, lens, hi - 1)};
   const int first[2] = {lo - it[0].u + kItemCost, hi - 1 - it[1].u + kItemCost};  // first tiles
@@ -1238,7 +1247,7 @@ int check_attention(const ts_paged_kv* kv, const ts_attention_args* args) {
           (a.prefix_blocks > 0 ? pre_items * (a.prefix_blocks * bt / kTile + 1 + kItemCost) : 0) >
       double(INT32_MAX))
     return set_error(TS_INVALID_ARGUMENT, "batch, heads and table capacity too large for one call");
-  if (!(a.scale > 0.f) || !std::isfinite(a.scale))
+  if (!(a.scale > 0.f) || !std::isfinite(a.scale * kLog2e))
     return set_error(TS_INVALID_ARGUMENT, "scale must be finite and positive");
   return TS_OK;
 }
@@ -1271,7 +1280,7 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   w.tensor = pre && a.batch * a.new_tokens * group > 32 && prefix_geometry_ok(kv);
   const int64_t most = (pre && !w.tensor ? a.batch : 1) * a.new_tokens * group;
   w.rows = most <= 8 ? 8 : (most <= 16 ? 16 : 32);
-  w.ctas = 2 * sm_count(device);
+  w.ctas = walk_ctas(int(kv.head_dim), w.rows) * sm_count(device);
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = at;
@@ -1303,8 +1312,8 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
     walk = walk_kernel<T, D, kRows / 16>;
     smem = walk_smem<D>();
   }
-  static bool ready[64] = {};
-  if (device < 0 || device >= 64 || !ready[device]) {
+  static DevicesReady ready;
+  if (!ready.has(device)) {
     TS_CUDA_RET(cudaFuncSetAttribute(reinterpret_cast<const void*>(walk),
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
                 "attention shared memory");
@@ -1314,7 +1323,7 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
                                      cudaFuncAttributePreferredSharedMemoryCarveout,
                                      cudaSharedmemCarveoutMaxShared),
                 "attention shared memory");
-    if (device >= 0 && device < 64) ready[device] = true;
+    ready.add(device);
   }
   TS_CUDA_RET(launch_on(walk, unsigned(p.ctas), kWarps * 32, smem, s, p.tensor_ctas > 0, p),
               "attention launch");

@@ -42,6 +42,7 @@
 #include <numeric>
 #include <type_traits>
 
+#include "paged_kv.h"
 #include "prefix_attention.h"
 #include "ts_internal.h"
 
@@ -726,12 +727,12 @@ int make_map(CUtensorMap* map, const ts_paged_kv& kv, bool v, int piece) {
 template <typename T, int D>
 int launch(const PrefixParams& p, const CUtensorMap& k, const CUtensorMap& v, int device,
            cudaStream_t s) {
-  static bool ready[64] = {};
-  if (device >= 64 || !ready[device]) {
+  static DevicesReady ready;
+  if (!ready.has(device)) {
     TS_CUDA_RET(cudaFuncSetAttribute(prefix_kernel<T, D>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem),
                 "prefix attention shared memory");
-    if (device < 64) ready[device] = true;
+    ready.add(device);
   }
   prefix_kernel<T, D><<<p.ctas, kThreads, Shape<D>::kSmem, s>>>(p, k, v);
   TS_CUDA_RET(cudaGetLastError(), "prefix attention launch");

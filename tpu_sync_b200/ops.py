@@ -432,16 +432,19 @@ class PagedKV:
       raise ValueError("K and V pages must have one shape, dtype and device")
     if min(k_pages.shape[1:]) < 1:
       raise ValueError("pages need at least one token, head and element")
+    if k_pages.requires_grad or v_pages.requires_grad:
+      raise ValueError("pages must not require grad: they are written in place")
     self.k_pages, self.v_pages, self.head_major = k_pages, v_pages, bool(head_major)
     self.device, self.dtype = k_pages.device, k_pages.dtype
     tok, head = (2, 1) if head_major else (1, 2)
     self.pages, self.block_tokens = k_pages.shape[0], k_pages.shape[tok]
     self.heads, self.head_dim = k_pages.shape[head], k_pages.shape[3]
+    # a dimension of one element is never stepped over: its stride says nothing
+    strides = [t.stride(i) if t.shape[i] > 1 else 0 for t in (k_pages, v_pages)
+               for i in (0, tok, head)]
     self._c = _native.PagedKvC(
         k_pages.data_ptr(), v_pages.data_ptr(), self.pages, self.block_tokens, self.heads,
-        self.head_dim, k_pages.stride(0), k_pages.stride(tok), k_pages.stride(head),
-        v_pages.stride(0), v_pages.stride(tok), v_pages.stride(head),
-        _PAGE_DTYPES[self.dtype], 0)
+        self.head_dim, *strides, _PAGE_DTYPES[self.dtype], 0)
     self._ref = ctypes.byref(self._c)
     self._index = self.device.index
     self._workspace = {}  # bytes of attention workspace by shapes
@@ -697,7 +700,8 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, block_table: torch.Tensor,
 
   Tokens of a table entry outside the pages are left out, a length is cut to
   what its table row holds, and either sets err_flag (int32, on the device) to
-  1.  Nothing is read back: lengths and tables may change between replays of a
+  1 (2: a kernel gave up waiting for its own loads, the result is not valid).
+  Nothing is read back: lengths and tables may change between replays of a
   captured call.
   """
   return _attention(kv, q, block_table, seq_lens, None, 0, scale, out, return_lse, err_flag,
