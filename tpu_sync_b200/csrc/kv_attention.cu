@@ -62,6 +62,8 @@ struct WalkParams {
   float* pre_ml;
   int* err;
   int ctas;
+  int beside;         // CTAs that fit beside the prefix kernel's, 0: it takes every SM (or
+  int beside_units;   // there is none); taken when that is at most so many units of work
   int block_shift;    // log2(block_tokens), or -1
   // the prefix part when prefix_attention.cu does it: its partition and partials
   int tensor_ctas;    // 0: it does not
@@ -172,7 +174,8 @@ struct Lengths {
       bad = bad || now;
     }
     if (flag && bad) raise(p.err);
-    return Cut(warp_sum(sum), p.ctas);
+    const int total = warp_sum(sum);
+    return Cut(total, total <= p.beside_units ? p.beside : p.ctas);
   }
   __device__ __forceinline__ int get(const WalkParams& p, int k) const {
     int len = 0;
@@ -1256,7 +1259,7 @@ int check_attention(const ts_paged_kv* kv, const ts_attention_args* args) {
 // the length the host knows), so that what every CTA pays once (about 7 us:
 // queries in, partials out) is not most of its time; the SMs left over run the
 // walk meanwhile.
-constexpr int kPrefixShare = 6;
+constexpr int kPrefixShare = 7;
 int prefix_ctas(const ts_paged_kv& kv, const ts_attention_args& a, int64_t row_tiles, int device) {
   const int64_t len = std::min<int64_t>(a.prefix_len, a.prefix_blocks * kv.block_tokens);
   const int64_t nt = (len + kPrefixTile - 1) / kPrefixTile;
@@ -1440,6 +1443,17 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
     t.whole_ml = p.pre_ml;
     t.err = err_flag;
     p.tensor_ctas = t.ctas;
+    // A prefix kernel that leaves SMs free runs beside the walk.  CTAs of the
+    // walk that wait for it to end add their own fixed 5 us to its end, so the
+    // walk keeps to the free SMs unless its shares there would outlast the
+    // prefix (7 us + 2 us a unit) by more than that: 18 + 2.2 u units of 0.9 us
+    // each beside u units.  Prefix 8192 with 64 sequences 47 -> 37 us.
+    const int free_sms = tsb::sm_count(device) - t.ctas;
+    const int64_t nt = (std::min<int64_t>(a.prefix_len, a.prefix_blocks * kv->block_tokens) +
+                        tsb::kPrefixTile - 1) / tsb::kPrefixTile;
+    const double share = double(nt + tsb::kPrefixUnitCost) * t.row_tiles * kv->heads / t.ctas;
+    p.beside = free_sms > 0 ? w.ctas / tsb::sm_count(device) * free_sms : 0;
+    p.beside_units = int(p.beside * (18 + 2.2 * share));
     p.tensor_row_tiles = t.row_tiles;
     p.tensor_acc = t.slots_acc;
     p.tensor_ml = t.slots_ml;
