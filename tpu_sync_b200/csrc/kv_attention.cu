@@ -51,7 +51,7 @@ struct WalkParams {
   float scale_log2;   // scale * log2(e): softmax in powers of two
   int group;          // query heads per KV head
   int rows_own;       // rows of a sequence and KV head: new_tokens * group
-  int row_tiles_own;  // tiles of 8, 16 or 32 rows of them
+  int row_tiles_own;  // tiles of 8, 16, 24 or 32 rows of them
   int rows_pre;       // rows of the shared prefix and a KV head: all sequences'
   int row_tiles_pre;  // 0: no prefix in this kernel
   float* slots_acc;   // [ctas][2][rows of a tile][D]: partials of items cut between CTAs
@@ -313,17 +313,19 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// CTAs of the walk on an SM.
-__host__ __device__ constexpr int walk_ctas(int d, int rows) {
-  return d == 64 && rows <= 16 ? 3 : 2;
+// CTAs of the walk on an SM (64-wide heads: smaller stages and fewer sums;
+// 24 x 4 drafted tokens 24.9 us with two, 22.8 with three), and how many its
+// registers leave room for: one more where that costs no spills, so that a CTA
+// of the join is resident beside them.
+__host__ __device__ constexpr int walk_ctas(int d) { return d == 64 ? 3 : 2; }
+__host__ __device__ constexpr int walk_bound(int d, int nt) {
+  return d == 64 || nt <= 2 ? 3 : 2;
 }
 template <int D>
 __host__ __device__ constexpr int stage_bytes() { return 2 * kWarpTokens * D * 2; }  // K and V of a warp's tokens
 template <int D>
-__host__ __device__ constexpr int join_floats() { return 2 * 16 * (D + 4); }
-template <int D>
 __host__ __device__ constexpr int walk_smem() {
-  return kWarps * kStages * stage_bytes<D>() + join_floats<D>() * 4 + kWarps * kStages * 4;
+  return kWarps * kStages * stage_bytes<D>() + kWarps * kStages * 4;
 }
 
 // Row r of an item: sequence b's new token j, query head g of the KV head.
@@ -433,21 +435,34 @@ struct Loader {
   }
 };
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kWarps * 32, walk_ctas(D, 16 * MT))
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The walk over 8 kNt query rows of a KV head at a time.  The tokens are the
+// rows of the products and the queries their columns, S^T = K Q^T and
+// O^T = V^T P^T: K and V fragments are read from shared memory once for all
+// queries, which come in eights (one token of up to eight query heads, the
+// common decode step, fills half of what a 16-row product of queries would
+// work on).  S^T's fragments become P^T's operand by a transposing register
+// move.
+template <typename T, int D, int kNt>
+__global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
     walk_kernel(const __grid_constant__ WalkParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tg = lane & 3;
+  constexpr int kRows = 8 * kNt;
   constexpr int kRowBytes = D * 2;
-  constexpr int kRows = 16 * MT;
   const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
-  float* join = reinterpret_cast<float*>(smem + kWarps * kStages * stage_bytes<D>());
-  uint32_t* masks = reinterpret_cast<uint32_t*>(join + join_floats<D>()) + warp * kStages;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * stage_bytes<D>()) +
+                    warp * kStages;
 
-  // Lets join_kernel take SMs as they fall free.  With a prefix kernel before
-  // it, this one may itself run early: it reads nothing that kernel writes, and
-  // waits for it before it ends, so that join_kernel's wait covers both.
+  // Lets the join take SMs as they have room.  With a prefix kernel before it,
+  // this one may itself run early: it reads nothing that kernel writes, and
+  // waits for it before it ends, so that the join's wait covers both.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Cursor cu = start_cursor(p);
   Loader<T, D> loader(cu, ring, masks);
@@ -455,326 +470,51 @@ __global__ void __launch_bounds__(kWarps * 32, walk_ctas(D, 16 * MT))
   for (int s = 0; s < kStages - 1; ++s) loader.load(p, s);
   int st = 0;
 
-  while (!cu.done()) {
-    const int head = cu.head;
-    const int row0 = cu.rt * kRows;
-    const bool own = cu.b < p.a.batch;
-    const int n_rows = own ? p.rows_own : p.rows_pre;
-    // the query rows as mma A fragments, and what each of this thread's rows sees
-    uint32_t qf[MT][D / 16][4];
-    int vis[MT][2];
-    int vis_min = INT32_MAX;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int row = row0 + mt * 16 + hf * 8 + g;
-        const bool in = row < n_rows;
-        const T* src = nullptr;
-        vis[mt][hf] = cu.len;
-        if (in) {
-          const Row q = row_of(p, cu.b, row);
-          src = reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
-                q.j * p.a.q_token_stride + (head * p.group + q.g) * p.a.q_head_stride;
-          if (own) vis[mt][hf] = cu.len - int(p.a.new_tokens) + 1 + q.j;
-        }
-        vis_min = min(vis_min, vis[mt][hf]);
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          uint32_t x = 0, y = 0;
-          if (in) {
-            x = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg);
-            y = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg + 8);
-          }
-          qf[mt][ks][hf] = x;
-          qf[mt][ks][hf + 2] = y;
-        }
-      }
-    }
-    vis_min = __reduce_min_sync(~0u, vis_min);
-    // halves of eight rows that hold any (one for up to eight query heads)
-    const int halves = min(2 * MT, (n_rows - row0 + 7) / 8);
-
-    float acc[MT][D / 8][4];
-    float m[MT][2], l[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        acc[mt][i][0] = acc[mt][i][1] = acc[mt][i][2] = acc[mt][i][3] = 0.f;
-    }
-
-    for (int tile = cu.tile; tile < cu.end; ++tile) {
-      cp_wait<kStages - 2>();
-      __syncwarp();  // the stage is here, and every lane is done with the one before
-      const uint32_t kb = ring + st * stage_bytes<D>();
-      const uint32_t vb = kb + kWarpTokens * kRowBytes;
-      const uint32_t mask = masks[st];
-      const int t0 = tile * kTile + warp * kWarpTokens;
-      // 16 rows: two accumulators of the scores, for even and odd steps, halve
-      // the chain of products (32 rows are two chains anyway)
-      constexpr int kChains = MT == 1 ? 2 : 1;
-      float s[kChains][MT][2][4];
-#pragma unroll
-      for (int c = 0; c < kChains; ++c)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[c][mt][i][e] = 0.f;
-      // S = Q K^T: lane addresses rows (tokens) 0-7 / 8-15 and the two halves of 16 elements
-      {
-        const int r = (lane & 7) + ((lane >> 4) << 3);
-        const int hb = (lane >> 3) & 1;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          uint32_t b[4];
-          ldsm4(b, kb + r * kRowBytes + (((2 * ks + hb) ^ (r & 7)) << 4));
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            Ops<T>::mma(s[ks % kChains][mt][0], qf[mt][ks], b[0], b[1]);
-            Ops<T>::mma(s[ks % kChains][mt][1], qf[mt][ks], b[2], b[3]);
-          }
-        }
-      }
-      // The stage read in the round before is free: its refill runs under the
-      // products.
-      {
-        const int fill = st + kStages - 1;
-        loader.load(p, fill >= kStages ? fill - kStages : fill);
-      }
-      const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
-      uint32_t pf[MT][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          pf[mt][hf] = pf[mt][hf + 2] = 0;
-          if (2 * mt + hf >= halves) continue;
-          float x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[i] = s[0][mt][i / 2][2 * hf + i % 2];
-            if (kChains > 1) x[i] += s[kChains - 1][mt][i / 2][2 * hf + i % 2];
-            x[i] *= p.scale_log2;
-          }
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int tok = (i >> 1) * 8 + 2 * tg + (i & 1);
-              if (!((mask >> tok) & 1) || t0 + tok >= vis[mt][hf]) x[i] = -INFINITY;
-            }
-          }
-          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-          const float mn = fmaxf(m[mt][hf], mx);
-          const float base = mn == -INFINITY ? 0.f : mn;
-          const float corr = ex2(m[mt][hf] - base);
-          m[mt][hf] = mn;
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[i] = ex2(x[i] - base);
-            sum += x[i];
-          }
-          l[mt][hf] = l[mt][hf] * corr + sum;
-          pf[mt][hf] = Ops<T>::pack(x[0], x[1]);
-          pf[mt][hf + 2] = Ops<T>::pack(x[2], x[3]);
-          if (__any_sync(~0u, corr != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-              acc[mt][i][2 * hf] *= corr;
-              acc[mt][i][2 * hf + 1] *= corr;
-            }
-          }
-        }
-      }
-      // acc += P V
-      {
-        const int r = lane & 15, hb = lane >> 4;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t b[4];
-          ldsm4_t(b, vb + r * kRowBytes + (((2 * i + hb) ^ (r & 7)) << 4));
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            Ops<T>::mma(acc[mt][2 * i], pf[mt], b[0], b[1]);
-            Ops<T>::mma(acc[mt][2 * i + 1], pf[mt], b[2], b[3]);
-          }
-        }
-      }
-      if (++st == kStages) st = 0;
-    }
-
-    // Join the four warps (2 and 3 into 0 and 1, then 1 into 0), one 16-row
-    // tile at a time through a buffer of two.
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        l[mt][hf] += __shfl_xor_sync(~0u, l[mt][hf], 1);
-        l[mt][hf] += __shfl_xor_sync(~0u, l[mt][hf], 2);
-      }
-#pragma unroll
-      for (int step = 2; step >= 1; step >>= 1) {
-        __syncthreads();
-        float* buf = join + (warp & 1 & (step - 1)) * 16 * (D + 4);
-        if (warp >= step && warp < 2 * step) {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            if (2 * mt + hf >= halves) break;
-            float* row = buf + (hf * 8 + g) * (D + 4);
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-              *reinterpret_cast<float2*>(row + i * 8 + 2 * tg) =
-                  make_float2(acc[mt][i][2 * hf], acc[mt][i][2 * hf + 1]);
-            if (tg == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[mt][hf], l[mt][hf]);
-          }
-        }
-        __syncthreads();
-        if (warp < step) {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            if (2 * mt + hf >= halves) break;
-            const float* row = buf + (hf * 8 + g) * (D + 4);
-            const float2 ml = *reinterpret_cast<const float2*>(row + D);
-            const float mn = fmaxf(m[mt][hf], ml.x);
-            const float base = mn == -INFINITY ? 0.f : mn;
-            const float w0 = ex2(m[mt][hf] - base), w1 = ex2(ml.x - base);
-            m[mt][hf] = mn;
-            l[mt][hf] = l[mt][hf] * w0 + ml.y * w1;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-              const float2 o = *reinterpret_cast<const float2*>(row + i * 8 + 2 * tg);
-              acc[mt][i][2 * hf] = acc[mt][i][2 * hf] * w0 + o.x * w1;
-              acc[mt][i][2 * hf + 1] = acc[mt][i][2 * hf + 1] * w0 + o.y * w1;
-            }
-          }
-        }
-      }
-    }
-
-    if (warp == 0) {
-      const bool complete = cu.tile == 0 && cu.end == cu.nt;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int rl = mt * 16 + hf * 8 + g;
-          const int row = row0 + rl;
-          if (row >= n_rows) continue;
-          float *da, *dm;
-          if (!complete) {
-            const int64_t slot = int64_t(blockIdx.x) * 2 + (cu.tile == 0 ? 1 : 0);
-            da = p.slots_acc + (slot * kRows + rl) * D;
-            dm = p.slots_ml + (slot * kRows + rl) * 2;
-          } else {
-            const Row q = row_of(p, cu.b, row);
-            const int64_t out_row = (int64_t(q.b) * p.a.new_tokens + q.j) * p.a.q_heads +
-                                    head * p.group + q.g;
-            if (own && p.a.prefix_blocks == 0) {
-              // the whole row: the result itself
-              const float li = l[mt][hf];
-              const float inv = li > 0.f ? 1.f / li : (li == 0.f ? 0.f : li);
-              T* o = reinterpret_cast<T*>(p.a.out) + out_row * D;
-#pragma unroll
-              for (int i = 0; i < D / 8; ++i)
-                *reinterpret_cast<uint32_t*>(o + i * 8 + 2 * tg) =
-                    Ops<T>::pack(acc[mt][i][2 * hf] * inv, acc[mt][i][2 * hf + 1] * inv);
-              if (p.a.lse && tg == 0)
-                reinterpret_cast<float*>(p.a.lse)[out_row] =
-                    li == 0.f ? -INFINITY : (m[mt][hf] + log2f(li)) * kLn2;
-              continue;
-            }
-            da = (own ? p.own_acc : p.pre_acc) + out_row * D;
-            dm = (own ? p.own_ml : p.pre_ml) + out_row * 2;
-          }
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-            *reinterpret_cast<float2*>(da + i * 8 + 2 * tg) =
-                make_float2(acc[mt][i][2 * hf], acc[mt][i][2 * hf + 1]);
-          if (tg == 0) *reinterpret_cast<float2*>(dm) = make_float2(m[mt][hf], l[mt][hf]);
-        }
-    }
-    cu.next_item(p);
-  }
-  cp_wait<0>();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-// Up to eight query rows of a KV head (one token of up to eight query heads,
-// the common decode step): the tokens are the rows of the products and the
-// queries their eight columns, S^T = K Q^T and O^T = V^T P^T, so no product
-// works on rows that are not there, and a thread holds half as many sums.
-// S^T's fragments become P^T's operand by a transposing register move.
-template <int D>
-__host__ __device__ constexpr int walk8_smem() {
-  return kWarps * kStages * stage_bytes<D>() + kWarps * kStages * 4;
-}
-
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32, 3)
-    walk8_kernel(const __grid_constant__ WalkParams p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, tg = lane & 3;
-  constexpr int kRowBytes = D * 2;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
-  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * stage_bytes<D>()) +
-                    warp * kStages;
-
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // as in walk_kernel
-  Cursor cu = start_cursor(p);
-  Loader<T, D> loader(cu, ring, masks);
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) loader.load(p, s);
-  int st = 0;
-
-  // The queries as operand B (this thread: row g), and how many tokens this
-  // thread's two rows see.  Rows past the last one repeat it and are not written.
-  uint32_t qf[D / 16][2];
-  int vis[2], vis_min = 0;
+  // The queries as operand B (this thread: row g of each eight), and how many
+  // tokens this thread's two rows of each see.  Rows past the last one repeat it
+  // and are not written.
+  uint32_t qf[kNt][D / 16][2];
+  int vis[kNt][2], vis_min = 0;
   auto load_queries = [&](const Cursor& c) {
     const bool own = c.b < p.a.batch;
     const int n_rows = own ? p.rows_own : p.rows_pre;
     vis_min = INT32_MAX;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const Row q = row_of(p, c.b, min(c.rt * 8 + 2 * tg + e, n_rows - 1));
-      vis[e] = own ? c.len - int(p.a.new_tokens) + 1 + q.j : c.len;
-      vis_min = min(vis_min, vis[e]);
+    for (int nt = 0; nt < kNt; ++nt) {
+      const int row0 = c.rt * kRows + nt * 8;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const Row q = row_of(p, c.b, min(row0 + 2 * tg + e, n_rows - 1));
+        vis[nt][e] = own ? c.len - int(p.a.new_tokens) + 1 + q.j : c.len;
+        vis_min = min(vis_min, vis[nt][e]);
+      }
+      const Row q = row_of(p, c.b, min(row0 + g, n_rows - 1));
+      const T* src = reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
+                     q.j * p.a.q_token_stride + (c.head * p.group + q.g) * p.a.q_head_stride;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qf[nt][ks][0] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg);
+        qf[nt][ks][1] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg + 8);
+      }
     }
     vis_min = __reduce_min_sync(~0u, vis_min);
-    const Row q = row_of(p, c.b, min(c.rt * 8 + g, n_rows - 1));
-    const T* src = reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
-                   q.j * p.a.q_token_stride + (c.head * p.group + q.g) * p.a.q_head_stride;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      qf[ks][0] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg);
-      qf[ks][1] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tg + 8);
-    }
   };
   if (!cu.done()) load_queries(cu);
 
   while (!cu.done()) {
-    const int row0 = cu.rt * 8;
     const bool own = cu.b < p.a.batch;
     const int n_rows = own ? p.rows_own : p.rows_pre;
-    // acc[i]: elements 16 i + g and 16 i + g + 8 of rows 2 tg and 2 tg + 1
-    float acc[D / 16][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // acc[.][i]: elements 16 i + g and 16 i + g + 8 of rows 2 tg and 2 tg + 1
+    float acc[kNt][D / 16][4];
+    float m[kNt][2], l[kNt][2];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    for (int nt = 0; nt < kNt; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+    }
 
     for (int tile = cu.tile; tile < cu.end; ++tile) {
       cp_wait<kStages - 2>();
@@ -783,15 +523,24 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
       const uint32_t vb = kb + kWarpTokens * kRowBytes;
       const uint32_t mask = masks[st];
       const int t0 = tile * kTile + warp * kWarpTokens;
-      // S^T = K Q^T in two accumulators, for even and odd steps
-      float s[2][4] = {};
+      // S^T = K Q^T; eight rows alone in two accumulators, for even and odd
+      // steps, which halves the chain of products (more rows are more chains)
+      constexpr int kChains = kNt == 1 ? 2 : 1;
+      float s[kChains][kNt][4];
+#pragma unroll
+      for (int c = 0; c < kChains; ++c)
+#pragma unroll
+        for (int nt = 0; nt < kNt; ++nt)
+          s[c][nt][0] = s[c][nt][1] = s[c][nt][2] = s[c][nt][3] = 0.f;
       {
         const int r = lane & 15, hb = lane >> 4;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t a[4];
           ldsm4(a, kb + r * kRowBytes + (((2 * ks + hb) ^ (r & 7)) << 4));
-          Ops<T>::mma(s[ks & 1], a, qf[ks][0], qf[ks][1]);
+#pragma unroll
+          for (int nt = 0; nt < kNt; ++nt)
+            Ops<T>::mma(s[ks % kChains][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
         }
       }
       // The stage read in the round before is free: its refill runs under the
@@ -801,41 +550,63 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
         loader.load(p, fill >= kStages ? fill - kStages : fill);
       }
       const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
-      float x[4], corr[2];
+      float x[kNt][4];
+      bool grew = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = (s[0][i] + s[1][i]) * p.scale_log2;
-      if (!whole) {
+      for (int nt = 0; nt < kNt; ++nt) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int tok = g + (i >> 1) * 8;
-          if (!((mask >> tok) & 1) || t0 + tok >= vis[i & 1]) x[i] = -INFINITY;
+          x[nt][i] = s[0][nt][i];
+          if (kChains > 1) x[nt][i] += s[kChains - 1][nt][i];
+          x[nt][i] *= p.scale_log2;
+          if (!whole) {
+            const int tok = g + (i >> 1) * 8;
+            if (!((mask >> tok) & 1) || t0 + tok >= vis[nt][i & 1]) x[nt][i] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) grew = grew || fmaxf(x[nt][e], x[nt][e + 2]) > m[nt][e] + 8.f;
+      }
+      // m is any common reference of a row: it follows the maximum only when
+      // that grew by more than 2^8, so that most tiles need no exchange between
+      // lanes and no rescaling, and no weight passes 2^8.
+      if (__any_sync(~0u, grew)) {
+#pragma unroll
+        for (int nt = 0; nt < kNt; ++nt) {
+          float corr[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(x[nt][e], x[nt][e + 2]);
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
+            const float mn = fmaxf(m[nt][e], mx);
+            corr[e] = ex2(m[nt][e] - (mn == -INFINITY ? 0.f : mn));
+            m[nt][e] = mn;
+            l[nt][e] *= corr[e];
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            acc[nt][i][0] *= corr[0];
+            acc[nt][i][1] *= corr[1];
+            acc[nt][i][2] *= corr[0];
+            acc[nt][i][3] *= corr[1];
+          }
         }
       }
+      uint32_t pf[kNt][2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float mx = fmaxf(x[e], x[e + 2]);
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
-        const float mn = fmaxf(m[e], mx);
-        const float base = mn == -INFINITY ? 0.f : mn;
-        corr[e] = ex2(m[e] - base);
-        m[e] = mn;
-        x[e] = ex2(x[e] - base);
-        x[e + 2] = ex2(x[e + 2] - base);
-        l[e] = l[e] * corr[e] + x[e] + x[e + 2];
-      }
-      if (__any_sync(~0u, corr[0] != 1.f || corr[1] != 1.f)) {
+      for (int nt = 0; nt < kNt; ++nt) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          acc[i][0] *= corr[0];
-          acc[i][1] *= corr[1];
-          acc[i][2] *= corr[0];
-          acc[i][3] *= corr[1];
+        for (int e = 0; e < 2; ++e) {
+          const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+          x[nt][e] = ex2(x[nt][e] - base);
+          x[nt][e + 2] = ex2(x[nt][e + 2] - base);
+          l[nt][e] += x[nt][e] + x[nt][e + 2];
         }
+        pf[nt][0] = transpose8(Ops<T>::pack(x[nt][0], x[nt][1]));
+        pf[nt][1] = transpose8(Ops<T>::pack(x[nt][2], x[nt][3]));
       }
-      const uint32_t p0 = transpose8(Ops<T>::pack(x[0], x[1]));
-      const uint32_t p1 = transpose8(Ops<T>::pack(x[2], x[3]));
       // O^T += V^T P^T
       {
         const int r = (lane & 7) + ((lane >> 4) << 3), hb = (lane >> 3) & 1;
@@ -843,7 +614,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
         for (int i = 0; i < D / 16; ++i) {
           uint32_t a[4];
           ldsm4_t(a, vb + r * kRowBytes + (((2 * i + hb) ^ (r & 7)) << 4));
-          Ops<T>::mma(acc[i], a, p0, p1);
+#pragma unroll
+          for (int nt = 0; nt < kNt; ++nt) Ops<T>::mma(acc[nt][i], a, pf[nt][0], pf[nt][1]);
         }
       }
       if (++st == kStages) st = 0;
@@ -854,31 +626,37 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     next.next_item(p);
     if (!next.done()) load_queries(next);
 
-    // All four warps' parts through shared memory, each in its ring's stage that
-    // was read last and is not refilled before the next item's first tile; then
-    // 16 threads a row.
+    // All four warps' parts through shared memory, eight rows at a time, each
+    // in its ring's stage that was read last and is not refilled before the next
+    // item's first tile; then 16 threads a row.
     static_assert(8 * (D + 4) * 4 <= stage_bytes<D>(), "a warp's part fits a stage");
     const int free_st = st == 0 ? kStages - 1 : st - 1;
     auto part = [&](int w) {
       return reinterpret_cast<float*>(smem + (w * kStages + free_st) * stage_bytes<D>());
     };
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int nt = 0; nt < kNt; ++nt) {
+      const int row0 = cu.rt * kRows + nt * 8;
+      if (row0 >= n_rows) break;
 #pragma unroll
-      for (int k = 4; k < 32; k <<= 1) l[e] += __shfl_xor_sync(~0u, l[e], k);
-    __syncwarp();  // every lane is done with the stage
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float* row = part(warp) + (2 * tg + e) * (D + 4);
+        for (int k = 4; k < 32; k <<= 1) l[nt][e] += __shfl_xor_sync(~0u, l[nt][e], k);
+      if (nt == 0)
+        __syncwarp();  // every lane is done with the stage
+      else
+        __syncthreads();  // the eight rows before have been read
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        row[16 * i + g] = acc[i][e];
-        row[16 * i + g + 8] = acc[i][e + 2];
+      for (int e = 0; e < 2; ++e) {
+        float* row = part(warp) + (2 * tg + e) * (D + 4);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          row[16 * i + g] = acc[nt][i][e];
+          row[16 * i + g + 8] = acc[nt][i][e + 2];
+        }
+        if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[nt][e], l[nt][e]);
       }
-      if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[e], l[e]);
-    }
-    __syncthreads();
-    {
+      __syncthreads();
       constexpr int kPer = D / 16;  // elements a thread joins
       const int rl = threadIdx.x >> 4, at = (threadIdx.x & 15) * kPer;
       const int row = row0 + rl;
@@ -928,7 +706,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
             da = (own ? p.own_acc : p.pre_acc) + out_row * D;
             dm = (own ? p.own_ml : p.pre_ml) + out_row * 2;
           } else {
-            const int64_t slot = (int64_t(blockIdx.x) * 2 + (cu.tile == 0 ? 1 : 0)) * 8 + rl;
+            const int64_t slot = (int64_t(blockIdx.x) * 2 + (cu.tile == 0 ? 1 : 0)) * kRows +
+                                 nt * 8 + rl;
             da = p.slots_acc + slot * D;
             dm = p.slots_ml + slot * 2;
           }
@@ -1282,8 +1061,8 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   const bool pre = a.prefix_blocks > 0;
   w.tensor = pre && a.batch * a.new_tokens * group > 32 && prefix_geometry_ok(kv);
   const int64_t most = (pre && !w.tensor ? a.batch : 1) * a.new_tokens * group;
-  w.rows = most <= 8 ? 8 : (most <= 16 ? 16 : 32);
-  w.ctas = walk_ctas(int(kv.head_dim), w.rows) * sm_count(device);
+  w.rows = most <= 24 ? std::max(1, int(most + 7) / 8) * 8 : 32;
+  w.ctas = walk_ctas(int(kv.head_dim)) * sm_count(device);
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = at;
@@ -1306,15 +1085,8 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
 
 template <typename T, int D, int kRows>
 int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
-  void (*walk)(WalkParams);
-  size_t smem;
-  if constexpr (kRows == 8) {
-    walk = walk8_kernel<T, D>;
-    smem = walk8_smem<D>();
-  } else {
-    walk = walk_kernel<T, D, kRows / 16>;
-    smem = walk_smem<D>();
-  }
+  void (*walk)(WalkParams) = walk_kernel<T, D, kRows / 8>;
+  constexpr size_t smem = walk_smem<D>();
   static DevicesReady ready;
   if (!ready.has(device)) {
     TS_CUDA_RET(cudaFuncSetAttribute(reinterpret_cast<const void*>(walk),
@@ -1352,6 +1124,7 @@ template <typename T, int D>
 int launch_rows(const WalkParams& p, int rows, int device, cudaStream_t s) {
   return rows == 8    ? launch_attention<T, D, 8>(p, device, s)
          : rows == 16 ? launch_attention<T, D, 16>(p, device, s)
+         : rows == 24 ? launch_attention<T, D, 24>(p, device, s)
                       : launch_attention<T, D, 32>(p, device, s);
 }
 template <typename T>
