@@ -325,7 +325,7 @@ template <int D>
 __host__ __device__ constexpr int stage_bytes() { return 2 * kWarpTokens * D * 2; }  // K and V of a warp's tokens
 template <int D>
 __host__ __device__ constexpr int walk_smem() {
-  return kWarps * kStages * stage_bytes<D>() + kWarps * kStages * 4;
+  return kWarps * kStages * (stage_bytes<D>() + 12) + 4 + 1024;
 }
 
 // Row r of an item: sequence b's new token j, query head g of the KV head.
@@ -343,77 +343,106 @@ __device__ __forceinline__ Row row_of(const WalkParams& p, int seq, int row) {
   return r;
 }
 
+// Pages as TMA loads them (pages of a multiple of 16 tokens: a warp's 16 tokens
+// are one box per 64 elements).
+struct PageMaps {
+  CUtensorMap k, v;
+};
+
 // A warp's loads: the 16 tokens it owns of each tile of the CTA's share, one
-// ring stage (K, then V) per tile, across items.
-template <typename T, int D>
+// ring stage (K, then V) per tile, across items.  A stage holds blocks of 64
+// elements, [16 tokens][128 bytes] in the 128-byte swizzle (16-byte piece c of
+// token r at piece c ^ (r & 7)).  With kTma one lane loads a stage by TMA;
+// else (other page sizes) all lanes by 16-byte copies, which took 200 of the
+// 416 instructions a warp spends on a tile where TMA takes about 40.
+template <typename T, int D, bool kTma>
 struct Loader {
-  static constexpr int kChunks = D / 8;  // 16-byte pieces of a head vector
-  static constexpr int kRowBytes = D * 2;
+  static constexpr int kBlock = kWarpTokens * 128;  // 64 elements of 16 tokens
   Cursor at;
   int tile;
   uint32_t ring;    // of this warp
+  uint32_t bars;    // kTma: a stage's barrier
   uint32_t* masks;  // tokens of each stage that count, one bit each
   // table entries [window, window + 32) of sequence window_seq, one a lane
   int window, entry, window_seq;
 
-  __device__ __forceinline__ Loader(const Cursor& c, uint32_t r, uint32_t* m)
-      : at(c), tile(c.tile), ring(r), masks(m), window(-1), entry(0), window_seq(-1) {}
+  __device__ __forceinline__ Loader(const Cursor& c, uint32_t r, uint32_t b, uint32_t* m)
+      : at(c), tile(c.tile), ring(r), bars(b), masks(m), window(-1), entry(0), window_seq(-1) {}
 
-  // Queues the next tile into stage `st` (an empty group past the last one).
-  __device__ __forceinline__ void load(const WalkParams& p, int st) {
+  __device__ __forceinline__ int block_of(const WalkParams& p, int t) const {
+    return p.block_shift >= 0 ? t >> p.block_shift
+                              : int(uint32_t(t) / uint32_t(p.kv.block_tokens));
+  }
+  // Table entries from block `first` on, unless `count` of them are held.
+  __device__ __forceinline__ void hold(const WalkParams& p, int first, int count) {
+    if (at.b == window_seq && first >= window && first + count <= window + 32) return;
+    window = first;
+    window_seq = at.b;
+    const int32_t* table =
+        at.b < p.a.batch
+            ? reinterpret_cast<const int32_t*>(p.a.block_table) + at.b * p.a.block_table_stride
+            : reinterpret_cast<const int32_t*>(p.a.prefix_table);
+    const int mine = first + int(threadIdx.x & 31);
+    entry = mine <= block_of(p, at.len - 1) ? __ldg(table + mine) : 0;
+  }
+
+  // Queues the next tile into stage `st` (nothing past the last one).
+  __device__ __forceinline__ void load(const WalkParams& p, const PageMaps& maps, int st) {
     if (at.done()) {
-      cp_commit();
+      if (!kTma) cp_commit();
       return;
     }
-    const int bt = int(p.kv.block_tokens);
+    const int lane = threadIdx.x & 31;
     const int t0 = tile * kTile + int(threadIdx.x >> 5) * kWarpTokens;
     const uint32_t kdst = ring + st * stage_bytes<D>();
-    const uint32_t vdst = kdst + kWarpTokens * kRowBytes;
-    const int lane = threadIdx.x & 31;
-    const int c = lane % kChunks;
-    constexpr int kPer = 32 / kChunks;  // tokens a warp's 32 lanes copy at once
-    // lanes 0..15 place one token each
-    const int t = t0 + (lane & 15);
-    const int blk = p.block_shift >= 0 ? t >> p.block_shift : int(uint32_t(t) / uint32_t(bt));
-    const int off = t - blk * bt;
-    bool ok = t < at.len;
-    const int first = __shfl_sync(~0u, blk, 0);
-    // 16 tokens touch at most 16 entries: one window holds them
-    if (at.b != window_seq || first < window || first + 16 > window + 32) {
-      window = first;
-      window_seq = at.b;
-      const int32_t* table =
-          at.b < p.a.batch
-              ? reinterpret_cast<const int32_t*>(p.a.block_table) + at.b * p.a.block_table_stride
-              : reinterpret_cast<const int32_t*>(p.a.prefix_table);
-      const int last = p.block_shift >= 0 ? (at.len - 1) >> p.block_shift : (at.len - 1) / bt;
-      entry = window + lane <= last ? __ldg(table + window + lane) : 0;
-    }
-    const int page = __shfl_sync(~0u, entry, blk - window);
-    if (ok && (page < 0 || page >= p.kv.pages)) {
-      raise(p.err);
-      ok = false;
-    }
-    const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
-    if (lane == 0) masks[st] = mask;
-    const T* kp = reinterpret_cast<const T*>(p.kv.k_ptr) + at.head * p.kv.k_head_stride;
-    const T* vp = reinterpret_cast<const T*>(p.kv.v_ptr) + at.head * p.kv.v_head_stride;
-    if (mask == 0xffffu && bt % kWarpTokens == 0) {
-      // all in one page: one address, even steps
-      const int r0 = lane / kChunks;
-      const T* kr = kp + page * p.kv.k_page_stride + (__shfl_sync(~0u, off, 0) + r0) * p.kv.k_token_stride + c * 8;
-      const T* vr = vp + page * p.kv.v_page_stride + (__shfl_sync(~0u, off, 0) + r0) * p.kv.v_token_stride + c * 8;
-      const int64_t ks = kPer * p.kv.k_token_stride, vs = kPer * p.kv.v_token_stride;
-#pragma unroll
-      for (int i = 0; i < kWarpTokens / kPer; ++i) {
-        const int r = i * kPer + r0;
-        const uint32_t at = r * kRowBytes + ((c ^ (r & 7)) << 4);
-        cp_async16(kdst + at, kr, true);
-        cp_async16(vdst + at, vr, true);
-        kr += ks;
-        vr += vs;
+    const uint32_t vdst = kdst + kWarpTokens * D * 2;
+    if constexpr (kTma) {
+      int count = min(kWarpTokens, at.len - t0);  // tokens that count
+      const int blk = block_of(p, t0);
+      int page = 0;
+      if (count > 0) {
+        hold(p, blk, 1);
+        page = __shfl_sync(~0u, entry, blk - window);
+        if (page < 0 || page >= p.kv.pages) {
+          raise(p.err);
+          count = 0;
+        }
       }
+      const uint32_t bar = bars + 8 * st;
+      if (elect()) {
+        masks[st] = count > 0 ? (1u << count) - 1 : 0u;
+        if (count > 0) {
+          const int off = t0 - blk * int(p.kv.block_tokens);
+          bar_expect(bar, stage_bytes<D>());
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h) {
+            tma_4d(kdst + h * kBlock, &maps.k, bar, h * 64, off, at.head, page);
+            tma_4d(vdst + h * kBlock, &maps.v, bar, h * 64, off, at.head, page);
+          }
+        } else {
+          bar_arrive(bar);
+        }
+      }
+      __syncwarp();
     } else {
+      constexpr int kChunks = D / 8;      // 16-byte pieces of a head vector
+      constexpr int kPer = 32 / kChunks;  // tokens a warp's 32 lanes copy at once
+      const int c = lane % kChunks;
+      // lanes 0..15 place one token each
+      const int t = t0 + (lane & 15);
+      const int blk = block_of(p, t);
+      const int off = t - blk * int(p.kv.block_tokens);
+      bool ok = t < at.len;
+      hold(p, __shfl_sync(~0u, blk, 0), kWarpTokens);  // 16 tokens touch at most 16 entries
+      const int page = __shfl_sync(~0u, entry, blk - window);
+      if (ok && (page < 0 || page >= p.kv.pages)) {
+        raise(p.err);
+        ok = false;
+      }
+      const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
+      if (lane == 0) masks[st] = mask;
+      const T* kp = reinterpret_cast<const T*>(p.kv.k_ptr) + at.head * p.kv.k_head_stride;
+      const T* vp = reinterpret_cast<const T*>(p.kv.v_ptr) + at.head * p.kv.v_head_stride;
       const int64_t ko = page * p.kv.k_page_stride + off * p.kv.k_token_stride;
       const int64_t vo = page * p.kv.v_page_stride + off * p.kv.v_token_stride;
 #pragma unroll
@@ -421,13 +450,13 @@ struct Loader {
         const int r = i * kPer + lane / kChunks;
         const int64_t kr = __shfl_sync(~0u, ko, r), vr = __shfl_sync(~0u, vo, r);
         const bool in = (mask >> r) & 1;
-        const uint32_t at = r * kRowBytes + ((c ^ (r & 7)) << 4);
+        const uint32_t to = (c / 8) * kBlock + r * 128 + (((c % 8) ^ (r & 7)) << 4);
         // a source that is not read still is an address of the pages
-        cp_async16(kdst + at, in ? kp + kr + c * 8 : reinterpret_cast<const T*>(p.kv.k_ptr), in);
-        cp_async16(vdst + at, in ? vp + vr + c * 8 : reinterpret_cast<const T*>(p.kv.v_ptr), in);
+        cp_async16(kdst + to, in ? kp + kr + c * 8 : reinterpret_cast<const T*>(p.kv.k_ptr), in);
+        cp_async16(vdst + to, in ? vp + vr + c * 8 : reinterpret_cast<const T*>(p.kv.v_ptr), in);
       }
+      cp_commit();
     }
-    cp_commit();
     if (++tile == at.end) {
       at.next_item(p);
       tile = at.tile;
@@ -448,27 +477,38 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // common decode step, fills half of what a 16-row product of queries would
 // work on).  S^T's fragments become P^T's operand by a transposing register
 // move.
-template <typename T, int D, int kNt>
+template <typename T, int D, int kNt, bool kTma>
 __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
-    walk_kernel(const __grid_constant__ WalkParams p) {
-  extern __shared__ __align__(128) uint8_t smem[];
+    walk_kernel(const __grid_constant__ WalkParams p, const __grid_constant__ PageMaps maps) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tg = lane & 3;
   constexpr int kRows = 8 * kNt;
-  constexpr int kRowBytes = D * 2;
+  constexpr int kBlock = Loader<T, D, kTma>::kBlock;
   const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
-  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * stage_bytes<D>()) +
-                    warp * kStages;
+  uint8_t* ctl = smem + kWarps * kStages * stage_bytes<D>();
+  const uint32_t bars = smem_u32(ctl) + warp * kStages * 8;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(ctl + kWarps * kStages * 8) + warp * kStages;
+  volatile int* gone = reinterpret_cast<volatile int*>(ctl + kWarps * kStages * 12);
+  if (kTma) {
+    if (lane < kStages) bar_init(bars + 8 * lane, 1);
+    if (threadIdx.x == 0) *gone = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+  }
 
   // Lets the join take SMs as they have room.  With a prefix kernel before it,
   // this one may itself run early: it reads nothing that kernel writes, and
   // waits for it before it ends, so that the join's wait covers both.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Cursor cu = start_cursor(p);
-  Loader<T, D> loader(cu, ring, masks);
+  Loader<T, D, kTma> loader(cu, ring, bars, masks);
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) loader.load(p, s);
+  for (int s = 0; s < kStages - 1; ++s) loader.load(p, maps, s);
   int st = 0;
+  uint32_t phase = 0;
 
   // The queries as operand B (this thread: row g of each eight), and how many
   // tokens this thread's two rows of each see.  Rows past the last one repeat it
@@ -517,11 +557,31 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
     }
 
     for (int tile = cu.tile; tile < cu.end; ++tile) {
-      cp_wait<kStages - 2>();
-      __syncwarp();  // the stage is here, and every lane is done with the one before
+      // the stage is here, and every lane is done with the one before; a wait
+      // that runs out (flag 2, no valid result) cuts all further ones short
+      if constexpr (kTma) {
+        bar_wait(bars + 8 * st, phase, gone);
+      } else {
+        cp_wait<kStages - 2>();
+      }
+      __syncwarp();
       const uint32_t kb = ring + st * stage_bytes<D>();
-      const uint32_t vb = kb + kWarpTokens * kRowBytes;
+      const uint32_t vb = kb + kWarpTokens * D * 2;
       const uint32_t mask = masks[st];
+      if (kTma && mask != 0xffffu) {
+        // V of tokens that do not count: a page may hold anything there, which
+        // must not meet a weight of 0
+        for (int i = lane; i < kWarpTokens * D / 8; i += 32) {
+          const int r = i % kWarpTokens, c = i / kWarpTokens;
+          if (!((mask >> r) & 1))
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             vb + (c / 8) * kBlock + r * 128 + (c % 8) * 16),
+                         "r"(0)
+                         : "memory");
+        }
+        fence_async();
+        __syncwarp();
+      }
       const int t0 = tile * kTile + warp * kWarpTokens;
       // S^T = K Q^T; eight rows alone in two accumulators, for even and odd
       // steps, which halves the chain of products (more rows are more chains)
@@ -537,7 +597,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t a[4];
-          ldsm4(a, kb + r * kRowBytes + (((2 * ks + hb) ^ (r & 7)) << 4));
+          ldsm4(a, kb + (ks / 4) * kBlock + r * 128 + (((2 * (ks % 4) + hb) ^ (r & 7)) << 4));
 #pragma unroll
           for (int nt = 0; nt < kNt; ++nt)
             Ops<T>::mma(s[ks % kChains][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
@@ -547,7 +607,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
       // products.
       {
         const int fill = st + kStages - 1;
-        loader.load(p, fill >= kStages ? fill - kStages : fill);
+        loader.load(p, maps, fill >= kStages ? fill - kStages : fill);
       }
       const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
       float x[kNt][4];
@@ -613,12 +673,15 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           uint32_t a[4];
-          ldsm4_t(a, vb + r * kRowBytes + (((2 * i + hb) ^ (r & 7)) << 4));
+          ldsm4_t(a, vb + (i / 4) * kBlock + r * 128 + (((2 * (i % 4) + hb) ^ (r & 7)) << 4));
 #pragma unroll
           for (int nt = 0; nt < kNt; ++nt) Ops<T>::mma(acc[nt][i], a, pf[nt][0], pf[nt][1]);
         }
       }
-      if (++st == kStages) st = 0;
+      if (++st == kStages) {
+        st = 0;
+        phase ^= 1;
+      }
     }
 
     // The next item's queries are on their way while this one is joined.
@@ -719,10 +782,19 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
         }
       }
     }
+    if (kTma) fence_async();
     __syncthreads();  // the parts have been read: the stages may be refilled
     cu = next;
   }
-  cp_wait<0>();
+  if constexpr (kTma) {
+    if (*gone) {
+      // loads still in flight land before their shared memory is given back
+      if (lane == 0 && p.err) *reinterpret_cast<volatile int*>(p.err) = 2;
+      for (int i = 0; i < 100; ++i) __nanosleep(100000);
+    }
+  } else {
+    cp_wait<0>();
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
@@ -1083,9 +1155,9 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   return w;
 }
 
-template <typename T, int D, int kRows>
-int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
-  void (*walk)(WalkParams) = walk_kernel<T, D, kRows / 8>;
+template <typename T, int D, int kRows, bool kTma>
+int launch_walk(const WalkParams& p, const PageMaps& maps, int device, cudaStream_t s) {
+  void (*walk)(WalkParams, PageMaps) = walk_kernel<T, D, kRows / 8, kTma>;
   constexpr size_t smem = walk_smem<D>();
   static DevicesReady ready;
   if (!ready.has(device)) {
@@ -1100,8 +1172,22 @@ int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
                 "attention shared memory");
     ready.add(device);
   }
-  TS_CUDA_RET(launch_on(walk, unsigned(p.ctas), kWarps * 32, smem, s, p.tensor_ctas > 0, p),
+  TS_CUDA_RET(launch_on(walk, unsigned(p.ctas), kWarps * 32, smem, s, p.tensor_ctas > 0, p, maps),
               "attention launch");
+  return TS_OK;
+}
+
+template <typename T, int D, int kRows>
+int launch_attention(const WalkParams& p, int device, cudaStream_t s) {
+  PageMaps maps{};
+  // a warp's 16 tokens in one page, and strides as tensor maps take them
+  if (p.kv.block_tokens % kWarpTokens == 0 && prefix_geometry_ok(p.kv)) {
+    if (int rc = make_page_map(&maps.k, p.kv, false, kWarpTokens)) return rc;
+    if (int rc = make_page_map(&maps.v, p.kv, true, kWarpTokens)) return rc;
+    if (int rc = launch_walk<T, D, kRows, true>(p, maps, device, s)) return rc;
+  } else if (int rc = launch_walk<T, D, kRows, false>(p, maps, device, s)) {
+    return rc;
+  }
   if (p.a.prefix_blocks == 0) {
     TS_CUDA_RET(launch_on(join_cut_kernel<T, D, kRows>, unsigned(p.ctas), 128, 0, s, true, p),
                 "attention join launch");

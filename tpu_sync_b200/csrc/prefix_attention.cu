@@ -50,7 +50,6 @@ namespace tsb {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr uint32_t kWaitRounds = 1u << 24;  // try_waits (each suspends for a while): seconds
 
 template <int D>
 struct Shape {
@@ -64,51 +63,12 @@ struct Shape {
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return uint32_t(__cvta_generic_to_shared(p));
 }
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// A whole warp's wait; false (for all its lanes) when it ran out here or in
-// another role.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
-  bool ok = bar_try(bar, parity);
-  for (uint32_t i = 0; !ok && i < kWaitRounds && !*gone; ++i) ok = bar_try(bar, parity);
-  if (!ok) *gone = 1;
-  return __all_sync(~0u, ok);
-}
-
-// The same for one thread.
+// bar_wait for one thread.
 __device__ __forceinline__ bool bar_wait_one(uint32_t bar, uint32_t parity, volatile int* gone) {
   bool ok = bar_try(bar, parity);
   for (uint32_t i = 0; !ok && i < kWaitRounds && !*gone; ++i) ok = bar_try(bar, parity);
   if (!ok) *gone = 1;
   return ok;
-}
-
-__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
-                                       int token, int head, int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], "
-      "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(map), "r"(bar), "r"(x), "r"(token), "r"(head), "r"(page)
-      : "memory");
 }
 
 __device__ __forceinline__ void fence_before() {
@@ -121,14 +81,6 @@ __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
       : "memory");
-}
-// One lane of a converged warp, always the same one.
-__device__ __forceinline__ bool elect() {
-  uint32_t e;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(e));
-  return e != 0;
 }
 // D[tmem] (+)= A B, both operands in shared memory
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
@@ -396,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t at = dst + (c / 8) * kPrefixTile * 128 + r * 128 + (c % 8) * 16;
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            fence_async();
             __syncwarp();
             if (lane == 0) bar_arrive(full + 8 * st);
           }
@@ -523,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
                        : "memory");
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fence_async();
         bar_arrive(q_full + 8 * x);
       }
       // whether any page of the segment is bad: then every tile is looked at
@@ -698,9 +650,24 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-// [pages][heads][tokens][D] with the storage's strides; boxes of 64 elements x
-// `piece` tokens.
-int make_map(CUtensorMap* map, const ts_paged_kv& kv, bool v, int piece) {
+template <typename T, int D>
+int launch(const PrefixParams& p, const CUtensorMap& k, const CUtensorMap& v, int device,
+           cudaStream_t s) {
+  static DevicesReady ready;
+  if (!ready.has(device)) {
+    TS_CUDA_RET(cudaFuncSetAttribute(prefix_kernel<T, D>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem),
+                "prefix attention shared memory");
+    ready.add(device);
+  }
+  prefix_kernel<T, D><<<p.ctas, kThreads, Shape<D>::kSmem, s>>>(p, k, v);
+  TS_CUDA_RET(cudaGetLastError(), "prefix attention launch");
+  return TS_OK;
+}
+
+}  // namespace
+
+int make_page_map(CUtensorMap* map, const ts_paged_kv& kv, bool v, int piece) {
   const EncodeFn fn = encode_fn();
   if (!fn) return set_error(TS_INTERNAL, "cuTensorMapEncodeTiled is not available");
   const int64_t st[3] = {v ? kv.v_token_stride : kv.k_token_stride,
@@ -724,23 +691,6 @@ int make_map(CUtensorMap* map, const ts_paged_kv& kv, bool v, int piece) {
   return TS_OK;
 }
 
-template <typename T, int D>
-int launch(const PrefixParams& p, const CUtensorMap& k, const CUtensorMap& v, int device,
-           cudaStream_t s) {
-  static DevicesReady ready;
-  if (!ready.has(device)) {
-    TS_CUDA_RET(cudaFuncSetAttribute(prefix_kernel<T, D>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem),
-                "prefix attention shared memory");
-    ready.add(device);
-  }
-  prefix_kernel<T, D><<<p.ctas, kThreads, Shape<D>::kSmem, s>>>(p, k, v);
-  TS_CUDA_RET(cudaGetLastError(), "prefix attention launch");
-  return TS_OK;
-}
-
-}  // namespace
-
 bool prefix_geometry_ok(const ts_paged_kv& kv) {
   // a box of whole swizzle groups (eight tokens); strides as tensor maps take them
   if (kv.pages < 1 || std::gcd(kv.block_tokens, int64_t(kPrefixTile)) < 8) return false;
@@ -753,8 +703,8 @@ bool prefix_geometry_ok(const ts_paged_kv& kv) {
 
 int launch_prefix(const PrefixParams& p, int device, cudaStream_t s) {
   CUtensorMap k, v;
-  if (int rc = make_map(&k, p.kv, false, p.piece)) return rc;
-  if (int rc = make_map(&v, p.kv, true, p.piece)) return rc;
+  if (int rc = make_page_map(&k, p.kv, false, p.piece)) return rc;
+  if (int rc = make_page_map(&v, p.kv, true, p.piece)) return rc;
   if (p.kv.dtype == TS_DTYPE_BF16)
     return p.kv.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, k, v, device, s)
                                : launch<__nv_bfloat16, 128>(p, k, v, device, s);

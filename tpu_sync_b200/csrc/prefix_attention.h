@@ -2,6 +2,7 @@
 // generation tensor cores (prefix_attention.cu), as kv_attention.cu calls it.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -57,6 +58,64 @@ __host__ __device__ __forceinline__ int prefix_units(int nt, int units) {
 // tiles reads the prefix too).
 bool prefix_geometry_ok(const ts_paged_kv& kv);
 int launch_prefix(const PrefixParams& p, int device, cudaStream_t s);
+// Tensor map of a layer's K or V pages, as [pages][heads][tokens][D] with the
+// storage's strides: boxes of 64 elements x `piece` tokens of one head and page,
+// in the 128-byte swizzle; the page past the last one loads zeros.
+int make_page_map(CUtensorMap* map, const ts_paged_kv& kv, bool v, int piece);
+
+// Waits on a shared-memory barrier end after so many tries (each is suspended
+// for a while by the hardware): seconds.
+constexpr uint32_t kWaitRounds = 1u << 24;
+
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// A whole warp's wait; false (for all its lanes) when it ran out here or in
+// another part of the CTA, which `gone` says.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
+  bool ok = bar_try(bar, parity);
+  for (uint32_t i = 0; !ok && i < kWaitRounds && !*gone; ++i) ok = bar_try(bar, parity);
+  if (!ok) *gone = 1;
+  return __all_sync(~0u, ok);
+}
+// One lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                       int token, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(token), "r"(head), "r"(page)
+      : "memory");
+}
+// Orders this thread's plain shared-memory accesses before TMA's later ones.
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 
 // Tokens of the shared prefix, cut to what its table holds.
 __device__ __forceinline__ int prefix_tokens(const ts_paged_kv& kv, const ts_attention_args& a,
