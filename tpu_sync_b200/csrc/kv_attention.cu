@@ -610,6 +610,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
         loader.load(p, maps, fill >= kStages ? fill - kStages : fill);
       }
       const bool whole = mask == 0xffffu && t0 + kWarpTokens <= vis_min;
+      constexpr float kSlack = kNt == 4 ? 8.f : 0.f;
       float x[kNt][4];
       bool grew = false;
 #pragma unroll
@@ -625,11 +626,14 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
           }
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) grew = grew || fmaxf(x[nt][e], x[nt][e + 2]) > m[nt][e] + 8.f;
+        for (int e = 0; e < 2; ++e)
+          grew = grew || fmaxf(x[nt][e], x[nt][e + 2]) > m[nt][e] + kSlack;
       }
-      // m is any common reference of a row: it follows the maximum only when
-      // that grew by more than 2^8, so that most tiles need no exchange between
-      // lanes and no rescaling, and no weight passes 2^8.
+      // Lanes compare notes and sums are rescaled only in tiles that raise a
+      // row's maximum.  m may be any common reference: with 32 rows it follows
+      // only by steps of 2^8 (few tiles raise none; 64 x 4000 tokens 287 -> 248
+      // us), with fewer at once, as the largest weight is then exactly 1 and
+      // loses nothing when it is rounded.
       if (__any_sync(~0u, grew)) {
 #pragma unroll
         for (int nt = 0; nt < kNt; ++nt) {
@@ -1128,12 +1132,13 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   Layout w{};
   const int64_t group = a.q_heads / kv.heads;
   const int64_t rows = a.batch * a.new_tokens * a.q_heads;
-  // The smallest tile that holds a KV head's rows: more than 32 rows are read
-  // for in tiles of 32; a walked prefix counts the rows of the whole batch.
+  // The fewest tiles of at most 32 rows, and a KV head's rows spread evenly over
+  // them in eights; a walked prefix counts the rows of the whole batch.
   const bool pre = a.prefix_blocks > 0;
   w.tensor = pre && a.batch * a.new_tokens * group > 32 && prefix_geometry_ok(kv);
-  const int64_t most = (pre && !w.tensor ? a.batch : 1) * a.new_tokens * group;
-  w.rows = most <= 24 ? std::max(1, int(most + 7) / 8) * 8 : 32;
+  const int64_t most = std::max<int64_t>(1, (pre && !w.tensor ? a.batch : 1) * a.new_tokens * group);
+  const int64_t tiles = (most + 31) / 32;
+  w.rows = int(((most + tiles - 1) / tiles + 7) / 8 * 8);
   w.ctas = walk_ctas(int(kv.head_dim)) * sm_count(device);
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
