@@ -322,10 +322,17 @@ PREFIX = [
     (8, 2, 128, 256, False, 1, 700, [4 + i for i in range(70)]),
     (32, 8, 128, 16, False, 1, 6000, [17, 33]),
     # many rows and pages of other than a power of two tokens: loads of 8 and 16 tokens
-    (8, 1, 128, 24, False, 1, 500, [3, 0, 25, 49, 7]),
-    (12, 1, 64, 48, True, 1, 1111, [48, 1, 0, 2, 95, 96, 97]),
-    (10, 1, 128, 136, False, 2, 300, [2, 137, 0, 5, 1]),
-    (40, 1, 128, 20, False, 1, 260, [21, 3]),     # 20 tokens: not in whole groups of 8
+    (8, 1, 128, 24, False, 1, 500, [3, 0, 25, 49, 7] * 4),
+    (12, 1, 64, 48, True, 1, 1111, [48, 1, 0, 2, 95, 96, 97] * 2),
+    (10, 1, 128, 136, False, 2, 300, [2, 137, 0, 5, 1] * 2),
+    (40, 1, 128, 20, False, 1, 260, [21, 3, 0, 1]),     # 20 tokens: not in whole groups of 8
+    # fewer rows, where the walk reads the prefix: 24, 40, 64 and 112 of them
+    (24, 1, 128, 16, False, 1, 1023, [40]),
+    (8, 1, 128, 32, False, 1, 700, [3, 0, 25, 49, 7]),
+    (8, 2, 64, 24, True, 2, 301, [2, 137, 0, 5, 1, 9, 33, 4]),
+    (16, 1, 64, 16, False, 1, 97, [48, 1, 0, 2, 95, 96, 97]),
+    # rows times keys that pass the border: 20 x 30000
+    (20, 1, 128, 16, False, 1, 30000, [40]),
 ]
 
 
@@ -341,7 +348,8 @@ def test_shared_prefix_attention(cuda, case, dt):
                                          err_flag=err)
   assert int(err) == 0
   check(out, lse, q, own, shared, lens, hk, dt)
-  # the length as a device value gives the same bits
+  # the length as a device value gives the same bits (the host then goes by what the table
+  # holds, less than a page more)
   dev = torch.tensor([prefix], dtype=torch.int32, device="cuda")
   again = ops.shared_prefix_attention(kv, q, ptable, dev, table, lens_t)
   assert torch.equal(again, out)
@@ -511,11 +519,12 @@ def test_far_pages(cuda):
   check(out, lse, q, [[k.double(), v.double()]], None, [40], 8, BF)
   out, lse = ops.shared_prefix_attention(kv, q, table[0], 40, table, lens * 0, return_lse=True)
   check(out, lse, q, [[k[:0].double(), v[:0].double()]], [k.double(), v.double()], [0], 8, BF)
-  many = rand(g, 9, 1, 32, 128, dtype=BF)
-  out, lse = ops.shared_prefix_attention(kv, many, table[0], 40, table.repeat(9, 1),
-                                         lens.repeat(9) * 0, return_lse=True)
-  check(out, lse, many, [[k[:0].double(), v[:0].double()]] * 9, [k.double(), v.double()], [0] * 9,
-        8, BF)
+  for count in (9, 40):  # 36 and 160 rows per KV head
+    many = rand(g, count, 1, 32, 128, dtype=BF)
+    out, lse = ops.shared_prefix_attention(kv, many, table[0], 40, table.repeat(count, 1),
+                                           lens.repeat(count) * 0, return_lse=True)
+    check(out, lse, many, [[k[:0].double(), v[:0].double()]] * count, [k.double(), v.double()],
+          [0] * count, 8, BF)
 
 
 def test_other_stream_and_repeatable(cuda):
@@ -547,7 +556,7 @@ def test_other_stream_and_repeatable(cuda):
 def test_calls_from_threads(cuda):
   """Calls of several threads at once, each on its own stream, give the bits of one alone."""
   import threading
-  lens = [70, 0, 333]
+  lens = [70, 0, 333] * 7
   pools, table, lens_t, ptable, q, own, shared = build(16, FP, 16, 2, 64, 16, False, 1, lens, 500)
   kv = ops.PagedKV(*pools)
   want = ops.shared_prefix_attention(kv, q, ptable, 500, table, lens_t)
@@ -581,22 +590,23 @@ from tpu_sync_b200 import ops
 g = torch.Generator(device="cuda").manual_seed(1)
 pages = torch.randn(40, 16, 2, 64, generator=g, device="cuda").half()
 kv = ops.PagedKV(pages, pages.clone())
-q = torch.randn(20, 8, 64, generator=g, device="cuda").half()
+q = torch.randn(40, 8, 64, generator=g, device="cuda").half()
 k = torch.randn(3, 2, 64, generator=g, device="cuda").half()
 slots = torch.tensor([5, 6, 200], device="cuda")
-table = torch.arange(40, device="cuda", dtype=torch.int32).view(20, 2)
-lens = torch.full((20,), 25, device="cuda", dtype=torch.int32)
+table = torch.arange(40, device="cuda", dtype=torch.int32).view(40, 1)
+lens = torch.full((40,), 9, device="cuda", dtype=torch.int32)
+shared = torch.arange(2, device="cuda", dtype=torch.int32)
 torch.cuda.synchronize()
 graph = torch.cuda.CUDAGraph()
 with torch.cuda.graph(graph):
   ops.kv_append(kv, k, k, slots)
   a = ops.paged_attention(kv, q, table, lens)
-  b = ops.shared_prefix_attention(kv, q, table[0], 30, table, lens)
+  b = ops.shared_prefix_attention(kv, q, shared, 30, table, lens)
 graph.replay()
 torch.cuda.synchronize()
 assert torch.equal(kv.k_pages.view(-1, 2, 64)[slots], k)
 assert torch.equal(a, ops.paged_attention(kv, q, table, lens))
-assert torch.equal(b, ops.shared_prefix_attention(kv, q, table[0], 30, table, lens))
+assert torch.equal(b, ops.shared_prefix_attention(kv, q, shared, 30, table, lens))
 """
   root = Path(__file__).resolve().parents[1]
   r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
@@ -606,7 +616,7 @@ assert torch.equal(b, ops.shared_prefix_attention(kv, q, table[0], 30, table, le
 
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_other_device_than_the_current_one(cuda):
-  pools, table, lens_t, ptable, q, own, shared = build(17, BF, 32, 8, 128, 16, False, 1, [90] * 9,
+  pools, table, lens_t, ptable, q, own, shared = build(17, BF, 32, 8, 128, 16, False, 1, [90] * 40,
                                                        300)
   there = lambda t: t.to("cuda:1")
   kv = ops.PagedKV(*[there(p) for p in pools])

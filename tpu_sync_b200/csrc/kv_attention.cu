@@ -14,13 +14,26 @@
 //                 lengths, no empty CTAs for short sequences, the same code
 //                 for one long sequence and for many short ones.  A share that
 //                 cuts an item in two leaves a partial (m, l, acc).
-//   join_kernel   joins partials per query row, in a fixed order.
+//   join kernels  join the partials of a query row, in a fixed order.  They are
+//                 launched early (programmatic dependent launch) and are
+//                 resident beside the walk where registers leave room.
 //
-// A warp owns 16 tokens of each tile (its own cp.async ring, its own softmax
-// statistics and accumulator), so the loop over keys has no CTA barrier; the
+// A warp owns 16 tokens of each tile (its own ring of three stages, its own
+// softmax statistics and sums), so the loop over keys has no CTA barrier; the
 // four warps are joined once per item.  All query heads of a KV head, and all
-// new tokens, are rows of one mma tile: K and V are read once per KV head.
-// Decode is bound by reading K and V from HBM.
+// new tokens, are columns of the same products, up to 32: K and V are read
+// once for them.
+//
+// Bound: decode reads K and V from HBM, 436 us for 2.94 GB (128 sequences of
+// 3001..8192 tokens, 8 KV heads of 128: 6.7 TB/s, all of a plain copy's rate),
+// 91 us for 0.54 GB (64 of 17..4096).  Short batches are bound by chains of
+// latency: about 4 us from the lengths to the first tile, 0.8 us a tile in each
+// CTA, 4 us to the joined rows (one sequence of 8191 tokens 11 us of walk and 4
+// of join).  More than 16 rows are bound by the instructions of the products
+// and the softmax: 64 x 4000 tokens of one KV head 33, 38, 44 and 63 us for 8,
+// 16, 24 and 32 rows (at 32 some registers spill).  mma.sync is used and not
+// tcgen05: eight to 32 rows would fill a fraction of a 128-row tile, and the
+// products are not what bounds the common case.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1128,6 +1141,20 @@ struct Layout {
   uint64_t slots_acc, slots_ml, own_acc, own_ml, pre_acc, pre_ml, tensor_acc, tensor_ml, bytes;
 };
 
+// Whether the prefix goes to the tensor-core kernel rather than the walk, by
+// the length the host knows.  The walk starts faster (17 us a call against 25)
+// and reads K and V once for every 32 rows; measured, walk / tensor cores, us:
+//   16 rows x 8 KV heads: 18 / 26 at 8192 keys, 36 / 41 at 32768
+//   48 rows: 27 / 28 at 8192, 57 / 44 at 32768;  64 rows: 21 / 26, 34 / 28, 76 / 47
+//   128 rows: 30 / 28 at 1000, 53 / 30 at 8192 (1 KV head: 18 / 27, 23 / 26)
+bool prefix_on_tensor_cores(const ts_paged_kv& kv, const ts_attention_args& a) {
+  if (a.prefix_blocks == 0 || !prefix_geometry_ok(kv)) return false;
+  const int64_t rows = a.batch * a.new_tokens * (a.q_heads / kv.heads);
+  const int64_t len = std::min<int64_t>(a.prefix_len, a.prefix_blocks * kv.block_tokens);
+  return rows > 128 || (rows > 16 && rows * len > 400000);
+}
+
+// The workspace's size goes by the shapes alone: it holds either way of a prefix.
 Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) {
   Layout w{};
   const int64_t group = a.q_heads / kv.heads;
@@ -1135,7 +1162,7 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
   // The fewest tiles of at most 32 rows, and a KV head's rows spread evenly over
   // them in eights; a walked prefix counts the rows of the whole batch.
   const bool pre = a.prefix_blocks > 0;
-  w.tensor = pre && a.batch * a.new_tokens * group > 32 && prefix_geometry_ok(kv);
+  w.tensor = prefix_on_tensor_cores(kv, a);
   const int64_t most = std::max<int64_t>(1, (pre && !w.tensor ? a.batch : 1) * a.new_tokens * group);
   const int64_t tiles = (most + 31) / 32;
   w.rows = int(((most + tiles - 1) / tiles + 7) / 8 * 8);
@@ -1146,14 +1173,17 @@ Layout layout_of(const ts_paged_kv& kv, const ts_attention_args& a, int device) 
     at += (n * 4 + 255) / 256 * 256;
     return o;
   };
-  const uint64_t slot_rows = uint64_t(w.ctas) * 2 * w.rows;
+  const uint64_t slot_rows = uint64_t(w.ctas) * 2 * (pre ? 32 : w.rows);
   w.slots_acc = take(slot_rows * kv.head_dim);
   w.slots_ml = take(slot_rows * 2);
   w.own_acc = take(pre ? rows * kv.head_dim : 0);
   w.own_ml = take(pre ? rows * 2 : 0);
   w.pre_acc = take(pre ? rows * kv.head_dim : 0);
   w.pre_ml = take(pre ? rows * 2 : 0);
-  const uint64_t tensor_rows = w.tensor ? uint64_t(sm_count(device)) * 2 * kPrefixRows : 0;
+  const uint64_t tensor_rows =
+      pre && a.batch * a.new_tokens * group > 16 && prefix_geometry_ok(kv)
+          ? uint64_t(sm_count(device)) * 2 * kPrefixRows
+          : 0;
   w.tensor_acc = take(tensor_rows * kv.head_dim);
   w.tensor_ml = take(tensor_rows * 2);
   w.bytes = at;

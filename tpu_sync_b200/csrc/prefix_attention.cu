@@ -31,6 +31,18 @@
 //
 // Every wait is bounded: on running out it raises the flag (value 2), and all
 // roles leave.
+//
+// Bound: 1024 rows x 8 KV heads x 32768 keys x 128 (137 GFLOP) take 124 us, 1.1
+// PFLOP/s: 67% of a large cuBLAS product's burst rate, 80% of its sustained one.
+// A tile pair takes about 3300 cycles where its 32 products need 2050 (and, with
+// 8 KB of operands each, all of shared memory's bandwidth for them): the rest is
+// the chain scores -> softmax (2100 cycles) -> P -> products of each half, which
+// the other half's overlaps only in part, as S and P share TMEM.  Moving a
+// quarter of the exponentials to the multiply-add pipe changed nothing (138 us
+// either way then), so they stay on the special function unit.  One thread
+// issues all products, from descriptors made once: with the descriptors built
+// in a lane-0 branch a product took 130 cycles to issue instead of 65 (176 us
+// against 141).  A unit's fixed cost is about 7 us.
 
 #include <cuda.h>
 #include <cuda_bf16.h>
