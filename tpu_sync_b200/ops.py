@@ -13,7 +13,6 @@ pages and the attention that reads the pages.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import struct
 from typing import List, Optional, Sequence, Tuple, Union
@@ -478,9 +477,13 @@ def _check_index(kv: PagedKV, name: str, t: torch.Tensor, dtype: torch.dtype, di
     raise ValueError(f"{name} must hold {length} entries, got {list(t.shape)}")
 
 
-def _check_grad(*tensors: Optional[torch.Tensor]) -> None:
-  if any(t is not None and t.requires_grad for t in tensors):
-    raise ValueError("an input requires grad: the paged cache operators have no backward pass")
+def _weight_ok(t: torch.Tensor, dtype: torch.dtype, length: int, index: int) -> bool:
+  return (t.shape == (length,) and t.dtype is dtype and t.get_device() == index and
+          t.stride() == (1,))
+
+
+def _no_grad_path() -> ValueError:
+  return ValueError("an input requires grad: the paged cache operators have no backward pass")
 
 
 def _flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
@@ -489,9 +492,6 @@ def _flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
   if err_flag.dtype != torch.int32 or err_flag.device != kv.device or err_flag.numel() < 1:
     raise ValueError("err_flag must be an int32 tensor on the pages' device")
   return err_flag.data_ptr()
-
-
-_HERE = contextlib.nullcontext()
 
 
 def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -539,7 +539,9 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
         positions.shape != (tokens,) or positions.get_device() != index or
         positions.stride() != (1,)):
       _check_index(kv, "positions", positions, torch.int64, 1, tokens)
-    _check_index(kv, "cos_sin", cos_sin, torch.float32, 2, None)
+    if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or
+        cos_sin.get_device() != index or cos_sin.stride(1) != 1):
+      _check_index(kv, "cos_sin", cos_sin, torch.float32, 2, None)
     rows, rotary = cos_sin.shape
     if rows == 0:
       raise ValueError("cos_sin has no rows")
@@ -555,14 +557,20 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
     if q_weight is not None:
       if q is None:
         raise ValueError("q_weight needs q")
-      _check_index(kv, "q_weight", q_weight, w.dtype, 1, dim)
+      if not _weight_ok(q_weight, w.dtype, dim, index):
+        _check_index(kv, "q_weight", q_weight, w.dtype, 1, dim)
       wq = q_weight.data_ptr()
     if k_weight is not None:
-      _check_index(kv, "k_weight", k_weight, w.dtype, 1, dim)
+      if not _weight_ok(k_weight, w.dtype, dim, index):
+        _check_index(kv, "k_weight", k_weight, w.dtype, 1, dim)
       wk = k_weight.data_ptr()
     weight_dtype = _TORCH_TO_TS[w.dtype]
-  if torch.is_grad_enabled():
-    _check_grad(k, v, q, q_weight, k_weight, q_out)
+  if torch.is_grad_enabled() and (
+      k.requires_grad or v.requires_grad or (q is not None and q.requires_grad) or
+      (q_out is not None and q_out.requires_grad) or
+      (q_weight is not None and q_weight.requires_grad) or
+      (k_weight is not None and k_weight.requires_grad)):
+    raise _no_grad_path()
   q_ptr = out_ptr = heads = qt = qh = ot = oh = zero = 0
   if q is not None:
     heads = q.shape[1] if q.dim() == 3 else 0
@@ -623,7 +631,9 @@ def _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, ou
     _check_index(kv, "seq_lens", seq_lens, torch.int32, 1, batch)
   shared = blocks = length = length_ptr = 0
   if prefix_table is not None:
-    _check_index(kv, "prefix_table", prefix_table, torch.int32, 1, None)
+    if (prefix_table.dtype is not torch.int32 or prefix_table.dim() != 1 or
+        prefix_table.get_device() != index or prefix_table.stride(0) != 1):
+      _check_index(kv, "prefix_table", prefix_table, torch.int32, 1, None)
     shared, blocks = prefix_table.data_ptr(), prefix_table.shape[0]
     if isinstance(prefix_len, torch.Tensor):
       if prefix_len.dtype != torch.int32 or prefix_len.device != device or (
@@ -638,44 +648,46 @@ def _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, ou
     _check_heads(kv, "out", out, shape)
     if not out.is_contiguous():
       raise ValueError("out must be contiguous")
-  if torch.is_grad_enabled():
-    _check_grad(q, out)
+  if torch.is_grad_enabled() and (q.requires_grad or (out is not None and out.requires_grad)):
+    raise _no_grad_path()
   lib = _native.lib()
 
-  def pack(out_ptr, lse_ptr):
-    # a dimension of one element is never stepped over: its stride says nothing
-    return _ATTENTION_ARGS.pack(
-        q.data_ptr(), out_ptr, lse_ptr, strides[0] if batch > 1 else 0,
-        strides[1] if new > 1 else 0, strides[-2] if q_heads > 1 else 0, batch, new, q_heads,
-        block_table.data_ptr(), block_table.stride(0) if batch > 1 else 0, block_table.shape[1],
-        seq_lens.data_ptr(), shared, blocks, length, length_ptr,
-        dim ** -0.5 if scale is None else scale, 0)
-
+  # a dimension of one element is never stepped over: its stride says nothing
+  tail = (strides[0] if batch > 1 else 0, strides[1] if new > 1 else 0,
+          strides[-2] if q_heads > 1 else 0, batch, new, q_heads, block_table.data_ptr(),
+          block_table.stride(0) if batch > 1 else 0, block_table.shape[1], seq_lens.data_ptr(),
+          shared, blocks, length, length_ptr, dim ** -0.5 if scale is None else scale, 0)
   # the workspace's size follows from the shapes alone
   key = (batch, new, q_heads, blocks > 0)
   nbytes = kv._workspace.get(key)
   if nbytes is None:
     n = ctypes.c_uint64()
-    _native.check(lib.ts_paged_attention_workspace(index, kv._ref, pack(0, 0), ctypes.byref(n)),
-                  "attention: ")
+    _native.check(lib.ts_paged_attention_workspace(
+        index, kv._ref, _ATTENTION_ARGS.pack(0, 0, 0, *tail), ctypes.byref(n)), "attention: ")
     nbytes = n.value
     if len(kv._workspace) >= 1024:
       kv._workspace.clear()
     kv._workspace[key] = nbytes
   lse = None
-  # what a call allocates belongs to its stream
-  with _HERE if stream is None else torch.cuda.stream(stream):
+  if stream is None:
     if out is None:
       out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if return_lse:
       lse = q.new_empty(shape[:-1], dtype=torch.float32)
     work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-  rc = lib.ts_paged_attention(index, kv._ref,
-                              pack(out.data_ptr(), lse.data_ptr() if return_lse else 0),
-                              work.data_ptr(), nbytes,
-                              0 if err_flag is None else _flag(kv, err_flag),
-                              torch._C._cuda_getCurrentRawStream(index)
-                              if stream is None else stream.cuda_stream)
+    raw = torch._C._cuda_getCurrentRawStream(index)
+  else:
+    with torch.cuda.stream(stream):  # what a call allocates belongs to its stream
+      if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+      if return_lse:
+        lse = q.new_empty(shape[:-1], dtype=torch.float32)
+      work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    raw = stream.cuda_stream
+  args = _ATTENTION_ARGS.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                              *tail)
+  rc = lib.ts_paged_attention(index, kv._ref, args, work.data_ptr(), nbytes,
+                              0 if err_flag is None else _flag(kv, err_flag), raw)
   if rc:
     _native.check(rc, "attention: ")
   return (out, lse) if return_lse else out
