@@ -88,6 +88,7 @@ APPEND = [
     (dict(q_out=4 * BASE), "q itself"), (dict(q_out=6 * BASE + 2), "q itself"),
     (dict(q_out=BASE), "overlap the pages"), (dict(k=2 * BASE + 64), "overlap the pages"),
     (dict(v=BASE - 2), "overlap the pages"),
+    (dict(q_out=6 * BASE, k=6 * BASE), "q itself"), (dict(q_out=6 * BASE, v=6 * BASE), "q itself"),
 ]
 
 

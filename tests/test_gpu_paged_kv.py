@@ -753,6 +753,8 @@ def test_refusals_on_the_device(cuda):
       dict(q=q3, q_out=q3[:, :4]), dict(q=q3, q_out=q3[:1].expand(3, 8, 128)),
       dict(k=kp[0, :3]), dict(q=q3, q_weight=w, eps=-1.0), dict(q=q3, q_weight=w, eps=math.nan),
       dict(k=k.clone().requires_grad_()), dict(k_weight=w.clone().requires_grad_()),
+      dict(positions=slots, cos_sin=cs.clone().requires_grad_()),
+      dict(k=q3[:, :2], q=q3, q_out=q3),
   ]
   for b in bad:
     with pytest.raises((ValueError, _native.NativeError)):

@@ -552,8 +552,11 @@ extern "C" int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_appen
     const bool in_place = a.q == a.q_out && a.q_token_stride == a.q_out_token_stride &&
                           a.q_head_stride == a.q_out_head_stride;
     // Projections in one buffer interleave rows: q_out inside that buffer is
-    // told from an overlap only when it is q itself.
-    if (!in_place && (eo.meets(eq) || eo.meets(ek) || eo.meets(ev)))
+    // told from an overlap only when it is q itself; q that is also k or v would
+    // be overwritten while other warps read it as those.
+    const bool apart = in_place ? a.q != a.k && a.q != a.v
+                                : !(eo.meets(eq) || eo.meets(ek) || eo.meets(ev));
+    if (!apart)
       return set_error(TS_INVALID_ARGUMENT, "q_out must be q itself or apart from the new tokens");
   }
   for (int i = 0; i < 2; ++i) {

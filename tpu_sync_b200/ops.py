@@ -512,7 +512,7 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
   head by row positions[t] (int64), pairs (i, i + rotary/2), or (2i, 2i+1) if
   `interleaved`.  q_weight / k_weight [head_dim] (the pages' dtype or float32)
   apply x * weight / sqrt(mean(x^2) + eps) to every query / key head before the
-  rotation.  q_out may be q itself; its padding rows stay as they were (a new
+  rotation.  q_out may be q itself (not k or v); its padding rows stay as they were (a new
   one has zeros there).
 
   The slots of one call are distinct: where two tokens name one slot, it is not
@@ -568,6 +568,7 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
   if torch.is_grad_enabled() and (
       k.requires_grad or v.requires_grad or (q is not None and q.requires_grad) or
       (q_out is not None and q_out.requires_grad) or
+      (cos_sin is not None and cos_sin.requires_grad) or
       (q_weight is not None and q_weight.requires_grad) or
       (k_weight is not None and k_weight.requires_grad)):
     raise _no_grad_path()
