@@ -770,3 +770,89 @@ def test_refusals_on_the_device(cuda):
   spread = kp[:1].expand(4, 16, 2, 128)
   with pytest.raises(_native.NativeError):
     ops.paged_attention(ops.PagedKV(spread, kp), q, table, lens)
+
+
+# -- values that a row does not see --------------------------------------------
+
+
+def poison(seed, pools, table, lens, own, n, bt, major):
+  """Infinities and NaN in V of some of the last n tokens of each sequence: single elements, and
+  the whole head vector of the last one.  Keeps the pages and the 64-bit copies alike."""
+  g = torch.Generator().manual_seed(seed)
+  v = pools[1].transpose(1, 2) if major else pools[1]
+  for i, length in enumerate(lens):
+    for t in range(max(0, length - n + 1), length):
+      if t < length - 1 and torch.rand((), generator=g) < 0.5:
+        continue
+      value = (math.inf, -math.inf, math.nan)[(i + t) % 3]
+      at = slice(None) if t == length - 1 and i % 2 else int(
+          torch.randint(0, v.shape[3], (), generator=g))
+      v[int(table[i, t // bt]), t % bt, :, at] = value
+      own[i][1][t, :, at] = value
+
+
+def check_seen(got, lse, q, own, shared, lens, hk, dt):
+  """check() of rows whose own visible V may not be finite: those elements are not finite, all
+  others keep the bound."""
+  b, n, hq, d = q.shape
+  g = hq // hk
+  for i in range(b):
+    for j in range(n):
+      seen = max(0, lens[i] - n + 1 + j)
+      k, v = own[i][0][:seen], own[i][1][:seen]
+      if shared is not None:
+        k, v = torch.cat([shared[0], k]), torch.cat([shared[1], v])
+      if k.shape[0] == 0:
+        assert (got[i, j] == 0).all() and (lse[i, j] == -math.inf).all(), (i, j)
+        continue
+      x = torch.einsum("hgd,thd->hgt", q[i, j].double().view(hk, g, d), k) * d ** -0.5
+      p = torch.softmax(x, -1)
+      fine = torch.isfinite(v).all(0).repeat_interleave(g, 0)  # [hq, d]
+      v = torch.where(torch.isfinite(v), v, 0.0)
+      want = torch.einsum("hgt,thd->hgd", p, v).reshape(hq, d)
+      size = torch.einsum("hgt,thd->hgd", p, v.abs()).reshape(hq, d)
+      tol = U[dt] * (size + want.abs()) + 2.0 ** -15 * size
+      if dt == FP:
+        tol += 2.0 ** -25 * v.abs().sum(0).repeat_interleave(g, 0)
+      off = (got[i, j].double() - want).abs()
+      assert bool((off <= tol)[fine].all()), (i, j)
+      assert not bool(torch.isfinite(got[i, j])[~fine].any()), (i, j)
+      assert float((lse[i, j].double() - torch.logsumexp(x, -1).view(hq)).abs().max()) <= 2.0 ** -15
+
+
+UNSEEN = [
+    # q heads, kv heads, d, block tokens, head major, new tokens, lengths: 4, 12, 24, 32 and 80
+    # rows a KV head, pages that are loaded by TMA and others
+    (4, 2, 128, 16, False, 2, [1, 2, 3, 16, 17, 64, 65, 300]),
+    (4, 2, 64, 5, False, 2, [1, 2, 17, 64, 65]),
+    (8, 2, 128, 64, True, 3, [0, 1, 2, 3, 18, 65, 130]),
+    (8, 1, 64, 16, False, 3, [1, 3, 63, 64, 65, 66, 1000]),
+    (8, 1, 128, 24, False, 3, [2, 66, 191]),
+    (8, 2, 128, 16, False, 8, [3, 8, 20, 70, 135]),
+    (4, 1, 64, 48, True, 8, [1, 7, 9, 100]),
+    (2, 1, 128, 16, False, 40, [12, 40, 100]),
+    (2, 1, 64, 3, False, 40, [39, 77]),
+]
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("case", UNSEEN, ids=str)
+def test_values_of_later_drafts_do_not_reach_earlier_ones(cuda, case, dt):
+  hq, hk, d, bt, major, n, lens = case
+  pools, table, lens_t, _, q, own, _ = build(21, dt, hq, hk, d, bt, major, n, lens)
+  poison(22, pools, table, lens, own, n, bt, major)
+  out, lse = ops.paged_attention(ops.PagedKV(*pools, head_major=major), q, table, lens_t,
+                                 return_lse=True)
+  check_seen(out, lse, q, own, None, lens, hk, dt)
+
+
+@pytest.mark.parametrize("hq,hk,prefix,count", [(8, 2, 100, 5), (8, 1, 600, 30)],
+                         ids=["few", "many"])
+def test_values_of_later_drafts_behind_a_prefix(cuda, hq, hk, prefix, count):
+  lens = [(13 * i) % 140 for i in range(count)]
+  pools, table, lens_t, ptable, q, own, shared = build(23, BF, hq, hk, 128, 16, False, 3, lens,
+                                                       prefix)
+  poison(24, pools, table, lens, own, 3, 16, False)
+  out, lse = ops.shared_prefix_attention(ops.PagedKV(*pools), q, ptable, prefix, table, lens_t,
+                                         return_lse=True)
+  check_seen(out, lse, q, own, shared, lens, hk, BF)

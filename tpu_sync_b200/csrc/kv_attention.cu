@@ -303,6 +303,9 @@ struct Ops<__nv_bfloat16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ float2 unpack(uint32_t x) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+  }
 };
 template <>
 struct Ops<__half> {
@@ -317,6 +320,9 @@ struct Ops<__half> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
   }
 };
 
@@ -338,7 +344,7 @@ template <int D>
 __host__ __device__ constexpr int stage_bytes() { return 2 * kWarpTokens * D * 2; }  // K and V of a warp's tokens
 template <int D>
 __host__ __device__ constexpr int walk_smem() {
-  return kWarps * kStages * (stage_bytes<D>() + 12) + 4 + 1024;
+  return kWarps * kStages * (stage_bytes<D>() + 12) + 8 + 1024;
 }
 
 // Row r of an item: sequence b's new token j, query head g of the KV head.
@@ -483,6 +489,132 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
+// kPer elements (8 or 4, aligned to as many) in 32 bits.
+template <typename T, int kPer>
+__device__ __forceinline__ void load_f32(const T* src, float* f) {
+  uint32_t w[kPer / 2];
+  if constexpr (kPer == 8)
+    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
+  else
+    *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i) {
+    const float2 x = Ops<T>::unpack(w[i]);
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
+  }
+}
+template <int kPer>
+__device__ __forceinline__ bool all_finite(const float* f) {
+  float zero = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) zero = fmaf(f[i], 0.f, zero);
+  return zero == 0.f;
+}
+
+// Writes elements [at, at + D / 16) of row r of the item's row tile: the result
+// itself where this CTA did the whole row, else its partial.
+template <typename T, int D, int kRows>
+__device__ __forceinline__ void put_row(const WalkParams& p, const Cursor& c, int r, int at,
+                                        const float* o, float m, float l) {
+  constexpr int kPer = D / 16;
+  const bool own = c.b < p.a.batch;
+  const Row q = row_of(p, c.b, c.rt * kRows + r);
+  const int64_t out_row = (int64_t(q.b) * p.a.new_tokens + q.j) * p.a.q_heads +
+                          c.head * p.group + q.g;
+  const bool complete = c.tile == 0 && c.end == c.nt;
+  if (complete && own && p.a.prefix_blocks == 0) {
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T* out = reinterpret_cast<T*>(p.a.out) + out_row * D + at;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4)
+      *reinterpret_cast<uint2*>(out + i) =
+          make_uint2(Ops<T>::pack(o[i] * inv, o[i + 1] * inv),
+                     Ops<T>::pack(o[i + 2] * inv, o[i + 3] * inv));
+    if (p.a.lse && at == 0)
+      reinterpret_cast<float*>(p.a.lse)[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    return;
+  }
+  float *da, *dm;
+  if (complete) {
+    da = (own ? p.own_acc : p.pre_acc) + out_row * D;
+    dm = (own ? p.own_ml : p.pre_ml) + out_row * 2;
+  } else {
+    const int64_t slot = (int64_t(blockIdx.x) * 2 + (c.tile == 0 ? 1 : 0)) * kRows + r;
+    da = p.slots_acc + slot * D;
+    dm = p.slots_ml + slot * 2;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; i += 4)
+    *reinterpret_cast<float4*>(da + at + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+  if (at == 0) *reinterpret_cast<float2*>(dm) = make_float2(m, l);
+}
+
+// The products give tokens that a row does not see (later drafts) a weight of 0,
+// and 0 times an infinity or a NaN in their V is NaN.  Where a CTA of the walk
+// met sums that are not finite, this computes all rows of its share again, in 32
+// bits, that have such a neighbour, from what they see; 16 threads a row, the
+// ones that wrote it.  Only those batches pay for it (the others under 1%: 64 x
+// 4000 tokens of 32 rows 60.3 -> 60.4 us); a look at V of partly seen tiles in
+// the walk's loop cost walks of 16 and more rows 5 to 9%.
+template <typename T, int D, int kRows>
+__device__ __forceinline__ void redo_rows(const WalkParams& p) {
+  constexpr int kPer = D / 16;
+  const unsigned lanes = 0xffffu << (threadIdx.x & 16);  // of this thread's row
+  const int at = (threadIdx.x & 15) * kPer, bt = int(p.kv.block_tokens);
+  for (Cursor c = start_cursor(p); !c.done() && c.b < p.a.batch; c.next_item(p)) {
+    const int32_t* table =
+        reinterpret_cast<const int32_t*>(p.a.block_table) + c.b * p.a.block_table_stride;
+    const int tile0 = c.tile * kTile, last = min(c.len, c.end * kTile);
+    // elements [at, at + kPer) of K or V of a token; false where its page is none
+    auto load = [&](bool v, int t, float* f) {
+      const int64_t page = table[t / bt], off = t % bt;
+      if (page < 0 || page >= p.kv.pages) return false;
+      load_f32<T, kPer>(
+          reinterpret_cast<const T*>(v ? p.kv.v_ptr : p.kv.k_ptr) + at +
+              page * (v ? p.kv.v_page_stride : p.kv.k_page_stride) +
+              off * (v ? p.kv.v_token_stride : p.kv.k_token_stride) +
+              c.head * (v ? p.kv.v_head_stride : p.kv.k_head_stride),
+          f);
+      return true;
+    };
+#pragma unroll 1
+    for (int r = threadIdx.x >> 4; r < min(kRows, p.rows_own - c.rt * kRows); r += 8) {
+      const Row q = row_of(p, c.b, c.rt * kRows + r);
+      const int seen = min(last, c.len - int(p.a.new_tokens) + 1 + q.j);
+      bool hidden = false;
+#pragma unroll 1
+      for (int t = max(seen, tile0); t < last && !hidden; ++t) {
+        float v[kPer];
+        hidden = __any_sync(lanes, load(true, t, v) && !all_finite<kPer>(v));
+      }
+      if (!hidden) continue;
+      float qf[kPer], o[kPer] = {}, m = -INFINITY, l = 0.f;
+      load_f32<T, kPer>(reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
+                            q.j * p.a.q_token_stride +
+                            (c.head * p.group + q.g) * p.a.q_head_stride + at,
+                        qf);
+#pragma unroll 1
+      for (int t = tile0; t < seen; ++t) {
+        float k[kPer], v[kPer], x = 0.f;
+        if (!load(false, t, k) || !load(true, t, v)) continue;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x = fmaf(qf[i], k[i], x);
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1) x += __shfl_xor_sync(lanes, x, s);
+        x *= p.scale_log2;
+        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.f : top;
+        const float f = ex2(m - base), w = ex2(x - base);
+        m = top;
+        l = fmaf(l, f, w);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], f, w * v[i]);
+      }
+      put_row<T, D, kRows>(p, c, r, at, o, m, l);
+    }
+  }
+}
+
 // The walk over 8 kNt query rows of a KV head at a time.  The tokens are the
 // rows of the products and the queries their columns, S^T = K Q^T and
 // O^T = V^T P^T: K and V fragments are read from shared memory once for all
@@ -505,12 +637,13 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
   const uint32_t bars = smem_u32(ctl) + warp * kStages * 8;
   uint32_t* masks = reinterpret_cast<uint32_t*>(ctl + kWarps * kStages * 8) + warp * kStages;
   volatile int* gone = reinterpret_cast<volatile int*>(ctl + kWarps * kStages * 12);
+  volatile int* odd = gone + 1;  // sums that are not finite were met
+  if (threadIdx.x == 0) *gone = *odd = 0;
   if (kTma) {
     if (lane < kStages) bar_init(bars + 8 * lane, 1);
-    if (threadIdx.x == 0) *gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncthreads();
   }
+  __syncthreads();
 
   // Lets the join take SMs as they have room.  With a prefix kernel before it,
   // this one may itself run early: it reads nothing that kernel writes, and
@@ -555,8 +688,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
   if (!cu.done()) load_queries(cu);
 
   while (!cu.done()) {
-    const bool own = cu.b < p.a.batch;
-    const int n_rows = own ? p.rows_own : p.rows_pre;
+    const int n_rows = cu.b < p.a.batch ? p.rows_own : p.rows_pre;
     // acc[.][i]: elements 16 i + g and 16 i + g + 8 of rows 2 tg and 2 tg + 1
     float acc[kNt][D / 16][4];
     float m[kNt][2], l[kNt][2];
@@ -764,45 +896,15 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
             o[i + 3] += v.w * f;
           }
         }
-        const Row q = row_of(p, cu.b, row);
-        const int64_t out_row = (int64_t(q.b) * p.a.new_tokens + q.j) * p.a.q_heads +
-                                cu.head * p.group + q.g;
-        const bool complete = cu.tile == 0 && cu.end == cu.nt;
-        if (complete && own && p.a.prefix_blocks == 0) {
-          // the whole row: the result itself
-          const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-          T* out = reinterpret_cast<T*>(p.a.out) + out_row * D + at;
-#pragma unroll
-          for (int i = 0; i < kPer; i += 4)
-            *reinterpret_cast<uint2*>(out + i) =
-                make_uint2(Ops<T>::pack(o[i] * inv, o[i + 1] * inv),
-                           Ops<T>::pack(o[i + 2] * inv, o[i + 3] * inv));
-          if (p.a.lse && at == 0)
-            reinterpret_cast<float*>(p.a.lse)[out_row] =
-                sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
-        } else {
-          float *da, *dm;
-          if (complete) {
-            da = (own ? p.own_acc : p.pre_acc) + out_row * D;
-            dm = (own ? p.own_ml : p.pre_ml) + out_row * 2;
-          } else {
-            const int64_t slot = (int64_t(blockIdx.x) * 2 + (cu.tile == 0 ? 1 : 0)) * kRows +
-                                 nt * 8 + rl;
-            da = p.slots_acc + slot * D;
-            dm = p.slots_ml + slot * 2;
-          }
-#pragma unroll
-          for (int i = 0; i < kPer; i += 4)
-            *reinterpret_cast<float4*>(da + at + i) =
-                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          if (at == 0) *reinterpret_cast<float2*>(dm) = make_float2(mx, sum);
-        }
+        put_row<T, D, kRows>(p, cu, row0 - cu.rt * kRows + rl, at, o, mx, sum);
+        if (!all_finite<kPer>(o)) *odd = 1;
       }
     }
     if (kTma) fence_async();
     __syncthreads();  // the parts have been read: the stages may be refilled
     cu = next;
   }
+  if (p.a.new_tokens > 1 && *odd) redo_rows<T, D, kRows>(p);
   if constexpr (kTma) {
     if (*gone) {
       // loads still in flight land before their shared memory is given back
