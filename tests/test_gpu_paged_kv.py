@@ -18,6 +18,7 @@ Whatever the operators must not read (pages of no table, tokens past a length,
 unused table entries) is NaN or out of range.
 """
 
+import ctypes
 import math
 import subprocess
 import sys
@@ -856,3 +857,47 @@ def test_values_of_later_drafts_behind_a_prefix(cuda, hq, hk, prefix, count):
   out, lse = ops.shared_prefix_attention(ops.PagedKV(*pools), q, ptable, prefix, table, lens_t,
                                          return_lse=True)
   check_seen(out, lse, q, own, shared, lens, hk, BF)
+
+
+# -- the flag -------------------------------------------------------------------
+
+
+def test_a_flag_of_two_stays(cuda):
+  """2 (the result is not valid) is not lowered to 1 by anything that is left out later."""
+  lens = [60] * 40
+  pools, table, lens_t, ptable, q, own, shared = build(31, BF, 8, 1, 128, 16, False, 1, lens, 300)
+  kv = ops.PagedKV(*pools)
+  err = torch.full((1,), 2, dtype=torch.int32, device="cuda")
+  k = torch.zeros(3, 1, 128, dtype=BF, device="cuda")
+  ops.kv_append(kv, k, k, torch.tensor([2 ** 40, 2 ** 41, -1], device="cuda"), err_flag=err)
+  assert int(err) == 2
+  bad, short = table.clone(), table[:, :2].contiguous()
+  bad[:, 1] = -1
+  pbad = ptable.clone()
+  pbad[::3] = 2 ** 31 - 1
+  long = torch.tensor([10000], dtype=torch.int32, device="cuda")
+  for t, p, n in ((bad, ptable, 300), (short, ptable, 300), (table, pbad, 300),
+                  (table, ptable, long)):
+    ops.paged_attention(kv, q, t, lens_t, err_flag=err)
+    ops.shared_prefix_attention(kv, q[:3], p, n, t[:3], lens_t[:3], err_flag=err)  # by the walk
+    ops.shared_prefix_attention(kv, q, p, n, t, lens_t, err_flag=err)
+    assert int(err) == 2
+
+
+def test_flag_in_mapped_host_memory(cuda):
+  """The C entries take a flag in host memory that the device sees."""
+  kp = torch.zeros(4, 16, 2, 64, dtype=BF, device="cuda")
+  kv = ops.PagedKV(kp, kp.clone())
+  k = torch.zeros(2, 2, 64, dtype=BF, device="cuda")
+  slots = torch.tensor([1, 64], device="cuda")
+  flag = torch.zeros(1, dtype=torch.int32).pin_memory()
+  args = _native.KvAppendArgs(k=k.data_ptr(), v=k.data_ptr(), k_token_stride=128,
+                              k_head_stride=64, v_token_stride=128, v_head_stride=64, tokens=2,
+                              slots=slots.data_ptr())
+  torch.cuda.synchronize()
+  for was, now in ((0, 1), (2, 2)):
+    flag[0] = was
+    assert _native.lib().ts_kv_append(0, kv._ref, ctypes.byref(args), flag.data_ptr(),
+                                      None) == _native.OK
+    torch.cuda.synchronize()
+    assert int(flag) == now

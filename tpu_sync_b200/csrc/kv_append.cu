@@ -60,7 +60,7 @@ __device__ __forceinline__ bool token_place(const AppendParams& p, int64_t t, bo
   const int64_t pg = slot <= UINT32_MAX ? int64_t(uint32_t(slot) / uint32_t(p.kv.block_tokens))
                                         : slot / p.kv.block_tokens;
   if (pg >= p.kv.pages || (rot && (*pos < 0 || *pos >= p.a.max_position))) {
-    if (p.err != nullptr) *reinterpret_cast<volatile int*>(p.err) = 1;
+    flag_left_out(p.err);
     return false;
   }
   *page = pg;

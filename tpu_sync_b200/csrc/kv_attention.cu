@@ -85,10 +85,6 @@ struct WalkParams {
   float* tensor_ml;
 };
 
-__device__ __forceinline__ void raise(int* err) {
-  if (err != nullptr) *reinterpret_cast<volatile int*>(err) = 1;
-}
-
 // Tokens a sequence (b < batch) or the prefix (b == batch) holds, cut to what
 // its table holds.
 __device__ __forceinline__ int tokens_of(const WalkParams& p, int64_t b, bool* bad) {
@@ -186,7 +182,7 @@ struct Lengths {
       sum += cost_of(p, i < p.a.batch, tokens_of(p, i, &now));
       bad = bad || now;
     }
-    if (flag && bad) raise(p.err);
+    if (flag && bad) flag_left_out(p.err);
     const int total = warp_sum(sum);
     return Cut(total, total <= p.beside_units ? p.beside : p.ctas);
   }
@@ -423,7 +419,7 @@ struct Loader {
         hold(p, blk, 1);
         page = __shfl_sync(~0u, entry, blk - window);
         if (page < 0 || page >= p.kv.pages) {
-          raise(p.err);
+          flag_left_out(p.err);
           count = 0;
         }
       }
@@ -455,7 +451,7 @@ struct Loader {
       hold(p, __shfl_sync(~0u, blk, 0), kWarpTokens);  // 16 tokens touch at most 16 entries
       const int page = __shfl_sync(~0u, entry, blk - window);
       if (ok && (page < 0 || page >= p.kv.pages)) {
-        raise(p.err);
+        flag_left_out(p.err);
         ok = false;
       }
       const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
@@ -908,7 +904,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
   if constexpr (kTma) {
     if (*gone) {
       // loads still in flight land before their shared memory is given back
-      if (lane == 0 && p.err) *reinterpret_cast<volatile int*>(p.err) = 2;
+      if (lane == 0) flag_not_valid(p.err);
       for (int i = 0; i < 100; ++i) __nanosleep(100000);
     }
   } else {

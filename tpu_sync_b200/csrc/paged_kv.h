@@ -26,6 +26,16 @@ class DevicesReady {
   std::atomic<uint64_t> mask_{0};
 };
 
+// The caller's flag (may be null, may be host-mapped): 1, a token was left out
+// or a length cut; 2, a kernel gave up waiting and the result is not valid,
+// which a later 1 must not hide.
+__device__ __forceinline__ void flag_left_out(int* err) {
+  if (err != nullptr) atomicCAS(err, 0, 1);
+}
+__device__ __forceinline__ void flag_not_valid(int* err) {
+  if (err != nullptr) atomicExch(err, 2);
+}
+
 // Address range [lo, hi) of a strided tensor of 2-byte elements, for the
 // overlap checks; empty for a tensor without elements.
 struct Extent {

@@ -252,8 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Shares shares{};
   shares.nt = (len + kPrefixTile - 1) / kPrefixTile;
   const Cut cut(prefix_units(shares.nt, p.row_tiles * heads), p.ctas);
-  if (bad && blockIdx.x == 0 && threadIdx.x == 0 && p.err)
-    *reinterpret_cast<volatile int*>(p.err) = 1;
+  if (bad && blockIdx.x == 0 && threadIdx.x == 0) flag_left_out(p.err);
   if (blockIdx.x >= cut.ctas) return;
   shares.lo = cut.start(blockIdx.x);
   shares.hi = cut.start(blockIdx.x + 1);
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (page < 0 || page > p.kv.pages ||
               (page == p.kv.pages && lane < pieces &&
                (seg.tile + j) * kPrefixTile + lane * p.piece < len)) {
-            if (p.err) *reinterpret_cast<volatile int*>(p.err) = 1;
+            flag_left_out(p.err);
             page = int(p.kv.pages);
           }
           int next_off = 0, next = 0;
@@ -635,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (*gone) {
     // a wait ran out: give copies and products in flight time to land before
     // the shared memory and TMEM they target are given back
-    if (threadIdx.x == 0 && p.err) *reinterpret_cast<volatile int*>(p.err) = 2;
+    if (threadIdx.x == 0) flag_not_valid(p.err);
     for (int i = 0; i < 100; ++i) __nanosleep(100000);
     __syncthreads();
   }
