@@ -746,7 +746,8 @@ TS_API int ts_paged_attention_workspace(int device, const ts_paged_kv* kv,
  * out, lengths are cut to what their table holds, and either sets *err_flag
  * (device or host-mapped int, may be NULL) to 1; 2 says that a kernel gave up
  * waiting for its own loads (its waits are bounded) and the result is not
- * valid; a flag of 2 stays 2.  What lies in pages past a length is never used
+ * valid: the rows it worked on are NaN, with or without a flag.  A flag of 2
+ * stays 2.  What lies in pages past a length is never used
  * (it may be NaN), and no query depends on a token it does not see (a later
  * draft's V may be infinite or NaN).  head_dim is 64 or 128. */
 TS_API int ts_paged_attention(int device, const ts_paged_kv* kv, const ts_attention_args* args,

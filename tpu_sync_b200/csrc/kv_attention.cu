@@ -892,6 +892,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
             o[i + 3] += v.w * f;
           }
         }
+        if (kTma && *gone) sum = NAN;  // of tiles that did not come: so is the row
         put_row<T, D, kRows>(p, cu, row0 - cu.rt * kRows + rl, at, o, mx, sum);
         if (!all_finite<kPer>(o)) *odd = 1;
       }

@@ -285,6 +285,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int32_t* table = reinterpret_cast<const int32_t*>(p.a.prefix_table);
   const int bt = int(p.kv.block_tokens);
   Segment seg;
+  // Writes a softmax thread's row of statistics; its place among the whole rows
+  // or the slots, -1 past the last row.
+  auto put_statistics = [&](const Segment& s, float m, float l) {
+    const int head = s.unit % heads, row = s.unit / heads * kPrefixRows + int(threadIdx.x);
+    if (row >= p.rows) return int64_t(-1);
+    const int tok = int(uint32_t(row) / uint32_t(p.group));
+    const bool whole = s.count == shares.nt;
+    const int64_t to = whole ? tok * p.a.q_heads + head * p.group + row - tok * p.group
+                             : (int64_t(blockIdx.x) * 2 + (s.tile == 0 ? 1 : 0)) * kPrefixRows +
+                                   int(threadIdx.x);
+    *reinterpret_cast<float2*>((whole ? p.whole_ml : p.slots_ml) + to * 2) = make_float2(m, l);
+    return to;
+  };
 
   // The softmax warps hold 128 scores each; the loading and issuing warpgroup
   // gives up registers for them: 2 x 128 x 208 + 128 x 88 = 384 x 168.
@@ -585,17 +598,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_after();
       // The rows' partials: turned in shared memory (the queries' place, which
       // the products are done with), so that eight lanes write 128 bytes of a row.
-      const int row = row0 + r;
-      int64_t to_row = -1;  // first element of this lane's row
       const bool whole = seg.count == shares.nt;
-      if (row < p.rows) {
-        const int tok = int(uint32_t(row) / uint32_t(p.group));
-        to_row = whole ? tok * p.a.q_heads + head * p.group + row - tok * p.group
-                       : (int64_t(blockIdx.x) * 2 + (seg.tile == 0 ? 1 : 0)) * kPrefixRows +
-                             x * 128 + r;
-        *reinterpret_cast<float2*>((whole ? p.whole_ml : p.slots_ml) + to_row * 2) =
-            make_float2(m, l);
-      }
+      const int64_t to_row = put_statistics(seg, m, l);
       float* acc = whole ? p.whole_acc : p.slots_acc;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -636,6 +640,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the shared memory and TMEM they target are given back
     if (threadIdx.x == 0) flag_not_valid(p.err);
     for (int i = 0; i < 100; ++i) __nanosleep(100000);
+    // no row of this CTA's share passes for a result
+    if (warp < 8) {
+      shares.lo = cut.start(blockIdx.x);
+      while (shares.next(&seg)) put_statistics(seg, -INFINITY, NAN);
+    }
     __syncthreads();
   }
   __syncwarp();

@@ -713,7 +713,8 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, block_table: torch.Tensor,
 
   Tokens of a table entry outside the pages are left out, a length is cut to
   what its table row holds, and either sets err_flag (int32, on the device) to
-  1 (2: a kernel gave up waiting for its own loads, the result is not valid).
+  1 (2: a kernel gave up waiting for its own loads, the result is not valid and
+  the rows it worked on are NaN).
   Nothing is read back: lengths and tables may change between replays of a
   captured call.
   """
