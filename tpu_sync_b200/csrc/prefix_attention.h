@@ -63,9 +63,9 @@ int launch_prefix(const PrefixParams& p, int device, cudaStream_t s);
 // in the 128-byte swizzle; the page past the last one loads zeros.
 int make_page_map(CUtensorMap* map, const ts_paged_kv& kv, bool v, int piece);
 
-// Waits on a shared-memory barrier end after so many tries (each is suspended
-// for a while by the hardware): seconds.
-constexpr uint32_t kWaitRounds = 1u << 24;
+// Waits on a shared-memory barrier end after so many tries: about 2 s (the
+// hardware suspends one that fails for 3.95 us).
+constexpr uint32_t kWaitRounds = 1u << 19;
 
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
