@@ -672,8 +672,8 @@ typedef struct ts_paged_kv {
   int32_t pad_;
 } ts_paged_kv;
 
-/* New tokens of ts_kv_append.  All pointers are device addresses; strides
- * count elements, the last dimension is contiguous. */
+/* New tokens of ts_kv_append.  All pointers are device addresses, aligned to
+ * their elements; strides count elements, the last dimension is contiguous. */
 typedef struct ts_kv_append_args {
   uint64_t k, v;       /* [tokens, heads, head_dim], the storages' dtype */
   uint64_t q;          /* [tokens, q_heads, head_dim], or 0: no queries */
@@ -708,7 +708,8 @@ typedef struct ts_kv_append_args {
 TS_API int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_append_args* args,
                         int* err_flag, void* stream);
 
-/* Queries of ts_paged_attention (device addresses, strides in elements). */
+/* Queries of ts_paged_attention (device addresses, strides in elements).  q, out
+ * and the pages are aligned to 16 bytes, the others to their elements. */
 typedef struct ts_attention_args {
   uint64_t q;           /* [batch, new_tokens, q_heads, head_dim], the storages' dtype */
   uint64_t out;         /* the same shape, contiguous */

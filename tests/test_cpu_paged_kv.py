@@ -163,3 +163,36 @@ def test_wrappers_need_cuda_tensors():
   t = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
   with pytest.raises(ValueError, match="CUDA"):
     ops.PagedKV(t, t)
+
+
+# Addresses that are not aligned to their elements would be misaligned accesses.
+UNALIGNED_APPEND = [
+    dict(k=4 * BASE + 1), dict(v=5 * BASE + 1), dict(q=6 * BASE + 1), dict(q_out=7 * BASE + 1),
+    dict(slots=8 * BASE + 4), dict(positions=9 * BASE + 4), dict(cos_sin=10 * BASE + 2),
+    dict(q_weight=11 * BASE + 2), dict(k_weight=12 * BASE + 2),
+    dict(k_weight=12 * BASE + 1, weight_dtype=_native.DTYPE_BF16),
+]
+UNALIGNED_ATTENTION = [
+    dict(lse=6 * BASE + 2), dict(block_table=7 * BASE + 1), dict(seq_lens=8 * BASE + 2),
+    dict(prefix_table=9 * BASE + 2), dict(prefix_len_dev=10 * BASE + 3),
+]
+
+
+def test_unaligned_addresses_are_refused():
+  for over in UNALIGNED_APPEND:
+    assert append(kv(), append_args(**over)) == _native.INVALID_ARGUMENT, over
+    assert "aligned" in _native.last_error()
+  for over in UNALIGNED_ATTENTION:
+    assert attend(kv(), attention_args(**over)) == _native.INVALID_ARGUMENT, over
+    assert "aligned" in _native.last_error()
+  for over in (dict(k_ptr=BASE + 1), dict(v_ptr=2 * BASE + 1)):
+    for rc in (append(kv(**over), append_args()), attend(kv(**over), attention_args())):
+      assert rc == _native.INVALID_ARGUMENT
+      assert "aligned" in _native.last_error()
+  lib, flag = _native.lib(), 13 * BASE + 2
+  assert lib.ts_kv_append(0, ctypes.byref(kv()), ctypes.byref(append_args()), flag,
+                          None) == _native.INVALID_ARGUMENT
+  assert "aligned" in _native.last_error()
+  assert lib.ts_paged_attention(0, ctypes.byref(kv()), ctypes.byref(attention_args()), 13 * BASE,
+                                1 << 40, flag, None) == _native.INVALID_ARGUMENT
+  assert "aligned" in _native.last_error()

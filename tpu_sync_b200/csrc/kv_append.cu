@@ -487,6 +487,8 @@ int check_paged_kv(const ts_paged_kv* kv) {
     return set_error(TS_INVALID_ARGUMENT, "page geometry too large");
   if (kv->pages > 0 && (!kv->k_ptr || !kv->v_ptr))
     return set_error(TS_INVALID_ARGUMENT, "null pointer argument");
+  if ((kv->k_ptr | kv->v_ptr) % 2)
+    return set_error(TS_INVALID_ARGUMENT, "pages are not aligned to their elements");
   // no element of the pages at two indexes
   for (int i = 0; i < 2; ++i) {
     std::pair<int64_t, int64_t> dim[3] = {
@@ -532,6 +534,11 @@ extern "C" int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_appen
   if (a.k_token_stride < 0 || a.k_head_stride < 0 || a.v_token_stride < 0 ||
       a.v_head_stride < 0 || (a.q && (a.q_token_stride < 0 || a.q_head_stride < 0)))
     return set_error(TS_INVALID_ARGUMENT, "strides must be non-negative");
+  const uint64_t weights = a.q_weight | a.k_weight;
+  if ((a.k | a.v | a.q | (a.q ? a.q_out : 0)) % 2 || (a.slots | (a.cos_sin ? a.positions : 0)) % 8 ||
+      a.cos_sin % 4 || weights % (a.weight_dtype == TS_DTYPE_F32 ? 4 : 2) ||
+      reinterpret_cast<uintptr_t>(err_flag) % 4)
+    return set_error(TS_INVALID_ARGUMENT, "an address is not aligned to its elements");
   const int64_t d = kv->head_dim;
   const tsb::Extent ek = tsb::extent(a.k, a.tokens, a.k_token_stride, kv->heads,
                                      a.k_head_stride, 1, 0, d);

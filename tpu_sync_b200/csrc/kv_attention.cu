@@ -1386,6 +1386,10 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
       return set_error(TS_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
   if (kv->k_ptr % 16 || kv->v_ptr % 16 || a.q % 16 || a.out % 16)
     return set_error(TS_INVALID_ARGUMENT, "pages, queries and output must be 16-byte aligned");
+  if ((a.lse | a.seq_lens | a.prefix_len_dev | (a.max_blocks > 0 ? a.block_table : 0) |
+       (a.prefix_blocks > 0 ? a.prefix_table : 0)) % 4 ||
+      reinterpret_cast<uintptr_t>(err_flag) % 4)
+    return set_error(TS_INVALID_ARGUMENT, "an address is not aligned to its elements");
   const tsb::Extent eq = tsb::extent(a.q, a.batch, a.q_batch_stride, a.new_tokens,
                                      a.q_token_stride, a.q_heads, a.q_head_stride, kv->head_dim);
   const tsb::Extent eo{a.out, a.out + uint64_t(a.batch * a.new_tokens * a.q_heads *
