@@ -677,7 +677,7 @@ typedef struct ts_paged_kv {
 typedef struct ts_kv_append_args {
   uint64_t k, v;       /* [tokens, heads, head_dim], the storages' dtype */
   uint64_t q;          /* [tokens, q_heads, head_dim], or 0: no queries */
-  uint64_t q_out;      /* [tokens, q_heads, head_dim]; may be q itself, never k or v */
+  uint64_t q_out;      /* [tokens, q_heads, head_dim]; q itself, or apart from q, k and v */
   int64_t k_token_stride, k_head_stride;
   int64_t v_token_stride, v_head_stride;
   int64_t q_token_stride, q_head_stride;

@@ -196,3 +196,26 @@ def test_unaligned_addresses_are_refused():
   assert lib.ts_paged_attention(0, ctypes.byref(kv()), ctypes.byref(attention_args()), 13 * BASE,
                                 1 << 40, flag, None) == _native.INVALID_ARGUMENT
   assert "aligned" in _native.last_error()
+
+
+# Queries rotated in place whose elements are also keys' or values' (reads of one
+# race with writes of the other): by heads, by rows, by a part of a head.
+SHARED_IN_PLACE = [
+    dict(k=6 * BASE + 2 * 256, k_token_stride=512),             # heads 2 and 3 of q
+    dict(v=6 * BASE + 2 * 384, v_token_stride=512),             # heads 3 and 4: one is q's
+    dict(k=6 * BASE + 2 * 512),                                  # q's next row
+    dict(v=6 * BASE + 2 * 511, v_token_stride=768, q_token_stride=768, q_out_token_stride=768),
+    dict(k=6 * BASE - 2 * 255, k_token_stride=768, q_token_stride=768, q_out_token_stride=768),
+    # heads of [token, head, 3, 128]: k one element too early
+    dict(k=6 * BASE + 2 * 127, k_head_stride=384, k_token_stride=1536, q_head_stride=384,
+         q_token_stride=1536, q_out_head_stride=384, q_out_token_stride=1536),
+    # heads before tokens: k is q's last head and one more
+    dict(k=6 * BASE + 2 * 3 * 384, k_head_stride=384, k_token_stride=128, q_head_stride=384,
+         q_token_stride=128, q_out_head_stride=384, q_out_token_stride=128),
+]
+
+
+@pytest.mark.parametrize("over", SHARED_IN_PLACE, ids=str)
+def test_in_place_queries_that_are_keys_or_values(over):
+  assert append(kv(), append_args(q_out=6 * BASE, **over)) == _native.INVALID_ARGUMENT
+  assert "q itself" in _native.last_error()

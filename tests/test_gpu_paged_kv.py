@@ -901,3 +901,43 @@ def test_flag_in_mapped_host_memory(cuda):
                                       None) == _native.OK
     torch.cuda.synchronize()
     assert int(flag) == now
+
+
+# -- queries written beside or over their projections --------------------------
+
+
+@pytest.mark.parametrize("layout", ["rows", "heads", "grouped", "head first", "one token"])
+@pytest.mark.parametrize("out", ["itself", "columns"])
+def test_append_within_one_buffer(cuda, layout, out):
+  """Parts of one projection in any order of its dimensions are apart: queries are rewritten in
+  place, or into columns of their own, and keys and values are read as they were."""
+  g = gen(41)
+  t, h, d = (1 if layout == "one token" else 37), 4, 64
+  if layout in ("rows", "one token"):  # [t, (q, k, v, out) of h heads]
+    buf = rand(g, t, 4 * h, d, dtype=BF)
+    q, k, v, spare = (buf[:, i * h:(i + 1) * h] for i in range(4))
+  elif layout == "heads":  # [t, h, (q, k, v, out)]
+    buf = rand(g, t, h, 4, d, dtype=BF)
+    q, k, v, spare = (buf[:, :, i] for i in range(4))
+  elif layout == "grouped":  # two query heads to a KV head, side by side in its group
+    buf = rand(g, t, 2, 6, d, dtype=BF)
+    q, k, v, spare = buf[:, :, 0], buf[:, :, 2], buf[:, :, 3], buf[:, :, 4]
+  else:
+    buf = rand(g, 4 * h, t, d, dtype=BF).transpose(0, 1)
+    q, k, v, spare = (buf[:, i * h:(i + 1) * h] for i in range(4))
+  kp = torch.zeros(4, 16, k.shape[1], d, dtype=BF, device="cuda")
+  kv = ops.PagedKV(kp, torch.zeros_like(kp))
+  slots = torch.randperm(64, generator=g, device="cuda")[:t]
+  pos = torch.arange(t, device="cuda")
+  table = rotation_table(t, d)
+  q0, k0, v0 = q.clone(), k.clone(), v.clone()
+  got = ops.kv_append(kv, k, v, slots, q=q, positions=pos, cos_sin=table,
+                      q_out=q if out == "itself" else spare)
+  want, big = want_head(q0, None, 0, table, False)
+  assert close(got, want, big, BF)
+  want, big = want_head(k0, None, 0, table, False)
+  assert close(kp.view(64, -1, d)[slots], want, big, BF)
+  assert torch.equal(kv.v_pages.view(64, -1, d)[slots], v0)
+  assert torch.equal(k, k0) and torch.equal(v, v0)
+  if out == "columns":
+    assert torch.equal(q, q0)

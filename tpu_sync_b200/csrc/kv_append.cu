@@ -545,6 +545,9 @@ extern "C" int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_appen
   const tsb::Extent ev = tsb::extent(a.v, a.tokens, a.v_token_stride, kv->heads,
                                      a.v_head_stride, 1, 0, d);
   tsb::Extent eq{0, 0}, eo{0, 0};
+  auto heads_of = [&](uint64_t base, int64_t heads, int64_t token, int64_t head) {
+    return tsb::Strided{base, {a.tokens, heads, 1}, {token, head, 0}, d};
+  };
   if (a.q) {
     eq = tsb::extent(a.q, a.tokens, a.q_token_stride, a.q_heads, a.q_head_stride, 1, 0, d);
     eo = tsb::extent(a.q_out, a.tokens, a.q_out_token_stride, a.q_heads, a.q_out_head_stride, 1,
@@ -558,12 +561,15 @@ extern "C" int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_appen
       return set_error(TS_INVALID_ARGUMENT, "q_out strides overlap");
     const bool in_place = a.q == a.q_out && a.q_token_stride == a.q_out_token_stride &&
                           a.q_head_stride == a.q_out_head_stride;
-    // Projections in one buffer interleave rows: q_out inside that buffer is
-    // told from an overlap only when it is q itself; q that is also k or v would
-    // be overwritten while other warps read it as those.
-    const bool apart = in_place ? a.q != a.k && a.q != a.v
-                                : !(eo.meets(eq) || eo.meets(ek) || eo.meets(ev));
-    if (!apart)
+    // The parts of one projection interleave rows and may be apart all the same.
+    // A q_out that shares elements with k or v would be written while other
+    // warps read those, with q too unless each head is rewritten where it lies.
+    const tsb::Strided out = heads_of(a.q_out, a.q_heads, a.q_out_token_stride,
+                                      a.q_out_head_stride);
+    if (tsb::share_elements(out, heads_of(a.k, kv->heads, a.k_token_stride, a.k_head_stride)) ||
+        tsb::share_elements(out, heads_of(a.v, kv->heads, a.v_token_stride, a.v_head_stride)) ||
+        (!in_place && tsb::share_elements(out, heads_of(a.q, a.q_heads, a.q_token_stride,
+                                                        a.q_head_stride))))
       return set_error(TS_INVALID_ARGUMENT, "q_out must be q itself or apart from the new tokens");
   }
   for (int i = 0; i < 2; ++i) {

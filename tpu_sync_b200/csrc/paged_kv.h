@@ -52,6 +52,74 @@ inline Extent extent(uint64_t base, int64_t n0, int64_t s0, int64_t n1, int64_t 
   const Wide hi = Wide(base) + last * 2;
   return {base, hi > UINT64_MAX ? UINT64_MAX : uint64_t(hi)};
 }
+
+// A tensor [n0, n1, n2, d] of 2-byte elements (strides in elements, the last
+// dimension contiguous), for telling whether two share an element.
+struct Strided {
+  uint64_t base;
+  int64_t count[3], stride[3];
+  int64_t d;
+};
+using Wide = __int128;
+struct StridedPair {
+  int n;  // dimensions that both step over, largest stride first
+  Wide stride[3], a[3], b[3], len_a, len_b;
+  // b's first element lies `at` elements behind a's; the dimensions before `k`
+  // are settled.  The strides are nested, so only two index differences can
+  // bring the rest together.
+  bool meet(int k, Wide at) const {
+    if (k == n) return at < len_a && at + len_b > 0;
+    Wide r = at % stride[k];
+    if (r < 0) r += stride[k];
+    const Wide j = (r - at) / stride[k];  // index of b less index of a
+    return (j > -a[k] && j < b[k] && meet(k + 1, r)) ||
+           (j - 1 > -a[k] && j - 1 < b[k] && meet(k + 1, r - stride[k]));
+  }
+};
+// Whether a and b share an element.  Exact where both step by the same strides
+// and those are nested, as for the parts of one projection or one joint cache,
+// with the inner dimensions taken as one run of elements if need be; else by
+// the address ranges, which then may say yes to tensors that only interleave.
+inline bool share_elements(const Strided& a, const Strided& b) {
+  auto range = [](const Strided& t) {
+    return extent(t.base, t.count[0], t.stride[0], t.count[1], t.stride[1], t.count[2],
+                  t.stride[2], t.d);
+  };
+  if (!range(a).meets(range(b))) return false;
+  if (a.base % 2 != b.base % 2) return true;
+  for (int dims = 3; dims >= 1; --dims) {  // the first `dims` are stepped over
+    StridedPair p{};
+    p.len_a = a.d;
+    p.len_b = b.d;
+    bool same = true;
+    for (int i = 0; i < 3; ++i) {
+      if (i >= dims) {
+        p.len_a += Wide(a.count[i] - 1) * a.stride[i];
+        p.len_b += Wide(b.count[i] - 1) * b.stride[i];
+      } else if (a.count[i] > 1 || b.count[i] > 1) {
+        same = same && (a.count[i] == 1 || b.count[i] == 1 || a.stride[i] == b.stride[i]);
+        int at = p.n++;
+        const Wide stride = a.count[i] > 1 ? a.stride[i] : b.stride[i];
+        for (; at > 0 && p.stride[at - 1] < stride; --at) {
+          p.stride[at] = p.stride[at - 1];
+          p.a[at] = p.a[at - 1];
+          p.b[at] = p.b[at - 1];
+        }
+        p.stride[at] = stride;
+        p.a[at] = a.count[i];
+        p.b[at] = b.count[i];
+      }
+    }
+    Wide span_a = p.len_a, span_b = p.len_b;
+    for (int k = p.n - 1; same && k >= 0; --k) {
+      same = p.stride[k] >= span_a && p.stride[k] >= span_b;
+      span_a += (p.a[k] - 1) * p.stride[k];
+      span_b += (p.b[k] - 1) * p.stride[k];
+    }
+    if (same && !p.meet(0, (Wide(b.base) - Wide(a.base)) / 2)) return false;
+  }
+  return true;
+}
 inline Extent pages_extent(const ts_paged_kv& kv, bool v) {
   return v ? extent(kv.v_ptr, kv.pages, kv.v_page_stride, kv.block_tokens, kv.v_token_stride,
                     kv.heads, kv.v_head_stride, kv.head_dim)

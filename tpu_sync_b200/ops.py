@@ -512,7 +512,8 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
   head by row positions[t] (int64), pairs (i, i + rotary/2), or (2i, 2i+1) if
   `interleaved`.  q_weight / k_weight [head_dim] (the pages' dtype or float32)
   apply x * weight / sqrt(mean(x^2) + eps) to every query / key head before the
-  rotation.  q_out may be q itself (not k or v); its padding rows stay as they were (a new
+  rotation.  q_out is q itself, or shares no element with q, k and v (other
+  columns of their buffer will do); its padding rows stay as they were (a new
   one has zeros there).
 
   The slots of one call are distinct: where two tokens name one slot, it is not
