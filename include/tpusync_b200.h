@@ -704,7 +704,8 @@ typedef struct ts_kv_append_args {
  * distinct; of tokens that name the same slot, the pieces of any may stay.
  * A slot past the storage or a position outside the table writes nothing for
  * that token (its q_out row counts as padding) and sets *err_flag (device or
- * host-mapped int, may be NULL) to 1.  New tokens must not overlap the pages. */
+ * host-mapped int, may be NULL) to 1.  New tokens must not overlap the pages,
+ * nor K pages V pages (views of a joint cache that interleave are apart). */
 TS_API int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_append_args* args,
                         int* err_flag, void* stream);
 

@@ -219,3 +219,21 @@ SHARED_IN_PLACE = [
 def test_in_place_queries_that_are_keys_or_values(over):
   assert append(kv(), append_args(q_out=6 * BASE, **over)) == _native.INVALID_ARGUMENT
   assert "q itself" in _native.last_error()
+
+
+# K and V pages that share elements: the two scatters of an append would race.
+SHARED_PAGES = [
+    dict(v_ptr=BASE), dict(v_ptr=BASE + 2 * 128), dict(v_ptr=BASE + 2 * 16 * 256),
+    dict(k_ptr=2 * BASE - 2 * (9 * 16 * 256 + 8 * 256)),
+    # [pages, 2, 16, 2, 128] with V a token early
+    dict(k_page_stride=8192, v_page_stride=8192, v_ptr=BASE + 2 * 15 * 256),
+    # [pages, 16, 2, 2 x 128] with V an element early
+    dict(v_ptr=BASE + 2 * 127, k_page_stride=8192, v_page_stride=8192, k_token_stride=512,
+         v_token_stride=512, k_head_stride=256, v_head_stride=256),
+]
+
+
+@pytest.mark.parametrize("over", SHARED_PAGES, ids=str)
+def test_append_refuses_pages_of_k_that_are_v(over):
+  assert append(kv(**over), append_args()) == _native.INVALID_ARGUMENT
+  assert "K and V pages overlap" in _native.last_error()

@@ -941,3 +941,27 @@ def test_append_within_one_buffer(cuda, layout, out):
   assert torch.equal(k, k0) and torch.equal(v, v0)
   if out == "columns":
     assert torch.equal(q, q0)
+
+
+@pytest.mark.parametrize("at", [0, 1, 2, 3])
+def test_append_into_joint_caches(cuda, at):
+  """K and V interleaved at any dimension of one tensor are apart; one tensor as both is
+  refused by the append, and may be read by the attention."""
+  g = gen(42)
+  shape = [4, 16, 2, 64]
+  joint = torch.zeros(*shape[:at], 2, *shape[at:], dtype=FP, device="cuda")
+  kp, vp = joint.select(at, 0), joint.select(at, 1)
+  k, v = rand(g, 9, 2, 64, dtype=FP), rand(g, 9, 2, 64, dtype=FP)
+  slots = torch.randperm(64, generator=g, device="cuda")[:9]
+  ops.kv_append(ops.PagedKV(kp, vp), k, v, slots)
+  assert torch.equal(kp[slots // 16, slots % 16], k)
+  assert torch.equal(vp[slots // 16, slots % 16], v)
+  one = ops.PagedKV(kp, kp)
+  with pytest.raises(_native.NativeError, match="overlap"):
+    ops.kv_append(one, k, v, slots)
+  if at == 1:
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([16], dtype=torch.int32, device="cuda")
+    q = rand(g, 1, 1, 4, 64, dtype=FP)
+    out, lse = ops.paged_attention(one, q, table, lens, return_lse=True)
+    check(out, lse, q, [[kp[0].double(), kp[0].double()]], None, [16], 2, FP)

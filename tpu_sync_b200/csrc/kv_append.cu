@@ -577,6 +577,13 @@ extern "C" int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_appen
     if (e.meets(ek) || e.meets(ev) || e.meets(eq) || e.meets(eo))
       return set_error(TS_INVALID_ARGUMENT, "new tokens overlap the pages");
   }
+  auto pages = [&](uint64_t base, int64_t page, int64_t token, int64_t head) {
+    return tsb::Strided{base, {kv->pages, kv->block_tokens, kv->heads}, {page, token, head}, d};
+  };
+  if (tsb::share_elements(
+          pages(kv->k_ptr, kv->k_page_stride, kv->k_token_stride, kv->k_head_stride),
+          pages(kv->v_ptr, kv->v_page_stride, kv->v_token_stride, kv->v_head_stride)))
+    return set_error(TS_INVALID_ARGUMENT, "K and V pages overlap");
   tsb::DeviceGuard g(device);
   tsb::AppendParams p{*kv, a, err_flag};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
