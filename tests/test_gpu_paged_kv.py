@@ -965,3 +965,23 @@ def test_append_into_joint_caches(cuda, at):
     q = rand(g, 1, 1, 4, 64, dtype=FP)
     out, lse = ops.paged_attention(one, q, table, lens, return_lse=True)
     check(out, lse, q, [[kp[0].double(), kp[0].double()]], None, [16], 2, FP)
+
+
+def test_a_prefix_is_not_dropped_unseen(cuda):
+  """No table is refused; a length on the device beside a table without blocks is cut to none,
+  with the flag."""
+  pools, table, lens_t, ptable, q, own, shared = build(43, BF, 4, 2, 64, 16, False, 1, [20, 3], 40)
+  kv = ops.PagedKV(*pools)
+  want = ops.paged_attention(kv, q, table, lens_t)
+  length = torch.zeros(1, dtype=torch.int32, device="cuda")
+  err = torch.zeros(1, dtype=torch.int32, device="cuda")
+  for n in (40, length):
+    with pytest.raises(ValueError, match="prefix_table"):
+      ops.shared_prefix_attention(kv, q, None, n, table, lens_t)
+  for n in (0, 1, 2 ** 31 - 1, -1):
+    length.fill_(n)
+    err.zero_()
+    out = ops.shared_prefix_attention(kv, q, ptable[:0], length, table, lens_t, err_flag=err)
+    assert torch.equal(out, want) and int(err) == int(n != 0)
+  with pytest.raises(ValueError, match="does not hold"):
+    ops.shared_prefix_attention(kv, q, ptable[:0], 1, table, lens_t)

@@ -1054,6 +1054,12 @@ __global__ void __launch_bounds__(128) join_cut_kernel(const __grid_constant__ W
   Lengths lens;
   const Cut cut = lens.read(p, false);
   const int heads = int(p.a.q_heads), n_new = int(p.a.new_tokens);
+  if (w == 0 && threadIdx.x == 0 && p.a.prefix_len_dev) {
+    // a prefix whose table has no block: any length is past it
+    bool bad;
+    prefix_tokens(p.kv, p.a, &bad);
+    if (bad) flag_left_out(p.err);
+  }
   for (int b = w; b < p.a.batch; b += gridDim.x) {
     bool ignore;
     if (tokens_of(p, b, &ignore) != 0) continue;

@@ -739,5 +739,7 @@ def shared_prefix_attention(kv: PagedKV, q: torch.Tensor, prefix_table: torch.Te
   prefix_len: an int, or one int32 on the device (cut to what the table holds,
   with err_flag set).
   """
+  if prefix_table is None:
+    raise ValueError("prefix_table is missing: paged_attention is the form without a prefix")
   return _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, out,
                     return_lse, err_flag, stream)
