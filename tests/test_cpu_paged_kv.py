@@ -237,3 +237,17 @@ SHARED_PAGES = [
 def test_append_refuses_pages_of_k_that_are_v(over):
   assert append(kv(**over), append_args()) == _native.INVALID_ARGUMENT
   assert "K and V pages overlap" in _native.last_error()
+
+
+def test_strides_whose_products_pass_64_bits():
+  """Overlaps hidden by a product that would wrap."""
+  # 3 heads 2^62 apart: the span of 2^63 + 128 is past the token stride, wrapped it was negative
+  over = dict(heads=3, k_head_stride=1 << 62, k_token_stride=(1 << 62) + 8, v_token_stride=384,
+              v_page_stride=16 * 384, k_page_stride=(1 << 62) + 16)
+  for rc in (append(kv(**over), append_args(q=0)),
+             attend(kv(**over), attention_args(q_heads=3))):
+    assert rc == _native.INVALID_ARGUMENT
+    assert "page strides overlap" in _native.last_error()
+  over = dict(q_heads=4, q_out_head_stride=1 << 62, q_out_token_stride=1 << 61)
+  assert append(kv(), append_args(**over)) == _native.INVALID_ARGUMENT
+  assert "q_out strides" in _native.last_error()

@@ -496,11 +496,11 @@ int check_paged_kv(const ts_paged_kv* kv) {
         {i ? kv->v_token_stride : kv->k_token_stride, kv->block_tokens},
         {i ? kv->v_head_stride : kv->k_head_stride, kv->heads}};
     std::sort(dim, dim + 3);
-    int64_t span = kv->head_dim;
+    Wide span = kv->head_dim;  // strides of a caller's own making must not wrap it
     for (const auto& x : dim) {
       if (x.second <= 1) continue;
       if (x.first < span) return set_error(TS_INVALID_ARGUMENT, "page strides overlap");
-      span += (x.second - 1) * x.first;
+      span += Wide(x.second - 1) * x.first;
     }
   }
   return TS_OK;
@@ -552,10 +552,13 @@ extern "C" int ts_kv_append(int device, const ts_paged_kv* kv, const ts_kv_appen
     eq = tsb::extent(a.q, a.tokens, a.q_token_stride, a.q_heads, a.q_head_stride, 1, 0, d);
     eo = tsb::extent(a.q_out, a.tokens, a.q_out_token_stride, a.q_heads, a.q_out_head_stride, 1,
                      0, d);
-    const bool rows = a.q_out_token_stride >= (a.q_heads - 1) * a.q_out_head_stride + d &&
-                      a.q_out_head_stride >= d;
-    const bool cols = a.q_out_head_stride >= (a.tokens - 1) * a.q_out_token_stride + d &&
-                      a.q_out_token_stride >= d;
+    using tsb::Wide;
+    const bool rows =
+        a.q_out_token_stride >= Wide(a.q_heads - 1) * a.q_out_head_stride + d &&
+        a.q_out_head_stride >= d;
+    const bool cols =
+        a.q_out_head_stride >= Wide(a.tokens - 1) * a.q_out_token_stride + d &&
+        a.q_out_token_stride >= d;
     if (!(rows || cols || (a.tokens == 1 && a.q_out_head_stride >= d) ||
           (a.q_heads == 1 && a.q_out_token_stride >= d) || (a.tokens == 1 && a.q_heads == 1)))
       return set_error(TS_INVALID_ARGUMENT, "q_out strides overlap");
