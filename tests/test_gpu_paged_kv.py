@@ -985,3 +985,25 @@ def test_a_prefix_is_not_dropped_unseen(cuda):
     assert torch.equal(out, want) and int(err) == int(n != 0)
   with pytest.raises(ValueError, match="does not hold"):
     ops.shared_prefix_attention(kv, q, ptable[:0], 1, table, lens_t)
+
+
+def test_no_pages(cuda):
+  """Storages of no pages: every token is left out, with the flag."""
+  kp = torch.zeros(0, 16, 2, 64, dtype=BF, device="cuda")
+  kv = ops.PagedKV(kp, kp.clone())
+  q = torch.ones(3, 2, 8, 64, dtype=BF, device="cuda")
+  table = torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+  lens = torch.tensor([5, 0, 64], dtype=torch.int32, device="cuda")
+  err = torch.zeros(1, dtype=torch.int32, device="cuda")
+  for prefix in (None, 20):
+    err.zero_()
+    if prefix is None:
+      out, lse = ops.paged_attention(kv, q, table, lens, return_lse=True, err_flag=err)
+    else:
+      out, lse = ops.shared_prefix_attention(kv, q, table[0], prefix, table, lens,
+                                             return_lse=True, err_flag=err)
+    assert (out == 0).all() and (lse == -math.inf).all() and int(err) == 1
+  err.zero_()
+  k = torch.ones(2, 2, 64, dtype=BF, device="cuda")
+  got = ops.kv_append(kv, k, k, torch.tensor([0, -1], device="cuda"), q=q[0], err_flag=err)
+  assert (got == 0).all() and int(err) == 1
