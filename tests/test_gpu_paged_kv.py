@@ -1007,3 +1007,32 @@ def test_no_pages(cuda):
   k = torch.ones(2, 2, 64, dtype=BF, device="cuda")
   got = ops.kv_append(kv, k, k, torch.tensor([0, -1], device="cuda"), q=q[0], err_flag=err)
   assert (got == 0).all() and int(err) == 1
+
+
+def test_tangents_are_refused(cuda):
+  """Forward-mode derivatives would be lost without a word."""
+  from torch.autograd import forward_ad as fwd
+  dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+  kp = torch.zeros(4, 16, 2, 64, dtype=BF, device="cuda")
+  kv = ops.PagedKV(kp, kp.clone())
+  q = torch.zeros(2, 8, 64, dtype=BF, device="cuda")
+  k = torch.zeros(2, 2, 64, dtype=BF, device="cuda")
+  table = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+  lens = torch.ones(2, dtype=torch.int32, device="cuda")
+  slots = torch.arange(2, device="cuda")
+  cs, w = torch.zeros(9, 64, device="cuda"), torch.ones(64, device="cuda")
+  with fwd.dual_level():
+    for grad in (torch.enable_grad, torch.no_grad):
+      with grad():
+        for call in (lambda: ops.paged_attention(kv, dual(q), table, lens),
+                     lambda: ops.shared_prefix_attention(kv, dual(q), table[0], 3, table, lens),
+                     lambda: ops.paged_attention(ops.PagedKV(kp, dual(kp.clone())), q, table, lens),
+                     lambda: ops.kv_append(kv, dual(k), k, slots),
+                     lambda: ops.kv_append(kv, k, dual(k), slots),
+                     lambda: ops.kv_append(kv, k, k, slots, q=dual(q)),
+                     lambda: ops.kv_append(kv, k, k, slots, k_weight=dual(w)),
+                     lambda: ops.kv_append(kv, k, k, slots, positions=slots, cos_sin=dual(cs))):
+          with pytest.raises(ValueError, match="tangent"):
+            call()
+        ops.kv_append(kv, k, k, slots, q=q)  # without one they run
+        ops.paged_attention(kv, q, table, lens)

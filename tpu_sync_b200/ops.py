@@ -19,6 +19,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from tpu_sync_b200 import _native
 
@@ -486,6 +487,13 @@ def _no_grad_path() -> ValueError:
   return ValueError("an input requires grad: the paged cache operators have no backward pass")
 
 
+def _refuse_tangents(kv: PagedKV, *tensors: Optional[torch.Tensor]) -> None:
+  """The same for forward-mode derivatives (called only within a dual level)."""
+  for t in (kv.k_pages, kv.v_pages, *tensors):
+    if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+      raise ValueError("an input has a tangent: the paged cache operators have no derivatives")
+
+
 def _flag(kv: PagedKV, err_flag: Optional[torch.Tensor]) -> int:
   if err_flag is None:
     return 0
@@ -573,6 +581,8 @@ def kv_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor
       (q_weight is not None and q_weight.requires_grad) or
       (k_weight is not None and k_weight.requires_grad)):
     raise _no_grad_path()
+  if forward_ad._current_level >= 0:
+    _refuse_tangents(kv, k, v, q, q_out, cos_sin, q_weight, k_weight)
   q_ptr = out_ptr = heads = qt = qh = ot = oh = zero = 0
   if q is not None:
     heads = q.shape[1] if q.dim() == 3 else 0
@@ -652,6 +662,8 @@ def _attention(kv, q, block_table, seq_lens, prefix_table, prefix_len, scale, ou
       raise ValueError("out must be contiguous")
   if torch.is_grad_enabled() and (q.requires_grad or (out is not None and out.requires_grad)):
     raise _no_grad_path()
+  if forward_ad._current_level >= 0:
+    _refuse_tangents(kv, q, out)
   lib = _native.lib()
 
   # a dimension of one element is never stepped over: its stride says nothing
