@@ -1036,3 +1036,122 @@ def test_tangents_are_refused(cuda):
             call()
         ops.kv_append(kv, k, k, slots, q=q)  # without one they run
         ops.paged_attention(kv, q, table, lens)
+
+
+# -- more than drafts, other streams, lengths far below the table's -------------
+
+
+PROMPTS = [
+    # q heads, kv heads, d, block tokens, head major, new tokens, prefix, lengths
+    (8, 2, 128, 16, False, 6, None, [6, 3, 0, 100]),
+    (32, 8, 128, 16, False, 20, None, [20, 90]),         # 80 rows a KV head: three row tiles
+    (8, 2, 128, 16, False, 100, None, [100, 37, 0, 250]),
+    (4, 1, 64, 64, True, 257, None, [257, 300]),
+    (2, 1, 128, 5, False, 200, None, [200, 13]),
+    (8, 2, 128, 16, False, 70, 200, [70, 3, 90]),        # the rest of a prompt behind a prefix
+    (4, 2, 64, 16, False, 150, 1000, [150, 151]),
+]
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("case", PROMPTS, ids=str)
+def test_many_new_tokens(cuda, case, dt):
+  hq, hk, d, bt, major, n, prefix, lens = case
+  pools, table, lens_t, ptable, q, own, shared = build(51, dt, hq, hk, d, bt, major, n, lens,
+                                                       prefix)
+  kv = ops.PagedKV(*pools, head_major=major)
+  if prefix is None:
+    out, lse = ops.paged_attention(kv, q, table, lens_t, return_lse=True)
+  else:
+    out, lse = ops.shared_prefix_attention(kv, q, ptable, prefix, table, lens_t, return_lse=True)
+  check(out, lse, q, own, shared, lens, hk, dt)
+
+
+@pytest.mark.parametrize("hq,hk,count", [(8, 2, 33), (8, 1, 70)])
+def test_replayed_prefix_lengths_far_below_the_table(cuda, hq, hk, count):
+  """A captured call of many rows, planned by a table of 4096 tokens, replayed with any length:
+  fewer units of work than CTAs were launched for, and none."""
+  lens = [(7 * i) % 60 for i in range(count)]
+  pools, table, lens_t, ptable, q, own, shared = build(52, BF, hq, hk, 128, 16, False, 1, lens,
+                                                       4096)
+  kv = ops.PagedKV(*pools)
+  plen = torch.tensor([4096], dtype=torch.int32, device="cuda")
+  err = torch.zeros(1, dtype=torch.int32, device="cuda")
+  ops.shared_prefix_attention(kv, q, ptable, plen, table, lens_t, return_lse=True)
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    out, lse = ops.shared_prefix_attention(kv, q, ptable, plen, table, lens_t, return_lse=True,
+                                           err_flag=err)
+  for p in (0, 1, 129, 4096, 127, 2000):
+    for new in (lens, [0] * count, [x // 2 for x in lens]):
+      lens_t.copy_(torch.tensor(new, dtype=torch.int32))
+      plen.fill_(p)
+      graph.replay()
+      torch.cuda.synchronize()
+      check(out, lse, q, own, [x[:p] for x in shared], new, hk, BF)
+  assert int(err) == 0
+
+
+@pytest.mark.parametrize("d", [64, 72])
+def test_append_on_a_given_stream(cuda, d):
+  """The append is ordered on the stream it is given, and allocates there."""
+  g = gen(53)
+  kp = torch.zeros(8, 16, 2, d, dtype=BF, device="cuda")
+  kv = ops.PagedKV(kp, torch.zeros_like(kp))
+  k, v, q = (rand(g, 50, h, d, dtype=BF) for h in (2, 2, 6))
+  late = [torch.zeros_like(x) for x in (k, v, q)]
+  slots = torch.randperm(128, generator=g, device="cuda")[:50]
+  s = torch.cuda.Stream()
+  s.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(s):
+    torch.cuda._sleep(20_000_000)
+    for to, x in zip(late, (k, v, q)):
+      to.copy_(x)
+  got = ops.kv_append(kv, late[0], late[1], slots, q=late[2], stream=s)
+  s.synchronize()
+  assert torch.equal(got, q)
+  assert torch.equal(kp.view(128, 2, d)[slots], k)
+  assert torch.equal(kv.v_pages.view(128, 2, d)[slots], v)
+
+
+@pytest.mark.parametrize("hq,prefix,count", [(4, None, 3), (4, 300, 3), (8, 700, 40)],
+                         ids=["own", "walked prefix", "many rows"])
+def test_visible_values_that_are_not_finite(cuda, hq, prefix, count):
+  """They reach exactly the rows and elements that the definition says: a NaN in K every element
+  of its KV head's rows, an infinity in K the rows whose score becomes +infinity (at -infinity
+  the key has no weight), one in V its element."""
+  lens = [40 + i for i in range(count)]
+  pools, table, lens_t, ptable, q, own, shared = build(54, BF, hq, 2, 128, 16, False, 1, lens,
+                                                       prefix)
+  kv = ops.PagedKV(*pools)
+
+  def put(pool, i, t, head, e, value):  # sequence i, or the prefix: None
+    pages, copy = (table[i], own[i]) if i is not None else (ptable, shared)
+    pools[pool][int(pages[t // 16]), t % 16, head, e] = value
+    copy[pool][t, head, e] = value
+
+  where = None if prefix else 1
+  put(0, 0, 5, 0, 3, math.nan)
+  put(1, 1, 39, 1, 7, math.inf)
+  put(0, 2, 17, 1, 11, math.inf)
+  put(0, where, 30, 1, 100, -math.inf)
+  put(1, where, 31, 0, 64, math.nan)
+  if prefix is None:
+    out, lse = ops.paged_attention(kv, q, table, lens_t, return_lse=True)
+  else:
+    out, lse = ops.shared_prefix_attention(kv, q, ptable, prefix, table, lens_t, return_lse=True)
+  g = hq // 2
+  for i in range(count):
+    k, v = own[i]
+    if prefix:
+      k, v = torch.cat([shared[0], k]), torch.cat([shared[1], v])
+    x = torch.einsum("hgd,thd->hgt", q[i, 0].double().view(2, g, 128), k) * 128 ** -0.5
+    p = torch.softmax(x, -1)  # NaN where a score is NaN or +infinity
+    fine = torch.isfinite(v).all(0)[:, None] & torch.isfinite(p).all(-1, keepdim=True)
+    want = torch.einsum("hgt,thd->hgd", p, torch.where(torch.isfinite(v), v, 0.0))
+    size = torch.einsum("hgt,thd->hgd", p, torch.where(torch.isfinite(v), v, 0.0).abs())
+    tol = U[BF] * (size + want.abs()) + 2.0 ** -15 * size
+    got = out[i, 0].double().view(2, g, 128)
+    assert bool(((got - want).abs() <= tol)[fine].all()), i
+    assert not bool(torch.isfinite(got)[~fine].any()), i
