@@ -466,9 +466,9 @@ struct Loader {
         const int64_t kr = __shfl_sync(~0u, ko, r), vr = __shfl_sync(~0u, vo, r);
         const bool in = (mask >> r) & 1;
         const uint32_t to = (c / 8) * kBlock + r * 128 + (((c % 8) ^ (r & 7)) << 4);
-        // a source that is not read still is an address: there may be no pages
-        cp_async16(kdst + to, in ? kp + kr + c * 8 : reinterpret_cast<const T*>(p.a.q), in);
-        cp_async16(vdst + to, in ? vp + vr + c * 8 : reinterpret_cast<const T*>(p.a.q), in);
+        // a source that is not read still is an address of the pages
+        cp_async16(kdst + to, in ? kp + kr + c * 8 : reinterpret_cast<const T*>(p.kv.k_ptr), in);
+        cp_async16(vdst + to, in ? vp + vr + c * 8 : reinterpret_cast<const T*>(p.kv.v_ptr), in);
       }
       cp_commit();
     }
@@ -1409,6 +1409,7 @@ extern "C" int ts_paged_attention(int device, const ts_paged_kv* kv,
   tsb::DeviceGuard g(device);
   tsb::WalkParams p{};
   p.kv = *kv;
+  if (kv->pages == 0) p.kv.k_ptr = p.kv.v_ptr = a.q;  // the source of copies of 0 bytes
   p.a = a;
   p.scale_log2 = a.scale * tsb::kLog2e;
   p.group = int(a.q_heads / kv->heads);
