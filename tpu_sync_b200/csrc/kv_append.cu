@@ -8,11 +8,13 @@
 //                                                  elements, optional)
 // and the result goes to q_out, or to page slot / block_tokens at offset
 // slot % block_tokens.  Everything is read once and written once with a
-// handful of operations per element: bound by HBM for prompts, by one chain of
-// dependent loads (position -> table row) for decode steps.
+// handful of operations per element: bound by instruction issue, next to HBM, for
+// prompts, by one chain of dependent loads (position -> table row) for decode
+// steps.
 //
 // Measured (32 query and 8 KV heads of 128, bf16): 8192 tokens with norms 37 us
-// for 206 MB (5.6 TB/s, 0.85 of a plain copy); a step of 8 tokens 4 us, of 256
+// for 206 MB (5.6 TB/s, 0.85 of a plain copy; 0.78 instructions a scheduler and
+// cycle, 4.0 TB/s seen by DRAM as half of it stays in L2); a step of 8 tokens 4 us, of 256
 // tokens with norms (8 and 1 heads) 4.3 us; a padded prompt of 1531 tokens (32
 // and 8 heads of 64) 6 us.
 
@@ -74,7 +76,9 @@ __device__ __forceinline__ float weight_at(uint64_t w, int f32, int e) {
 }
 
 // Any head size, alignment and stride: a warp per (token, head), a lane per
-// pair.  Serves what the vector kernel's rule leaves out.
+// pair.  Serves what the vector kernel's rule leaves out (heads of 80 or 96
+// elements, views at odd addresses), with loads of one element, as nothing wider
+// is aligned there: four times the vector kernel's time on work both can do.
 template <typename T>
 __global__ void __launch_bounds__(256) append_any_kernel(const __grid_constant__ AppendParams p) {
   const int lane = threadIdx.x & 31;

@@ -24,16 +24,20 @@
 // new tokens, are columns of the same products, up to 32: K and V are read
 // once for them.
 //
-// Bound: decode reads K and V from HBM, 436 us for 2.94 GB (128 sequences of
-// 3001..8192 tokens, 8 KV heads of 128: 6.7 TB/s, all of a plain copy's rate),
-// 91 us for 0.54 GB (64 of 17..4096).  Short batches are bound by chains of
-// latency: about 4 us from the lengths to the first tile, 0.8 us a tile in each
-// CTA, 4 us to the joined rows (one sequence of 8191 tokens 11 us of walk and 4
-// of join).  More than 16 rows are bound by the instructions of the products
-// and the softmax: 64 x 4000 tokens of one KV head 33, 38, 44 and 63 us for 8,
-// 16, 24 and 32 rows (at 32 some registers spill).  mma.sync is used and not
-// tcgen05: eight to 32 rows would fill a fraction of a 128-row tile, and the
-// products are not what bounds the common case.
+// Bound: decode reads K and V from HBM, 427 to 437 us for 2.94 GB (128 sequences
+// of 3001..8192 tokens, 8 KV heads of 128: 6.7 to 6.9 TB/s, where a kernel that
+// only reads reaches 7.2), 90 to 92 us for 0.54 GB (64 of 17..4096).  Short
+// batches are bound by chains of latency: about 4 us from the lengths to the
+// first tile, 0.8 us a tile in each CTA, 3 to 4 us from the walk's end to the
+// joined rows (one sequence of 8191 tokens: 9.9 us of walk, 13.1 in all).  More
+// than 16 rows are bound by the instructions of the products and the softmax: 64
+// x 4000 tokens of one KV head 30, 37, 44 and 61 us for 8, 16, 24 and 32 rows (at
+// 32 some registers spill).  mma.sync is used and not tcgen05: up to 16 rows the
+// products do not bound it.  Beyond, tokens could be the 128 rows of a tcgen05
+// tile as they are the rows here, with the sums out of registers; that is not
+// built.  Prompts (hundreds of new tokens) are correct and slow: every row tile
+// of 32 walks all tiles of its sequence, also those it does not see (4096 tokens
+// of 32 and 8 heads 1.9 ms, where the visible products need 0.08).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -772,9 +776,9 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
       }
       // Lanes compare notes and sums are rescaled only in tiles that raise a
       // row's maximum.  m may be any common reference: with 32 rows it follows
-      // only by steps of 2^8 (few tiles raise none; 64 x 4000 tokens 287 -> 248
-      // us), with fewer at once, as the largest weight is then exactly 1 and
-      // loses nothing when it is rounded.
+      // only by steps of 2^8 (few tiles raise none; 64 x 4000 tokens of 8 KV heads
+      // 287 -> 247 us, of one 64.5 -> 61.7), with fewer at once, as the largest
+      // weight is then exactly 1 and loses nothing when it is rounded.
       if (__any_sync(~0u, grew)) {
 #pragma unroll
         for (int nt = 0; nt < kNt; ++nt) {
@@ -1252,6 +1256,10 @@ struct Layout {
 //   16 rows x 8 KV heads: 18 / 26 at 8192 keys, 36 / 41 at 32768
 //   48 rows: 27 / 28 at 8192, 57 / 44 at 32768;  64 rows: 21 / 26, 34 / 28, 76 / 47
 //   128 rows: 30 / 28 at 1000, 53 / 30 at 8192 (1 KV head: 18 / 27, 23 / 26)
+// The rule is for several KV heads; one head alone with up to a few hundred rows
+// and a short prefix pays up to 10 us for it (16 sequences of 8 query heads behind
+// 1000 keys 14 us, 24 of them, past 128 rows, 27).  A length on the device is
+// planned for as what the table holds.
 bool prefix_on_tensor_cores(const ts_paged_kv& kv, const ts_attention_args& a) {
   if (a.prefix_blocks == 0 || !prefix_geometry_ok(kv)) return false;
   const int64_t rows = a.batch * a.new_tokens * (a.q_heads / kv.heads);

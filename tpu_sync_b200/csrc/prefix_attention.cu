@@ -29,8 +29,8 @@
 // anything there); table entries outside the pages load as zeros through TMA's
 // bounds and are masked.
 //
-// Every wait is bounded: on running out it raises the flag (value 2), and all
-// roles leave.
+// Every wait is bounded (about 2 s): on running out it raises the flag (value 2),
+// all roles leave, and the rows of the CTA's share become NaN.
 //
 // Bound: 1024 rows x 8 KV heads x 32768 keys x 128 (137 GFLOP) take 124 us, 1.1
 // PFLOP/s: 67% of a large cuBLAS product's burst rate, 80% of its sustained one.

@@ -716,11 +716,13 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, block_table: torch.Tensor,
   """Attention of each sequence's last tokens over its pages.
 
   q: [batch, q_heads, head_dim], or [batch, n, q_heads, head_dim] for the last
-  n tokens of each sequence (drafted tokens); query head h reads KV head
+  n tokens of each sequence.  It is made for drafted tokens: a prompt is
+  answered as well, but at tens of times what its products need (4096 tokens
+  1.9 ms a layer).  Query head h reads KV head
   h / (q_heads / heads).  block_table: int32 [batch, max_blocks], the pages of
   a sequence in order; seq_lens: int32 [batch], its tokens in the cache, the
   new ones included.  Query j sees the first seq_len - n + 1 + j tokens; one
-  that sees none gets zeros.  scale: default head_dim ** -0.5.  With
+  that sees none gets zeros, and none depends on a token it does not see.  scale: default head_dim ** -0.5.  With
   return_lse also returns float32 log(sum(exp(scores))) per query head (-inf
   for a query that sees nothing).  head_dim is 64 or 128.
 
@@ -749,7 +751,10 @@ def shared_prefix_attention(kv: PagedKV, q: torch.Tensor, prefix_table: torch.Te
   sequence's own tokens as in paged_attention: block_table and seq_lens count
   the tokens after the prefix (a sequence with none sees the prefix alone).
   prefix_len: an int, or one int32 on the device (cut to what the table holds,
-  with err_flag set).
+  with err_flag set).  With a length on the device the kernels and their CTAs
+  are chosen for all that the table holds: give a table about as long as the
+  prefix.  Pages whose size is no multiple of 8 tokens keep a prefix of many
+  rows off the tensor cores of the fifth generation (four times slower).
   """
   if prefix_table is None:
     raise ValueError("prefix_table is missing: paged_attention is the form without a prefix")
