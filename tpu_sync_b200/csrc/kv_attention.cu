@@ -489,21 +489,25 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// kPer elements (8 or 4, aligned to as many) in 32 bits.
+// kPer elements (8 or 4, aligned to as many), and the same in 32 bits.
 template <typename T, int kPer>
-__device__ __forceinline__ void load_f32(const T* src, float* f) {
-  uint32_t w[kPer / 2];
-  if constexpr (kPer == 8)
-    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
-  else
-    *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
-#pragma unroll
-  for (int i = 0; i < kPer / 2; ++i) {
-    const float2 x = Ops<T>::unpack(w[i]);
-    f[2 * i] = x.x;
-    f[2 * i + 1] = x.y;
+struct Piece {
+  uint32_t w[kPer / 2] = {};
+  __device__ __forceinline__ void load(const T* src) {
+    if constexpr (kPer == 8)
+      *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
+    else
+      *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
   }
-}
+  __device__ __forceinline__ void to_f32(float* f) const {
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) {
+      const float2 x = Ops<T>::unpack(w[i]);
+      f[2 * i] = x.x;
+      f[2 * i + 1] = x.y;
+    }
+  }
+};
 template <int kPer>
 __device__ __forceinline__ bool all_finite(const float* f) {
   float zero = 0.f;
@@ -554,11 +558,13 @@ __device__ __forceinline__ void put_row(const WalkParams& p, const Cursor& c, in
 // and 0 times an infinity or a NaN in their V is NaN.  Where a CTA of the walk
 // met sums that are not finite, this computes all rows of its share again, in 32
 // bits, that have such a neighbour, from what they see; 16 threads a row, the
-// ones that wrote it.  Only those batches pay for it (the others under 1%: 64 x
-// 4000 tokens of 32 rows 60.3 -> 60.4 us); a look at V of partly seen tiles in
-// the walk's loop cost walks of 16 and more rows 5 to 9%.
+// ones that wrote it.  Those batches pay for it (24 x 4 drafts with an infinity in
+// each last one 20 -> 198 us, a prompt of 4096 tokens 1.9 -> 41 ms), the others
+// hardly (64 x 4000 tokens, 8 to 32 rows: 1 to 4%, 0.3 to 1.6 us); a look at V of
+// partly seen tiles in the walk's loop cost all walks of 16 and more rows 5 to 9%.
+constexpr int kRedoTokens = 4;  // tokens whose loads are under way at once
 template <typename T, int D, int kRows>
-__device__ __forceinline__ void redo_rows(const WalkParams& p) {
+__device__ __forceinline__ void redo_rows(const WalkParams& p, int* far) {
   constexpr int kPer = D / 16;
   const unsigned lanes = 0xffffu << (threadIdx.x & 16);  // of this thread's row
   const int at = (threadIdx.x & 15) * kPer, bt = int(p.kv.block_tokens);
@@ -566,49 +572,86 @@ __device__ __forceinline__ void redo_rows(const WalkParams& p) {
     const int32_t* table =
         reinterpret_cast<const int32_t*>(p.a.block_table) + c.b * p.a.block_table_stride;
     const int tile0 = c.tile * kTile, last = min(c.len, c.end * kTile);
-    // elements [at, at + kPer) of K or V of a token; false where its page is none
-    auto load = [&](bool v, int t, float* f) {
-      const int64_t page = table[t / bt], off = t % bt;
-      if (page < 0 || page >= p.kv.pages) return false;
-      load_f32<T, kPer>(
-          reinterpret_cast<const T*>(v ? p.kv.v_ptr : p.kv.k_ptr) + at +
-              page * (v ? p.kv.v_page_stride : p.kv.k_page_stride) +
-              off * (v ? p.kv.v_token_stride : p.kv.k_token_stride) +
-              c.head * (v ? p.kv.v_head_stride : p.kv.k_head_stride),
-          f);
-      return true;
-    };
+    const T* kp = reinterpret_cast<const T*>(p.kv.k_ptr) + c.head * p.kv.k_head_stride + at;
+    const T* vp = reinterpret_cast<const T*>(p.kv.v_ptr) + c.head * p.kv.v_head_stride + at;
+    // the last token of the share with such a value: all threads, a token to 16
+    __syncthreads();
+    if (threadIdx.x == 0) *far = -1;
+    __syncthreads();
+    for (int t = max(max(c.len - int(p.a.new_tokens) + 1, tile0), 0) + int(threadIdx.x >> 4);
+         t < last; t += kWarps * 2) {
+      const int64_t page = table[t / bt];
+      if (page < 0 || page >= p.kv.pages) continue;
+      Piece<T, kPer> v;
+      float f[kPer];
+      v.load(vp + page * p.kv.v_page_stride + t % bt * p.kv.v_token_stride);
+      v.to_f32(f);
+      if (!all_finite<kPer>(f)) atomicMax(far, t);
+    }
+    __syncthreads();
+    const int hidden = *far;
 #pragma unroll 1
     for (int r = threadIdx.x >> 4; r < min(kRows, p.rows_own - c.rt * kRows); r += 8) {
       const Row q = row_of(p, c.b, c.rt * kRows + r);
-      const int seen = min(last, c.len - int(p.a.new_tokens) + 1 + q.j);
-      bool hidden = false;
-#pragma unroll 1
-      for (int t = max(seen, tile0); t < last && !hidden; ++t) {
-        float v[kPer];
-        hidden = __any_sync(lanes, load(true, t, v) && !all_finite<kPer>(v));
-      }
-      if (!hidden) continue;
+      const int seen = max(min(last, c.len - int(p.a.new_tokens) + 1 + q.j), 0);
+      if (hidden < seen) continue;
       float qf[kPer], o[kPer] = {}, m = -INFINITY, l = 0.f;
-      load_f32<T, kPer>(reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
-                            q.j * p.a.q_token_stride +
-                            (c.head * p.group + q.g) * p.a.q_head_stride + at,
-                        qf);
+      {
+        Piece<T, kPer> query;
+        query.load(reinterpret_cast<const T*>(p.a.q) + q.b * p.a.q_batch_stride +
+                   q.j * p.a.q_token_stride + (c.head * p.group + q.g) * p.a.q_head_stride + at);
+        query.to_f32(qf);
+      }
 #pragma unroll 1
-      for (int t = tile0; t < seen; ++t) {
-        float k[kPer], v[kPer], x = 0.f;
-        if (!load(false, t, k) || !load(true, t, v)) continue;
+      for (int t0 = tile0; t0 < seen; t0 += kRedoTokens) {
+        Piece<T, kPer> k[kRedoTokens], v[kRedoTokens];
+        float x[kRedoTokens], dot[kRedoTokens] = {}, top = m;
+        // tokens that do not count are loaded from the first page with no weight
+        // (a load under a condition of its own would wait for the one before);
+        // there is one, as a value of some page brought the CTA here
+        int64_t page[kRedoTokens];
+        bool in[kRedoTokens];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x = fmaf(qf[i], k[i], x);
+        for (int u = 0; u < kRedoTokens; ++u) page[u] = table[min(t0 + u, seen - 1) / bt];
 #pragma unroll
-        for (int s = 8; s > 0; s >>= 1) x += __shfl_xor_sync(lanes, x, s);
-        x *= p.scale_log2;
-        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.f : top;
-        const float f = ex2(m - base), w = ex2(x - base);
+        for (int u = 0; u < kRedoTokens; ++u) {
+          in[u] = t0 + u < seen && page[u] >= 0 && page[u] < p.kv.pages;
+          const int64_t off = min(t0 + u, seen - 1) % bt;
+          if (!in[u]) page[u] = 0;
+          k[u].load(kp + page[u] * p.kv.k_page_stride + off * p.kv.k_token_stride);
+          v[u].load(vp + page[u] * p.kv.v_page_stride + off * p.kv.v_token_stride);
+        }
+#pragma unroll
+        for (int u = 0; u < kRedoTokens; ++u) {
+          float f[kPer];
+          k[u].to_f32(f);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) dot[u] = fmaf(qf[i], f[i], dot[u]);
+        }
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1)
+#pragma unroll
+          for (int u = 0; u < kRedoTokens; ++u) dot[u] += __shfl_xor_sync(lanes, dot[u], s);
+#pragma unroll
+        for (int u = 0; u < kRedoTokens; ++u) {
+          x[u] = in[u] ? dot[u] * p.scale_log2 : -INFINITY;
+          top = fmaxf(top, x[u]);
+        }
+        const float base = top == -INFINITY ? 0.f : top, f = ex2(m - base);
         m = top;
-        l = fmaf(l, f, w);
+        l *= f;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], f, w * v[i]);
+        for (int i = 0; i < kPer; ++i) o[i] *= f;
+#pragma unroll
+        for (int u = 0; u < kRedoTokens; ++u) {
+          float values[kPer];
+          v[u].to_f32(values);
+          const float w = ex2(x[u] - base);
+          l += w;
+          // what does not count may hold anything
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) o[i] = in[u] ? fmaf(w, values[i], o[i]) : o[i];
+        }
       }
       put_row<T, D, kRows>(p, c, r, at, o, m, l);
     }
@@ -637,7 +680,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
   const uint32_t bars = smem_u32(ctl) + warp * kStages * 8;
   uint32_t* masks = reinterpret_cast<uint32_t*>(ctl + kWarps * kStages * 8) + warp * kStages;
   volatile int* gone = reinterpret_cast<volatile int*>(ctl + kWarps * kStages * 12);
-  volatile int* odd = gone + 1;  // sums that are not finite were met
+  int* odd = reinterpret_cast<int*>(ctl + kWarps * kStages * 12 + 4);  // met: sums not finite
   if (threadIdx.x == 0) *gone = *odd = 0;
   if (kTma) {
     if (lane < kStages) bar_init(bars + 8 * lane, 1);
@@ -905,7 +948,7 @@ __global__ void __launch_bounds__(kWarps * 32, walk_bound(D, kNt))
     __syncthreads();  // the parts have been read: the stages may be refilled
     cu = next;
   }
-  if (p.a.new_tokens > 1 && *odd) redo_rows<T, D, kRows>(p);
+  if (p.a.new_tokens > 1 && *odd) redo_rows<T, D, kRows>(p, odd);
   if constexpr (kTma) {
     if (*gone) {
       // loads still in flight land before their shared memory is given back
